@@ -42,11 +42,17 @@ int64_t g_launches = 0;  // kernels of this extension launched so far (host-side
 int64_t launch_count() { return g_launches; }
 Tensor error_flag_tensor();
 
-Tensor g_error_flag;
-int* error_flag_ptr() {
-    if (!g_error_flag.defined()) g_error_flag = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA));
-    return g_error_flag.data_ptr<int>();
-}
+// One error word on each device that launched a kernel (a kernel must not write another device's memory); current() is the current device's.
+struct ErrorFlags {
+    std::vector<Tensor> on;
+    Tensor& current() {
+        const size_t d = static_cast<size_t>(at::cuda::current_device());
+        if (on.size() <= d) on.resize(d + 1);
+        if (!on[d].defined()) on[d] = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(d)));
+        return on[d];
+    }
+} g_error_flags;
+int* error_flag_ptr() { return g_error_flags.current().data_ptr<int>(); }
 
 // fmt: bf16 -> 1 ; float8_e4m3fn -> 0 ; float8_e5m2 -> 1 (uint8 tensors take the explicit *_fmt argument)
 int fp8_fmt_of(const Tensor& t, int64_t explicit_fmt) {
@@ -127,15 +133,17 @@ std::tuple<bool, int, int, int64_t> gemm_plan(int64_t M, int64_t N, int64_t K, i
     return {plan.pair != 0, plan.splits, plan.split_from, static_cast<int64_t>(4 * (plan.workspace_floats + (plan.splits > 1 ? plan.num_counters : 0)))};
 }
 
-Tensor error_flag_tensor() {
-    error_flag_ptr();
-    return g_error_flag;
-}
+Tensor error_flag_tensor() { return g_error_flags.current(); }
 
+// The first error word that is set, of all devices (synchronises)
 int64_t read_error_flag(bool reset) {
-    if (!g_error_flag.defined()) return 0;
-    const int64_t v = g_error_flag.item<int>();
-    if (reset && v) g_error_flag.zero_();
+    int64_t v = 0;
+    for (Tensor& t : g_error_flags.on) {
+        if (!t.defined()) continue;
+        const int64_t x = t.item<int>();
+        if (reset && x) t.zero_();
+        if (!v) v = x;
+    }
     return v;
 }
 
@@ -605,4 +613,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw8_step", &adamw8_step);
     sg_register_extra(m);
     sg_register_device_io(m);
+    sg_register_decode(m);
 }

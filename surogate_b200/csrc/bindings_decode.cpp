@@ -1,0 +1,247 @@
+// Bindings of the answering path: paged key/value cache, attention over it, drawing of tokens.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <string>
+
+#include "ext_api.h"
+#include "paged_kv.h"
+#include "sampling.h"
+
+namespace {
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+// Numbers in messages go in as text: with some tool chains a stream's number formatting crashes inside an extension.
+std::string num(int64_t v) { return std::to_string(v); }
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int kv_type(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kBFloat16: return sg::kKvBf16;
+        case at::kHalf: return sg::kKvFp16;
+        case at::kFloat8_e4m3fn: return sg::kKvE4m3;
+        case at::kFloat: return sg::kKvFp32;
+        default: TORCH_CHECK(false, what, " must be bf16, fp16, fp32 or float8_e4m3fn, not ", c10::toString(t.scalar_type()));
+    }
+}
+const int* index_ptr(const Tensor& t, const Tensor& like, int64_t n, const char* what) {
+    TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && (n < 2 || t.stride(0) == 1), what, " must be int32 [", num(n),
+                "], contiguous, on the cache's device");
+    return t.data_ptr<int>();
+}
+
+// One layer's pages [pages, 2, heads, page size, dim]
+sg::KvPages pages_of(const Tensor& kv, const OptTensor& scales) {
+    TORCH_CHECK(kv.is_cuda() && kv.dim() == 5 && kv.size(1) == 2, "kv must be a CUDA tensor [pages, 2, kv heads, page size, head size]");
+    sg::KvPages k{};
+    k.type = kv_type(kv, "kv");
+    const int64_t es = kv.element_size();
+    TORCH_CHECK(kv.size(0) > 0 && kv.size(2) > 0 && kv.size(3) > 0 && kv.size(4) > 0, "kv must not be empty");
+    TORCH_CHECK(kv.size(0) < (int64_t{1} << 31) && kv.size(2) <= 65535, "kv: too many pages or heads");
+    TORCH_CHECK(kv.size(3) % 16 == 0 && kv.size(3) <= 65536, "kv: the page size must be a multiple of 16, not ", num(kv.size(3)));
+    TORCH_CHECK(kv.size(4) % 8 == 0 && kv.size(4) <= 256 && kv.size(4) * es % 16 == 0, "kv: the head size must fill 16-byte vectors and be at most 256, not ", num(kv.size(4)));
+    TORCH_CHECK(kv.stride(4) == 1 && aligned(kv.data_ptr(), 16), "kv: the elements of a head must be contiguous, and 16-byte aligned");
+    for (int i = 0; i < 4; ++i) TORCH_CHECK(kv.size(i) == 1 || (kv.stride(i) > 0 && kv.stride(i) * es % 16 == 0), "kv: strides must be positive multiples of 16 bytes");
+    k.data = kv.data_ptr();
+    k.page_stride = kv.stride(0);
+    k.kv_stride = kv.stride(1);
+    k.head_stride = kv.stride(2);
+    k.tok_stride = kv.stride(3);
+    k.num_pages = static_cast<int>(kv.size(0));
+    k.heads = static_cast<int>(kv.size(2));
+    k.page_size = static_cast<int>(kv.size(3));
+    k.dim = static_cast<int>(kv.size(4));
+    TORCH_CHECK(given(scales) == (k.type == sg::kKvE4m3), "scales go with a float8_e4m3fn cache, and only with one");
+    if (given(scales)) {
+        const Tensor& s = *scales;
+        TORCH_CHECK(s.device() == kv.device() && s.scalar_type() == at::kFloat && s.dim() == 4 && s.size(0) == kv.size(0) && s.size(1) == 2 && s.size(2) == kv.size(2) &&
+                        s.size(3) == kv.size(3),
+                    "scales must be fp32 [pages, 2, kv heads, page size] on the cache's device");
+        TORCH_CHECK(s.stride(3) == 1 && aligned(s.data_ptr(), 8) && s.stride(0) % 2 == 0 && s.stride(1) % 2 == 0 && s.stride(2) % 2 == 0,
+                    "scales: the places of a page must be contiguous and 8-byte aligned");
+        k.scales = s.data_ptr<float>();
+        k.s_page_stride = s.stride(0);
+        k.s_kv_stride = s.stride(1);
+        k.s_head_stride = s.stride(2);
+    }
+    return k;
+}
+void table_of(const Tensor& table, const Tensor& kv, int64_t B, const int*& ptr, int64_t& stride, int& width) {
+    TORCH_CHECK(table.device() == kv.device() && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && (table.size(1) < 2 || table.stride(1) == 1),
+                "page_table must be int32 [", num(B), ", pages of a row], rows contiguous, on the cache's device");
+    TORCH_CHECK(table.size(1) > 0 && table.size(1) * kv.size(3) <= (int64_t{1} << 30), "page_table: rows must hold 1 to 2^30 tokens");
+    ptr = table.data_ptr<int>();
+    stride = table.stride(0);
+    width = static_cast<int>(table.size(1));
+}
+
+void kv_append(const Tensor& kv, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& start, const OptTensor& count, const OptTensor& scales) {
+    sg::KvAppend p{};
+    p.kv = pages_of(kv, scales);
+    const Tensor* src[2] = {&k, &v};
+    for (int i = 0; i < 2; ++i) {
+        const Tensor& t = *src[i];
+        TORCH_CHECK(t.device() == kv.device() && t.dim() == 4 && t.size(2) == p.kv.heads && t.size(3) == p.kv.dim && t.sizes() == k.sizes() && t.scalar_type() == k.scalar_type(),
+                    "k and v must be [rows, tokens, ", num(p.kv.heads), ", ", num(p.kv.dim), "] of one type on the cache's device");
+        const int64_t es = t.element_size();
+        TORCH_CHECK((t.size(3) < 2 || t.stride(3) == 1) && aligned(t.data_ptr(), 16) && t.stride(0) * es % 16 == 0 && t.stride(1) * es % 16 == 0 && t.stride(2) * es % 16 == 0,
+                    "k and v: the elements of a head must be contiguous, heads 16-byte aligned");
+        p.src[i] = t.data_ptr();
+        p.b_stride[i] = t.stride(0);
+        p.t_stride[i] = t.stride(1);
+        p.h_stride[i] = t.stride(2);
+    }
+    p.src_type = kv_type(k, "k and v");
+    TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.src_type != sg::kKvE4m3 : p.src_type == p.kv.type, "k and v must have the cache's type (with an e4m3 cache: bf16, fp16 or fp32)");
+    const int64_t B = k.size(0), T = k.size(1);
+    TORCH_CHECK(B < (int64_t{1} << 31) && T < (int64_t{1} << 30) && B * T * 2 * p.kv.heads * 32 < (int64_t{1} << 40), "k and v: too many tokens for one call");
+    if (B == 0 || T == 0) return;
+    table_of(table, kv, B, p.table, p.table_stride, p.table_width);
+    p.start = index_ptr(start, kv, B, "start");
+    if (given(count)) p.count = index_ptr(*count, kv, B, "count");
+    p.B = static_cast<int>(B);
+    p.T = static_cast<int>(T);
+    const c10::cuda::CUDAGuard guard(kv.device());
+    p.error_flag = sg_error_flag();
+    sg_count_launch(1);
+    sg::kv_append(p, cur_stream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const OptTensor& scales) {
+    TORCH_CHECK(kv.is_cuda() && kv.dim() == 6 && kv.size(2) == 2, "kv must be a CUDA tensor [layers, pages, 2, kv heads, page size, head size]");
+    sg::KvCopy p{};
+    const Tensor none;
+    const Tensor* part[2] = {&kv, given(scales) ? &*scales : nullptr};
+    for (int i = 0; i < 2 && part[i]; ++i) {
+        const Tensor& t = *part[i];
+        if (i) TORCH_CHECK(t.device() == kv.device() && t.dim() == 5 && t.size(0) == kv.size(0) && t.size(1) == kv.size(1), "scales must be [layers, pages, 2, kv heads, page size] on the cache's device");
+        const int64_t es = t.element_size(), bytes = t.numel() ? t.numel() / (t.size(0) * t.size(1)) * es : 0;
+        TORCH_CHECK(t.numel() == 0 || t[0][0].is_contiguous(), i ? "scales" : "kv", ": each page must be contiguous");
+        TORCH_CHECK(bytes % 16 == 0 && aligned(t.data_ptr(), 16) && t.stride(0) * es % 16 == 0 && t.stride(1) * es % 16 == 0 && t.stride(0) >= 0 && t.stride(1) >= 0,
+                    i ? "scales" : "kv", ": pages must be 16-byte aligned");
+        p.base[i] = static_cast<uint8_t*>(t.data_ptr());
+        p.layer_bytes[i] = t.stride(0) * es;
+        p.page_stride_bytes[i] = t.stride(1) * es;
+        p.page_bytes[i] = bytes;
+    }
+    const int64_t n = src.numel();
+    TORCH_CHECK(n <= 65535 && kv.size(0) <= 65535 && kv.size(1) < (int64_t{1} << 31), "kv_copy_pages: at most 65535 pairs and layers in one call");
+    p.src = index_ptr(src, kv, n, "src");
+    p.dst = index_ptr(dst, kv, n, "dst");
+    if (n == 0 || kv.numel() == 0) return;
+    p.n = static_cast<int>(n);
+    p.layers = static_cast<int>(kv.size(0));
+    p.num_pages = static_cast<int>(kv.size(1));
+    const c10::cuda::CUDAGuard guard(kv.device());
+    p.error_flag = sg_error_flag();
+    sg_count_launch(1);
+    sg::kv_copy_pages(p, sms(), cur_stream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// -> (output [B, Hq, dim], log-sum-exp fp32 [B, Hq] or undefined)
+std::vector<Tensor> paged_attention(const Tensor& q, const Tensor& kv, const Tensor& table, const Tensor& lengths, double scale, int64_t window, double softcap,
+                                    const OptTensor& sinks, const OptTensor& scales, bool want_lse) {
+    sg::PagedAttention p{};
+    p.kv = pages_of(kv, scales);
+    TORCH_CHECK(p.kv.type != sg::kKvFp32, "paged_attention reads bf16, fp16 and float8_e4m3fn caches");
+    TORCH_CHECK(p.kv.dim == 64 || p.kv.dim == 128 || p.kv.dim == 256, "paged_attention takes head sizes 64, 128 and 256, not ", num(p.kv.dim));
+    TORCH_CHECK(q.device() == kv.device() && q.dim() == 3 && q.size(2) == p.kv.dim, "q must be [rows, query heads, ", num(p.kv.dim), "] on the cache's device");
+    p.q_type = kv_type(q, "q");
+    TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.q_type == sg::kKvBf16 || p.q_type == sg::kKvFp16 : p.q_type == p.kv.type, "q must have the cache's type (with an e4m3 cache: bf16 or fp16)");
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) <= 65535 && q.size(1) % p.kv.heads == 0, "the query heads must be a multiple of the ", num(p.kv.heads), " key heads");
+    const int64_t B = q.size(0);
+    TORCH_CHECK(B <= 65535, "paged_attention: at most 65535 rows in one call");
+    TORCH_CHECK(q.stride(2) == 1 && aligned(q.data_ptr(), 16) && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0, "q: the elements of a head must be contiguous, heads 16-byte aligned");
+    TORCH_CHECK(window >= 0 && softcap >= 0 && std::isfinite(scale) && std::isfinite(softcap), "window and softcap must not be negative, scale and softcap finite");
+    const c10::cuda::CUDAGuard guard(kv.device());
+    Tensor out = torch::empty({B, q.size(1), q.size(2)}, q.options()), lse;
+    if (want_lse) lse = torch::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
+    if (B == 0) return {out, lse};
+    table_of(table, kv, B, p.table, p.table_stride, p.table_width);
+    p.lengths = index_ptr(lengths, kv, B, "lengths");
+    if (given(sinks)) {
+        TORCH_CHECK(sinks->device() == kv.device() && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1), "sinks must be fp32 [query heads]");
+        p.sinks = sinks->data_ptr<float>();
+    }
+    p.q = q.data_ptr();
+    p.q_b_stride = q.stride(0);
+    p.q_h_stride = q.stride(1);
+    p.out = out.data_ptr();
+    p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+    p.B = static_cast<int>(B);
+    p.Hq = static_cast<int>(q.size(1));
+    const int64_t room = static_cast<int64_t>(p.table_width) * p.kv.page_size;
+    p.window = static_cast<int>(window >= room ? 0 : window);
+    p.scale = static_cast<float>(scale);
+    p.softcap = static_cast<float>(softcap);
+    p.error_flag = sg_error_flag();
+    const sg::PagedAttentionPlan plan = sg::paged_attention_plan(p.B, p.Hq, p.kv.heads, p.kv.dim, p.kv.type, p.window ? std::min<int64_t>(room, p.window + 64) : room, sms());
+    Tensor ws;      // from the caching allocator, on the stream that uses it
+    if (plan.workspace_floats) ws = torch::empty({plan.workspace_floats}, q.options().dtype(at::kFloat));
+    sg_count_launch(plan.whole ? 1 : 2);
+    const char* err = sg::paged_attention(p, plan, plan.workspace_floats ? ws.data_ptr<float>() : nullptr, cur_stream());
+    TORCH_CHECK(err == nullptr, err ? err : "");
+    return {out, lse};
+}
+
+std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& u, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p,
+                                         double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1), "logits must be a CUDA tensor [rows, vocabulary], rows contiguous");
+    sg::SampleTokens p{};
+    p.type = kv_type(logits, "logits");
+    TORCH_CHECK(p.type != sg::kKvE4m3, "logits must be bf16, fp16 or fp32");
+    const int64_t B = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(V > 0 && V <= (int64_t{1} << 28) && B < (int64_t{1} << 27), "logits: an empty or too large vocabulary, or too many rows");
+    auto floats = [&](const OptTensor& t, const char* what) -> const float* {
+        if (!given(t)) return nullptr;
+        TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == B && (B < 2 || t->stride(0) == 1), what, " must be fp32 [", num(B),
+                    "], contiguous, on the logits' device");
+        return t->data_ptr<float>();
+    };
+    p.u = floats(u, "u");
+    p.temperature = floats(temperature, "temperature");
+    p.top_p = floats(top_p, "top_p");
+    p.min_p = floats(min_p, "min_p");
+    if (given(top_k)) {
+        TORCH_CHECK(top_k->device() == logits.device() && top_k->scalar_type() == at::kInt && top_k->dim() == 1 && top_k->size(0) == B && (B < 2 || top_k->stride(0) == 1),
+                    "top_k must be int32 [", num(B), "], contiguous, on the logits' device");
+        p.top_k = top_k->data_ptr<int>();
+    }
+    p.temperature_all = static_cast<float>(temperature_all);
+    p.top_k_all = static_cast<int>(std::min<int64_t>(std::max<int64_t>(top_k_all, 0), V));
+    p.top_p_all = static_cast<float>(top_p_all);
+    p.min_p_all = static_cast<float>(min_p_all);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    Tensor token = torch::empty({B}, logits.options().dtype(at::kInt)), logprob = torch::empty({B}, logits.options().dtype(at::kFloat));
+    if (B == 0) return {token, logprob};
+    p.logits = logits.data_ptr();
+    p.row_stride = logits.stride(0);
+    p.B = static_cast<int>(B);
+    p.V = static_cast<int>(V);
+    p.token = token.data_ptr<int>();
+    p.logprob = logprob.data_ptr<float>();
+    sg_count_launch(1);
+    const char* err = sg::sample_tokens(p, sms(), cur_stream());
+    TORCH_CHECK(err == nullptr, err ? err : "");
+    return {token, logprob};
+}
+
+}  // namespace
+
+void sg_register_decode(pybind11::module_& m) {
+    namespace py = pybind11;
+    m.def("kv_append", &kv_append, py::arg("kv"), py::arg("k"), py::arg("v"), py::arg("page_table"), py::arg("start"), py::arg("count") = OptTensor(), py::arg("scales") = OptTensor());
+    m.def("kv_copy_pages", &kv_copy_pages, py::arg("kv"), py::arg("src"), py::arg("dst"), py::arg("scales") = OptTensor());
+    m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("kv"), py::arg("page_table"), py::arg("lengths"), py::arg("scale"), py::arg("window") = 0,
+          py::arg("softcap") = 0.0, py::arg("sinks") = OptTensor(), py::arg("scales") = OptTensor(), py::arg("want_lse") = false);
+    m.def("sample_tokens", &sample_tokens, py::arg("logits"), py::arg("u"), py::arg("temperature") = OptTensor(), py::arg("top_k") = OptTensor(), py::arg("top_p") = OptTensor(),
+          py::arg("min_p") = OptTensor(), py::arg("temperature_all") = 1.0, py::arg("top_k_all") = 0, py::arg("top_p_all") = 1.0, py::arg("min_p_all") = 0.0);
+}

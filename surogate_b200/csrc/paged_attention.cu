@@ -1,0 +1,647 @@
+// Attention of one new token a sequence over a paged key/value cache.
+//
+//   s_j = scale * q . k_j  (capped: c * tanh(s / c)),  o = sum_j e^{s_j} v_j / (sum_j e^{s_j} [+ e^{sink}]),  j in [max(0, n - window), n)
+//
+// Every key and value is read once for the query heads that share it: 4 * (query heads per key head) operations for each 2 or 4 bytes, so HBM
+// bounds it, and all the rest is arranged around reading without a pause.
+//
+// * A block of four warps takes tiles of 64 keys of one row and key head; a warp has 16 of them, one page at a time (a page holds a multiple of
+//   16 tokens).  The query heads of the key head are the rows of m16n8k16 products; warps have their own running maximum, sum and output, and
+//   meet once, at the end of the row's piece.
+// * The sums of a product may run over the head's elements in any order.  So a lane takes whole 16-byte pieces of the key rows: the piece
+//   that it loads is, word for word, its share of the operand, with the query laid out to match.  For the values the lane that loads four
+//   keys' pieces pairs their elements by byte permutes.  A lane therefore reads back from shared memory only what it copied there itself:
+//   the ring of asynchronous copies needs no barrier and no swizzle, and has no bank conflicts.
+// * Weights are split into two bf16 (or fp16) terms before they meet the values, hi + lo, which keeps 16 (22) bits: tensor cores have time to
+//   spare here, and the output's own rounding stays the only one that counts.  With e4m3 values one fp16 term (2^-12) is below the
+//   values' own 2^-4.
+// * e4m3: keys and values become fp16 exactly; the query as fp16 is scaled by a power of two to below 2 for each row (what it loses lies 2^-25
+//   below its largest element).  The scale of a key multiplies its score; that of a value goes into the exponent of its weight, whose
+//   running maximum then bounds weight times scale.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "launch_limits.h"
+#include "paged_kv.h"
+#include "sm100_ptx.cuh"
+
+namespace sg {
+
+namespace {
+
+constexpr int kTile = 64, kWarps = 4, kStep = 16;   // keys a tile, warps a block, keys a warp and tile
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(valid ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// d += a b: rows 0-7 of a in a0, a2, rows 8-15 in a1, a3
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same where rows 8-15 of a are zero: only rows 0-7 of d are kept
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[2], uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
+    float z0, z1;
+    const uint32_t zero = 0;
+    const float fz = 0.f;
+    if (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+            : "+f"(d[0]), "+f"(d[1]), "=f"(z0), "=f"(z1) : "r"(a0), "r"(zero), "r"(a2), "r"(b0), "r"(b1), "f"(fz));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+            : "+f"(d[0]), "+f"(d[1]), "=f"(z0), "=f"(z1) : "r"(a0), "r"(zero), "r"(a2), "r"(b0), "r"(b1), "f"(fz));
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+// two e4m3 values (the lower 16 bits) as two fp16
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+    return r;
+}
+
+// Compile-time layout of one variant.
+template <int KT, int D, int ROWS> struct Shape {
+    static constexpr int ES = KT == kKvE4m3 ? 1 : 2;               // bytes of a cached element
+    static constexpr bool BF16 = KT == kKvBf16;                    // operand type of the products: bf16, else fp16
+    static constexpr int KCH = D * ES / 64;                        // 16-byte pieces of a key row for each of the four lanes that share it
+    static constexpr int VB = D * ES >= 128 ? 16 : 8;              // bytes of a piece of a value row, shared by eight lanes
+    static constexpr int VCH = D * ES / (8 * VB);
+    static constexpr int E = VB / ES;                              // elements of that piece
+    static constexpr int KBYTES = 2 * KCH * 512, VBYTES = 4 * VCH * VB * 32, SBYTES = KT == kKvE4m3 ? 4 * 8 * 32 : 0;
+    static constexpr int STAGE = KBYTES + VBYTES + SBYTES;
+    static constexpr int STAGES = 24576 / STAGE > 8 ? 8 : 24576 / STAGE < 3 ? 3 : 24576 / STAGE;
+    static constexpr int RING = STAGE * STAGES;                    // of one warp; holds its ROWS x D fp32 outputs when warps meet
+    static constexpr int NT = D / 8;                               // n-tiles of the output
+    static constexpr int NACC = ROWS == 16 ? 4 : 2;
+    static constexpr int SMEM = kWarps * RING;
+    static_assert(RING >= ROWS * D * 4, "the ring holds a warp's outputs");
+};
+
+struct Cut {             // where the pieces of a shared problem go
+    float* part_o;       // [2 * blocks][ROWS][D]
+    float2* part_ml;     // [2 * blocks][ROWS]: maximum (base 2), sum
+    long long* prefix;   // [B + 2]: first unit of each row, all units, units a block
+    int blocks, min_units;
+};
+
+__device__ __forceinline__ int row_keys(const PagedAttention& p, int b) {
+    const int n = p.lengths[b];
+    const int64_t room = static_cast<int64_t>(p.table_width) * p.kv.page_size;
+    if (n < 0 || n > room) {
+        atomicExch(p.error_flag, kErrBadPage);
+        return n < 0 ? 0 : static_cast<int>(room);
+    }
+    return n;
+}
+__device__ __forceinline__ int first_key(const PagedAttention& p, int n) { return p.window > 0 ? max(0, n - p.window) : 0; }
+__device__ __forceinline__ int row_tiles(const PagedAttention& p, int n) { return (n + kTile - 1) / kTile - first_key(p, n) / kTile; }
+
+template <typename QT> __device__ __forceinline__ QT from_float(float x);
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+template <int KT, typename QT, int D, int ROWS>
+struct Piece {
+    using S = Shape<KT, D, ROWS>;
+    static constexpr bool HI = ROWS == 16;
+    // weights are carried as 2^15 times themselves where they become fp16, whose smallest step is 2^-24
+    static constexpr float kShift = S::BF16 ? 0.f : 15.f;
+
+    // Tiles [tb, te) of row b (tile numbers of the row's positions) and head group vh.  slot < 0: the whole row; its result is written.  Else the piece is.
+    static __device__ void run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, uint8_t* smem, float2 (*sh_ml)[16]) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const int G = p.Hq / p.kv.heads, kvh = vh / groups, h0 = kvh * G + (vh - kvh * groups) * ROWS, nrows = min(ROWS, kvh * G + G - h0);
+        const int lo = first_key(p, n), steps = te - tb;
+        const uint32_t ring = smem_u32(smem) + warp * S::RING;
+        const char* kv0 = static_cast<const char*>(p.kv.data) + static_cast<int64_t>(kvh) * p.kv.head_stride * S::ES;
+        const int* table = p.table + b * p.table_stride;
+
+        // page of the warp's keys in step base + lane; -1: none of them counts
+        auto load_pages = [&](int base) {
+            const int64_t t = static_cast<int64_t>(tb + base + lane) * kTile + warp * kStep;
+            if (base + lane >= steps || t >= n || t + kStep <= lo) return -1;
+            int page = table[t / p.kv.page_size];
+            if (page < 0 || page >= p.kv.num_pages) {
+                atomicExch(p.error_flag, kErrBadPage);
+                page = -1;
+            }
+            return page;
+        };
+        int pages = load_pages(0), pages_next = load_pages(32);
+        unsigned have = 0;            // bit i % 32: step i has a page
+
+        auto issue = [&](int i) {
+            if ((i & 31) == 0 && i > 0) {
+                pages = pages_next;
+                pages_next = load_pages(i + 32);
+            }
+            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+            have = (have & ~(1u << (i & 31))) | (page >= 0 ? 1u << (i & 31) : 0u);
+            if (page < 0) return;
+            const int t0 = (tb + i) * kTile + warp * kStep, place = t0 % p.kv.page_size;
+            const uint32_t dst = ring + (i % S::STAGES) * S::STAGE;
+            const char* kb = kv0 + (page * p.kv.page_stride + place * p.kv.tok_stride) * S::ES;
+            const char* vb = kb + p.kv.kv_stride * S::ES;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int k = t * 8 + g;
+                const bool ok = t0 + k >= lo && t0 + k < n;
+                const char* src = kb + k * p.kv.tok_stride * S::ES + c * 16;
+#pragma unroll
+                for (int j = 0; j < S::KCH; ++j) cp_async16(dst + (t * S::KCH + j) * 512 + lane * 16, ok ? src + j * 64 : kv0, ok);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int k = 2 * c + (t & 1) + (t >> 1) * 8;
+                const bool ok = t0 + k >= lo && t0 + k < n;
+                const char* src = vb + k * p.kv.tok_stride * S::ES + g * S::VB;
+#pragma unroll
+                for (int j = 0; j < S::VCH; ++j) {
+                    const uint32_t d = dst + S::KBYTES + (t * S::VCH + j) * (32 * S::VB) + lane * S::VB;
+                    if (S::VB == 16) cp_async16(d, ok ? src + j * 8 * S::VB : kv0, ok);
+                    else cp_async8(d, ok ? src + j * 8 * S::VB : kv0, ok);
+                }
+            }
+            if (KT == kKvE4m3) {
+                const float* sc = p.kv.scales + page * p.kv.s_page_stride + kvh * p.kv.s_head_stride + place + 2 * c;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    cp_async8(dst + S::KBYTES + S::VBYTES + t * 256 + lane * 8, sc + (t >> 1) * p.kv.s_kv_stride + (t & 1) * 8, true);
+            }
+        };
+
+#pragma unroll
+        for (int i = 0; i < S::STAGES - 1; ++i) {
+            if (i < steps) issue(i);
+            cp_commit();
+        }
+
+        // the query, piece by piece as the keys lie
+        constexpr int QW = KT == kKvE4m3 ? 8 : 4;                  // words of one row for one 16-byte piece of keys
+        uint32_t q[HI ? 2 : 1][S::KCH][QW];
+        float mult[HI ? 2 : 1];                                    // what turns a product into a score
+#pragma unroll
+        for (int r = 0; r < (HI ? 2 : 1); ++r) {
+            const int row = g + 8 * r;
+            const QT* src = static_cast<const QT*>(p.q) + b * p.q_b_stride + (h0 + (row < nrows ? row : 0)) * p.q_h_stride;
+            constexpr int EL = 16 / S::ES;                         // elements of a piece
+            mult[r] = p.scale;
+#pragma unroll
+            for (int j = 0; j < S::KCH; ++j) {
+#pragma unroll
+                for (int w = 0; w < QW; w += 4) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (row < nrows) v = *reinterpret_cast<const uint4*>(src + (j * 4 + c) * EL + w * 2);
+                    q[r][j][w] = v.x; q[r][j][w + 1] = v.y; q[r][j][w + 2] = v.z; q[r][j][w + 3] = v.w;
+                }
+            }
+            if (KT == kKvE4m3 && sizeof(QT) == 2 && !S::BF16) {
+                constexpr bool QBF = std::is_same<QT, __nv_bfloat16>::value;
+                if (QBF) {                                         // bf16 -> fp16 of the same value over a power of two
+                    float amax = 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::KCH; ++j)
+#pragma unroll
+                        for (int w = 0; w < QW; ++w) {
+                            const float2 f = unpack2<true>(q[r][j][w]);
+                            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        }
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 100);
+                    const float down = __uint_as_float((127 - e) << 23);
+                    mult[r] *= __uint_as_float((127 + e) << 23);
+#pragma unroll
+                    for (int j = 0; j < S::KCH; ++j)
+#pragma unroll
+                        for (int w = 0; w < QW; ++w) {
+                            const float2 f = unpack2<true>(q[r][j][w]);
+                            q[r][j][w] = pack2<false>(f.x * down, f.y * down);
+                        }
+                }
+            }
+            if (p.softcap == 0.f) mult[r] *= kLog2e;
+        }
+        const float cap = p.softcap, inv_cap2 = cap != 0.f ? 2.f * kLog2e / cap : 0.f, cap2 = cap * kLog2e;
+
+        float o[S::NT][S::NACC];
+        float m[HI ? 2 : 1], l[HI ? 2 : 1];
+#pragma unroll
+        for (int i = 0; i < S::NT; ++i)
+#pragma unroll
+            for (int k = 0; k < S::NACC; ++k) o[i][k] = 0.f;
+#pragma unroll
+        for (int r = 0; r < (HI ? 2 : 1); ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+
+        for (int i = 0; i < steps; ++i) {
+            if (i + S::STAGES - 1 < steps) issue(i + S::STAGES - 1);
+            cp_commit();
+            cp_wait<S::STAGES - 1>();
+            if (!((have >> (i & 31)) & 1)) continue;
+            const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
+
+            // scores of 16 keys: s[t][.] columns are keys t * 8 + 2c, + 1
+            float s[2][S::NACC];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int k = 0; k < S::NACC; ++k) s[t][k] = 0.f;
+#pragma unroll
+                for (int j = 0; j < S::KCH; ++j) {
+                    const uint4 kk = lds16(st + (t * S::KCH + j) * 512 + lane * 16);
+                    if (KT != kKvE4m3) {
+                        mma<S::BF16>(s[t], q[0][j][0], q[HI][j][0], q[0][j][1], q[HI][j][1], kk.x, kk.y);
+                        mma<S::BF16>(s[t], q[0][j][2], q[HI][j][2], q[0][j][3], q[HI][j][3], kk.z, kk.w);
+                    } else {
+                        const uint32_t kw[4] = {kk.x, kk.y, kk.z, kk.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            mma<false>(s[t], q[0][j][(2 * w) % QW], q[HI][j][(2 * w) % QW], q[0][j][(2 * w + 1) % QW], q[HI][j][(2 * w + 1) % QW],
+                                       e4m3x2_to_f16x2(static_cast<uint16_t>(kw[w])), e4m3x2_to_f16x2(static_cast<uint16_t>(kw[w] >> 16)));
+                    }
+                }
+            }
+            float lv[2][2];                                        // log2 of the values' scales
+            if (KT == kKvE4m3) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint2 ks = lds8(st + S::KBYTES + S::VBYTES + t * 256 + lane * 8), vs = lds8(st + S::KBYTES + S::VBYTES + (2 + t) * 256 + lane * 8);
+#pragma unroll
+                    for (int k = 0; k < S::NACC; ++k) s[t][k] *= __uint_as_float((k & 1) ? ks.y : ks.x);
+                    lv[t][0] = __log2f(fmaxf(__uint_as_float(vs.x), 0x1p-100f));
+                    lv[t][1] = __log2f(fmaxf(__uint_as_float(vs.y), 0x1p-100f));
+                }
+            }
+            const int t0 = (tb + i) * kTile + warp * kStep;
+            const bool full = t0 >= lo && t0 + kStep <= n;
+            float mx[HI ? 2 : 1];
+#pragma unroll
+            for (int r = 0; r < (HI ? 2 : 1); ++r) mx[r] = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int k = 0; k < S::NACC; ++k) {
+                    float x = s[t][k] * mult[k >> 1];
+                    if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
+                    const int key = t0 + t * 8 + 2 * c + (k & 1);
+                    if (!full && (key < lo || key >= n)) x = -INFINITY;
+                    s[t][k] = x;
+                    mx[k >> 1] = fmaxf(mx[k >> 1], KT == kKvE4m3 ? (x == -INFINITY ? x : x + lv[t][k & 1]) : x);
+                }
+            bool grew = false;
+            float fac[HI ? 2 : 1];
+#pragma unroll
+            for (int r = 0; r < (HI ? 2 : 1); ++r) {
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                const float mn = fmaxf(m[r], mx[r]);
+                grew |= mn > m[r];
+                fac[r] = mn == -INFINITY ? 1.f : ex2(m[r] - mn);
+                m[r] = mn;
+            }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int r = 0; r < (HI ? 2 : 1); ++r) l[r] *= fac[r];
+#pragma unroll
+                for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < S::NACC; ++k) o[nt][k] *= fac[k >> 1];
+            }
+            // weights, as the left operand of the second product: keys 2c, 2c+1 of the first eight (a0, a1), of the second (a2, a3)
+            uint32_t ph[2][HI ? 2 : 1], pl[2][HI ? 2 : 1];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < (HI ? 2 : 1); ++r) {
+                    const float mr = m[r] == -INFINITY ? 0.f : m[r];
+                    const float e0 = ex2(s[t][2 * r] - mr), e1 = ex2(s[t][2 * r + 1] - mr);
+                    l[r] += e0 + e1;
+                    float w0 = e0, w1 = e1;
+                    if (KT == kKvE4m3) {
+                        w0 = s[t][2 * r] == -INFINITY ? 0.f : ex2(s[t][2 * r] - mr + lv[t][0] + kShift);
+                        w1 = s[t][2 * r + 1] == -INFINITY ? 0.f : ex2(s[t][2 * r + 1] - mr + lv[t][1] + kShift);
+                    } else if (kShift != 0.f) {
+                        w0 *= 32768.f;
+                        w1 *= 32768.f;
+                    }
+                    ph[t][r] = pack2<S::BF16>(w0, w1);
+                    if (KT != kKvE4m3) {
+                        const float2 back = unpack2<S::BF16>(ph[t][r]);
+                        pl[t][r] = pack2<S::BF16>(w0 - back.x, w1 - back.y);
+                    }
+                }
+            // o += weights . values; the lane's piece of the value rows is column g of E n-tiles
+#pragma unroll
+            for (int j = 0; j < S::VCH; ++j) {
+                uint32_t v[4][S::VB / 4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t a = st + S::KBYTES + (t * S::VCH + j) * (32 * S::VB) + lane * S::VB;
+                    if (S::VB == 16) {
+                        const uint4 x = lds16(a);
+                        v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
+                    } else {
+                        const uint2 x = lds8(a);
+                        v[t][0] = x.x; v[t][1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < S::VB / 4; ++w) {
+                    if (KT != kKvE4m3) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t sel = x ? 0x7632 : 0x5410;
+                            const uint32_t b0 = __byte_perm(v[0][w], v[1][w], sel), b1 = __byte_perm(v[2][w], v[3][w], sel);
+                            float (&acc)[S::NACC] = o[j * S::E + 2 * w + x];
+                            mma<S::BF16>(acc, ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], b0, b1);
+                            mma<S::BF16>(acc, pl[0][0], pl[0][HI], pl[1][0], pl[1][HI], b0, b1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t sel = x ? 0x7362 : 0x5140;
+                            const uint32_t b0 = __byte_perm(v[0][w], v[1][w], sel), b1 = __byte_perm(v[2][w], v[3][w], sel);
+                            mma<false>(o[j * S::E + 4 * w + 2 * x], ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], e4m3x2_to_f16x2(static_cast<uint16_t>(b0)),
+                                       e4m3x2_to_f16x2(static_cast<uint16_t>(b1)));
+                            mma<false>(o[j * S::E + 4 * w + 2 * x + 1], ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], e4m3x2_to_f16x2(static_cast<uint16_t>(b0 >> 16)),
+                                       e4m3x2_to_f16x2(static_cast<uint16_t>(b1 >> 16)));
+                        }
+                    }
+                }
+            }
+        }
+        cp_wait<0>();
+
+        // the four warps meet
+#pragma unroll
+        for (int r = 0; r < (HI ? 2 : 1); ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (c == 0) sh_ml[warp][g + 8 * r] = make_float2(m[r], l[r]);
+        }
+        __syncthreads();
+        float* mine = reinterpret_cast<float*>(smem + warp * S::RING);
+#pragma unroll
+        for (int r = 0; r < (HI ? 2 : 1); ++r) {
+            float mm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][g + 8 * r].x);
+            const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - mm);
+#pragma unroll
+            for (int j = 0; j < S::VCH; ++j)
+#pragma unroll
+                for (int col = 0; col < 2; ++col)
+#pragma unroll
+                    for (int e = 0; e < S::E; ++e) mine[(g + 8 * r) * D + (j * 8 + 2 * c + col) * S::E + e] = o[j * S::E + e][2 * r + col] * f;
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < nrows * D; x += kWarps * 32) {
+            const int row = x / D, d = x - row * D;
+            float mm = -INFINITY, ll = 0.f, acc = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][row].x);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 v = sh_ml[w][row];
+                if (v.x != -INFINITY) ll += v.y * ex2(v.x - mm);
+                acc += reinterpret_cast<const float*>(smem + w * S::RING)[x];
+            }
+            if (slot >= 0) {
+                cut.part_o[(static_cast<int64_t>(slot) * ROWS + row) * D + d] = acc;
+                if (d == 0) cut.part_ml[slot * ROWS + row] = make_float2(mm, ll);
+            } else {
+                finish(p, b, h0 + row, d, mm, ll, acc);
+            }
+        }
+        __syncthreads();
+    }
+
+    static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float acc) {
+        float total = ll;
+        if (p.sinks) total += ex2(p.sinks[h] * kLog2e - mm);       // infinite where the sink outweighs all keys by 2^128: the output is 0
+        const float y = mm == -INFINITY ? 0.f : acc * (S::BF16 ? 1.f : 0x1p-15f) / total;
+        static_cast<QT*>(p.out)[(static_cast<int64_t>(b) * p.Hq + h) * D + d] = from_float<QT>(y);
+        if (d == 0 && p.lse) p.lse[static_cast<int64_t>(b) * p.Hq + h] = mm == -INFINITY ? -INFINITY : mm * kLn2 + logf(ll);
+    }
+};
+
+// One block for each row and head group.
+template <int KT, typename QT, int D, int ROWS>
+__global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(PagedAttention p, int groups) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 sh_ml[kWarps][16];
+    const int vhs = p.kv.heads * groups, b = blockIdx.x / vhs, vh = blockIdx.x - b * vhs;
+    const int n = row_keys(p, b);
+    const int tb = first_key(p, n) / kTile;
+    Piece<KT, QT, D, ROWS>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, smem, sh_ml);
+}
+
+// All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  A block's first and
+// last piece may be part of a row; each goes to a slot of its own.
+template <int KT, typename QT, int D, int ROWS>
+__global__ void __launch_bounds__(kWarps * 32) paged_attention_shared_kernel(PagedAttention p, Cut cut, int groups) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 sh_ml[kWarps][16];
+    __shared__ long long sh_sum[kWarps];
+    __shared__ int sh_b;
+    __shared__ long long sh_rest;
+    const int vhs = p.kv.heads * groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // units (tiles of one head group) before each row: a thread adds up its share of the rows, the block scans the sums
+    const int each = (p.B + kWarps * 32 - 1) / (kWarps * 32), r0 = min(p.B, static_cast<int>(threadIdx.x) * each), r1 = min(p.B, r0 + each);
+    long long mine = 0;
+    for (int b = r0; b < r1; ++b) mine += static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+    long long scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+    }
+    if (lane == 31) sh_sum[warp] = scan;
+    if (threadIdx.x == 0) sh_b = p.B;
+    __syncthreads();
+    long long before = scan - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sh_sum[w];
+        total += sh_sum[w];
+    }
+    const long long per = max(static_cast<long long>(cut.min_units), (total + cut.blocks - 1) / cut.blocks);
+    const long long begin = per * blockIdx.x, end = min(total, begin + per);
+    if (blockIdx.x == 0) {                                          // what the joining kernel needs
+        long long u = before;
+        for (int b = r0; b < r1; ++b) {
+            cut.prefix[b] = u;
+            u += static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+        }
+        if (threadIdx.x == 0) { cut.prefix[p.B] = total; cut.prefix[p.B + 1] = per; }
+    }
+    if (begin >= total) return;
+    if (begin >= before && begin < before + mine) {                 // exactly one thread
+        long long u = before;
+        for (int b = r0; b < r1; ++b) {
+            const long long k = static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+            if (begin < u + k) { sh_b = b; sh_rest = begin - u; break; }
+            u += k;
+        }
+    }
+    __syncthreads();
+    int b = sh_b;
+    long long rest = sh_rest, left = end - begin;                   // units into the row, units still to do
+    bool first = true;
+    while (left > 0 && b < p.B) {
+        const int n = row_keys(p, b), tiles = row_tiles(p, n);
+        if (rest >= static_cast<long long>(tiles) * vhs) { ++b; rest = 0; continue; }   // an empty row, or this one is done
+        const int vh = static_cast<int>(rest / tiles), t = static_cast<int>(rest - static_cast<long long>(vh) * tiles);
+        const int k = static_cast<int>(min(static_cast<long long>(tiles - t), left));
+        const int tb = first_key(p, n) / kTile + t;
+        Piece<KT, QT, D, ROWS>::run(p, cut, b, vh, n, tb, tb + k, groups, k == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), smem, sh_ml);
+        first = false;
+        rest += k;
+        left -= k;
+    }
+}
+
+// Joins the pieces of one row and query head, and writes the outputs of empty rows.  The pieces of a row come in the order of their blocks, so
+// the sums do not depend on which block ended first.
+template <int KT, typename QT, int D, int ROWS>
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttention p, Cut cut, int groups) {
+    __shared__ float sh_f[128];
+    const int G = p.Hq / p.kv.heads, b = blockIdx.y, h = blockIdx.x, kvh = h / G, vhs = p.kv.heads * groups, vh = kvh * groups + (h - kvh * G) / ROWS, row = (h - kvh * G) % ROWS;
+    const long long u = cut.prefix[b], tiles = (cut.prefix[b + 1] - u) / vhs, per = cut.prefix[p.B + 1], u0 = u + vh * tiles;
+    if (tiles == 0) {
+        for (int d = threadIdx.x; d < D; d += 128) Piece<KT, QT, D, ROWS>::finish(p, b, h, d, -INFINITY, 0.f, 0.f);
+        return;
+    }
+    const int c0 = static_cast<int>(u0 / per), c1 = static_cast<int>((u0 + tiles - 1) / per);
+    if (c0 == c1) return;
+    auto slot = [&](int c) { return static_cast<int64_t>(2 * c + (c == c0 && c0 * per < u0 ? 1 : 0)); };
+    float mm = -INFINITY, ll = 0.f;
+    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, cut.part_ml[slot(c) * ROWS + row].x);
+    float acc[(D + 127) / 128];
+#pragma unroll
+    for (int k = 0; k < (D + 127) / 128; ++k) acc[k] = 0.f;
+    for (int base = c0; base <= c1; base += 128) {
+        __syncthreads();
+        const int c = base + threadIdx.x;
+        if (c <= c1) {
+            const float2 v = cut.part_ml[slot(c) * ROWS + row];
+            sh_f[threadIdx.x] = v.x == -INFINITY ? 0.f : ex2(v.x - mm);
+        }
+        __syncthreads();
+        const int cnt = min(128, c1 + 1 - base);
+        for (int i = 0; i < cnt; ++i) {
+            const float f = sh_f[i];
+            ll += f * cut.part_ml[slot(base + i) * ROWS + row].y;
+#pragma unroll
+            for (int k = 0; k < (D + 127) / 128; ++k) {
+                const int d = k * 128 + threadIdx.x;
+                if (d < D) acc[k] += f * cut.part_o[(slot(base + i) * ROWS + row) * D + d];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < (D + 127) / 128; ++k) {
+        const int d = k * 128 + threadIdx.x;
+        if (d < D) Piece<KT, QT, D, ROWS>::finish(p, b, h, d, mm, ll, acc[k]);
+    }
+}
+
+template <int KT, typename QT, int D, int ROWS>
+const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
+    using S = Shape<KT, D, ROWS>;
+    static std::atomic<uint64_t> raised_whole{0}, raised_shared{0};
+    if (plan.whole) {
+        auto k = paged_attention_whole_kernel<KT, QT, D, ROWS>;
+        if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
+        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, S::SMEM, s>>>(p, plan.head_groups);
+    } else {
+        auto k = paged_attention_shared_kernel<KT, QT, D, ROWS>;
+        if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_shared)) return "paged_attention: the shared-memory limit could not be raised";
+        Cut cut;
+        cut.blocks = plan.blocks;
+        cut.min_units = 4;
+        cut.prefix = reinterpret_cast<long long*>(ws);
+        cut.part_ml = reinterpret_cast<float2*>(ws + 2 * (static_cast<int64_t>(p.B) + 2));
+        cut.part_o = reinterpret_cast<float*>(cut.part_ml + 2 * static_cast<int64_t>(plan.blocks) * ROWS);
+        k<<<plan.blocks, kWarps * 32, S::SMEM, s>>>(p, cut, plan.head_groups);
+        if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
+        paged_attention_join_kernel<KT, QT, D, ROWS><<<dim3(p.Hq, p.B), 128, 0, s>>>(p, cut, plan.head_groups);
+    }
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
+    return nullptr;
+}
+
+template <int KT, typename QT>
+const char* launch_dim(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
+    if (p.kv.dim == 64) return plan.rows == 16 ? launch<KT, QT, 64, 16>(p, plan, ws, s) : launch<KT, QT, 64, 8>(p, plan, ws, s);
+    if (p.kv.dim == 128) return plan.rows == 16 ? launch<KT, QT, 128, 16>(p, plan, ws, s) : launch<KT, QT, 128, 8>(p, plan, ws, s);
+    return launch<KT, QT, 256, 8>(p, plan, ws, s);
+}
+
+}  // namespace
+
+PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_type, int64_t max_keys, int num_sms) {
+    PagedAttentionPlan plan{};
+    const int G = Hq / Hkv;
+    // Eight rows of a product suffice up to eight query heads a key head.  Heads of 256 stay with eight: sixteen rows of 256 outputs and queries
+    // would not fit a thread's registers.
+    plan.rows = G > 8 && dim <= 128 ? 16 : 8;
+    plan.head_groups = (G + plan.rows - 1) / plan.rows;
+    const int64_t pairs = static_cast<int64_t>(B) * Hkv * plan.head_groups, tiles = (max_keys + kTile - 1) / kTile;
+    plan.whole = tiles <= 8;
+    plan.blocks = static_cast<int>(pairs * tiles < 2 * num_sms ? (pairs * tiles > 0 ? pairs * tiles : 1) : 2 * num_sms);
+    plan.workspace_floats = plan.whole ? 0 : 2 * (static_cast<int64_t>(B) + 2) + static_cast<int64_t>(plan.blocks) * 2 * plan.rows * (dim + 2);
+    return plan;
+}
+
+const char* paged_attention(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
+    if (p.B <= 0) return nullptr;
+    const bool qb = p.q_type == kKvBf16;
+    if (p.kv.type == kKvBf16) return launch_dim<kKvBf16, __nv_bfloat16>(p, plan, ws, s);
+    if (p.kv.type == kKvFp16) return launch_dim<kKvFp16, __half>(p, plan, ws, s);
+    return qb ? launch_dim<kKvE4m3, __nv_bfloat16>(p, plan, ws, s) : launch_dim<kKvE4m3, __half>(p, plan, ws, s);
+}
+
+}  // namespace sg

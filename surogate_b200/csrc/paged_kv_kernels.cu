@@ -1,0 +1,199 @@
+// Writing new tokens into a paged key/value cache, and copying pages through all of its layers.
+//
+// Both only move data, so HBM bounds them: an appended token is read once and written once (2 * 2 * heads * dim elements), a copied page
+// likewise, and nothing else is touched.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged_kv.h"
+
+namespace sg {
+
+namespace {
+
+// Page and place of new token t of row b.  False: the token is padding, or its place does not exist (reported).
+__device__ __forceinline__ bool locate_token(const KvAppend& p, int b, int t, int& page, int& place) {
+    const int count = p.count ? min(p.count[b], p.T) : p.T;
+    if (t >= count) return false;
+    const int64_t pos = static_cast<int64_t>(p.start[b]) + t;
+    const int64_t slot = pos / p.kv.page_size;
+    if (pos < 0 || slot >= p.table_width) {
+        atomicExch(p.error_flag, kErrBadPage);
+        return false;
+    }
+    page = p.table[b * p.table_stride + slot];
+    place = static_cast<int>(pos - slot * p.kv.page_size);
+    if (page < 0 || page >= p.kv.num_pages) {
+        atomicExch(p.error_flag, kErrBadPage);
+        return false;
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------ same type: 16-byte copies
+// Items are the 16-byte vectors of the new tokens, in the order (token, key / value, head, vector).  A block takes kThreads * kPerThread of
+// them; a thread requests all of its vectors before it stores the first.
+constexpr int kAppendThreads = 256, kAppendPerThread = 4;
+
+__global__ void __launch_bounds__(kAppendThreads) kv_append_copy_kernel(KvAppend p, int vec_per_head, int elem_bytes, int64_t items) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAppendThreads * kAppendPerThread) + threadIdx.x;
+    uint4 v[kAppendPerThread];
+    char* to[kAppendPerThread];
+    const int per_token = 2 * p.kv.heads * vec_per_head;
+#pragma unroll
+    for (int i = 0; i < kAppendPerThread; ++i) {
+        const int64_t item = first + i * kAppendThreads;
+        to[i] = nullptr;
+        if (item >= items) continue;
+        const int64_t token = item / per_token;
+        const int r = static_cast<int>(item - token * per_token);
+        const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
+        int page, place;
+        if (!locate_token(p, b, t, page, place)) continue;
+        const int row = r / vec_per_head, vec = r - row * vec_per_head;
+        const int which = row >= p.kv.heads, h = row - which * p.kv.heads;
+        const char* from = static_cast<const char*>(p.src[which]) + (b * p.b_stride[which] + t * p.t_stride[which] + h * p.h_stride[which]) * elem_bytes + vec * 16;
+        v[i] = *reinterpret_cast<const uint4*>(from);
+        to[i] = static_cast<char*>(p.kv.data) + (page * p.kv.page_stride + which * p.kv.kv_stride + h * p.kv.head_stride + place * p.kv.tok_stride) * elem_bytes + vec * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendPerThread; ++i)
+        if (to[i]) *reinterpret_cast<uint4*>(to[i]) = v[i];
+}
+
+// ------------------------------------------------------------------------------------------ to e4m3, one scale a token and head
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]);
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&f)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const __nv_bfloat162* t = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 x = __bfloat1622float2(t[i]); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&f)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const __half2* t = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 x = __half22float2(t[i]); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+// LANES lanes hold one head's row, eight elements each (lanes behind the row's end hold zeros): s = max |x| / 448 (at least 2^-100, so that
+// 1/s and log2 s stay finite; 1 for a row of zeros), q = e4m3(x / s).  The one rounding is the cache's own type, at most 2^-4 of a value.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) kv_append_e4m3_kernel(KvAppend p, int64_t rows) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= rows) return;                                           // whole groups of LANES lanes
+    const int lane = threadIdx.x % LANES;
+    const unsigned group = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+    const int heads2 = 2 * p.kv.heads;
+    const int64_t token = row / heads2;
+    const int r = static_cast<int>(row - token * heads2);
+    const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
+    int page, place;
+    if (!locate_token(p, b, t, page, place)) return;
+    const int which = r >= p.kv.heads, h = r - which * p.kv.heads;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    const bool inside = lane * 8 < p.kv.dim;
+    if (inside) load8<T>(static_cast<const T*>(p.src[which]) + b * p.b_stride[which] + t * p.t_stride[which] + h * p.h_stride[which] + lane * 8, f);
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(group, amax, o));
+    const float s = amax > 0.f ? fmaxf(amax / 448.f, 0x1p-100f) : 1.f;
+    if (inside) {
+        uint2 q;
+        uint8_t* q8 = reinterpret_cast<uint8_t*>(&q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q8[i] = __nv_cvt_float_to_fp8(f[i] / s, __NV_SATFINITE, __NV_E4M3);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.kv.data) + page * p.kv.page_stride + which * p.kv.kv_stride + h * p.kv.head_stride + place * p.kv.tok_stride + lane * 8) = q;
+    }
+    if (lane == 0) p.kv.scales[page * p.kv.s_page_stride + which * p.kv.s_kv_stride + h * p.kv.s_head_stride + place] = s;
+}
+
+template <typename T>
+void launch_e4m3(const KvAppend& p, cudaStream_t s) {
+    const int64_t rows = static_cast<int64_t>(p.B) * p.T * 2 * p.kv.heads;
+    const int need = (p.kv.dim + 7) / 8;
+    const int lanes = need <= 8 ? 8 : need <= 16 ? 16 : 32;
+    const int64_t blocks = (rows + 256 / lanes - 1) / (256 / lanes);
+    if (lanes == 8) kv_append_e4m3_kernel<T, 8><<<static_cast<unsigned>(blocks), 256, 0, s>>>(p, rows);
+    else if (lanes == 16) kv_append_e4m3_kernel<T, 16><<<static_cast<unsigned>(blocks), 256, 0, s>>>(p, rows);
+    else kv_append_e4m3_kernel<T, 32><<<static_cast<unsigned>(blocks), 256, 0, s>>>(p, rows);
+}
+
+}  // namespace
+
+void kv_append(const KvAppend& p, cudaStream_t s) {
+    if (p.B <= 0 || p.T <= 0) return;
+    if (p.kv.type != kKvE4m3) {
+        const int es = p.kv.type == kKvFp32 ? 4 : 2;
+        const int vec = p.kv.dim * es / 16;
+        const int64_t items = static_cast<int64_t>(p.B) * p.T * 2 * p.kv.heads * vec;
+        const int64_t per_block = kAppendThreads * kAppendPerThread;
+        kv_append_copy_kernel<<<static_cast<unsigned>((items + per_block - 1) / per_block), kAppendThreads, 0, s>>>(p, vec, es, items);
+    } else if (p.src_type == kKvBf16) launch_e4m3<__nv_bfloat16>(p, s);
+    else if (p.src_type == kKvFp16) launch_e4m3<__half>(p, s);
+    else launch_e4m3<float>(p, s);
+}
+
+// ------------------------------------------------------------------------------------------ pages
+// blockIdx.y: pair of pages, blockIdx.z: group of layers, blockIdx.x: 16 KB piece of a page (the pages' pieces first, then the scales').
+// The pairs of one call run in any order, so no page may be written that another pair reads or writes: every block looks its target up among
+// all sources and targets and leaves a pair that breaks this (or lies outside the cache) undone, with the error word set.
+constexpr int kCopyThreads = 256, kCopyPerThread = 4, kCopyPiece = kCopyThreads * kCopyPerThread * 16;
+
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_pages_kernel(KvCopy p, int pieces0, int layers_per_block) {
+    const int pair = blockIdx.y;
+    const int from = p.src[pair], to = p.dst[pair];
+    const bool outside = from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages;
+    int clash = 0;
+    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) clash |= j != pair && (p.src[j] == to || p.dst[j] == to);
+    clash = __syncthreads_or(clash);
+    if (outside || clash) {
+        if (threadIdx.x == 0) atomicExch(p.error_flag, outside ? kErrBadPage : kErrPageOverlap);
+        return;
+    }
+    const int part = static_cast<int>(blockIdx.x) >= pieces0;
+    const int64_t off = static_cast<int64_t>(part ? blockIdx.x - pieces0 : blockIdx.x) * kCopyPiece;
+    const int64_t left = p.page_bytes[part] - off;
+    const int l0 = blockIdx.z * layers_per_block, l1 = min(p.layers, l0 + layers_per_block);
+    for (int l = l0; l < l1; ++l) {
+        const uint8_t* a = p.base[part] + l * p.layer_bytes[part] + from * p.page_stride_bytes[part] + off;
+        uint8_t* b = p.base[part] + l * p.layer_bytes[part] + to * p.page_stride_bytes[part] + off;
+        uint4 v[kCopyPerThread];
+#pragma unroll
+        for (int i = 0; i < kCopyPerThread; ++i) {
+            const int x = (i * kCopyThreads + threadIdx.x) * 16;
+            if (x < left) v[i] = *reinterpret_cast<const uint4*>(a + x);
+        }
+#pragma unroll
+        for (int i = 0; i < kCopyPerThread; ++i) {
+            const int x = (i * kCopyThreads + threadIdx.x) * 16;
+            if (x < left) *reinterpret_cast<uint4*>(b + x) = v[i];
+        }
+    }
+}
+
+void kv_copy_pages(const KvCopy& p, int num_sms, cudaStream_t s) {
+    if (p.n <= 0 || p.layers <= 0) return;
+    const int pieces0 = static_cast<int>((p.page_bytes[0] + kCopyPiece - 1) / kCopyPiece);
+    const int pieces1 = p.base[1] ? static_cast<int>((p.page_bytes[1] + kCopyPiece - 1) / kCopyPiece) : 0;
+    // one layer a block while that is what fills the GPU (eight blocks an SM); beyond it a block takes several, and looks its pair up once
+    const int64_t per_layer = static_cast<int64_t>(pieces0 + pieces1) * p.n;
+    int groups = static_cast<int>((static_cast<int64_t>(num_sms) * 8 * 4 + per_layer - 1) / per_layer);
+    groups = groups < 1 ? 1 : groups > p.layers ? p.layers : groups;
+    const int layers_per_block = (p.layers + groups - 1) / groups;
+    groups = (p.layers + layers_per_block - 1) / layers_per_block;
+    kv_copy_pages_kernel<<<dim3(pieces0 + pieces1, p.n, groups), kCopyThreads, 0, s>>>(p, pieces0, layers_per_block);
+}
+
+}  // namespace sg

@@ -38,5 +38,13 @@ def check_device_errors(reset: bool = True) -> None:
     """Raise if any kernel reported a pipeline time-out (bounded waits) since the last check. Synchronises."""
     flag = ext().read_error_flag(reset)
     if flag:
-        what = {1: "a bounded device-side wait timed out", 2: "a token id outside [0, vocab_size) reached the embedding"}.get(flag, "a kernel reported an error")
+        what = {1: "a bounded device-side wait timed out", 2: "a token id outside [0, vocab_size) reached the embedding",
+                8: "a page number, position or length outside a paged key/value cache", 9: "a page was copied onto one that another pair of the same call reads or writes"
+                }.get(flag, "a kernel reported an error")
         raise RuntimeError(f"surogate_b200 device error flag = {flag}: {what}")
+
+
+from .paged_kv import PagedKVCache, kv_append, kv_copy_pages, paged_attention  # noqa: E402
+from .sampling import sample_tokens  # noqa: E402
+
+__all__ = ["PagedKVCache", "check_device_errors", "ext", "host", "host_available", "kv_append", "kv_copy_pages", "paged_attention", "sample_tokens"]
