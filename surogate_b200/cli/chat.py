@@ -1,6 +1,6 @@
 """``surogate chat <model dir> [--adapter dir]``: a minimal interactive / one-shot generation loop for checking a trained model.
 
-Decoding re-runs the full prefix every token (no KV cache): fine for a smoke test of a checkpoint, not a serving path.
+Answers come from ``Trainer.generate``: a paged key/value cache where the model's layers allow one, else the whole prefix for every token.
 
 Parity: scripts/chat.py.
 """
@@ -10,25 +10,11 @@ import argparse
 import sys
 from typing import List, Optional
 
-import numpy as np
 
-
-def generate(trainer, tokenizer, prompt_ids: List[int], max_new_tokens: int = 64, temperature: float = 0.0, seed: int = 0, eos_id: Optional[int] = None) -> List[int]:
-    import torch
-
-    ids = list(prompt_ids)
-    gen = torch.Generator().manual_seed(seed)
+def generate(trainer, tokenizer, prompt_ids: List[int], max_new_tokens: int = 64, temperature: float = 0.0, seed: int = 0, eos_id: Optional[int] = None, top_k: int = 0,
+             top_p: float = 1.0, min_p: float = 0.0) -> List[int]:
     eos = tokenizer.eos_token_id if eos_id is None and tokenizer is not None else eos_id
-    for _ in range(max_new_tokens):
-        logits = trainer.logits(np.asarray([ids], np.int32))[0, -1].float().cpu()
-        if temperature > 0:
-            nxt = int(torch.multinomial(torch.softmax(logits / temperature, -1), 1, generator=gen))
-        else:
-            nxt = int(logits.argmax())
-        ids.append(nxt)
-        if eos is not None and nxt == eos:
-            break
-    return ids[len(prompt_ids):]
+    return trainer.generate([prompt_ids], max_new_tokens=max_new_tokens, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, seed=seed, eos_id=eos)[0][0].tokens
 
 
 def main(argv, command: str = "chat") -> int:
@@ -38,6 +24,10 @@ def main(argv, command: str = "chat") -> int:
     p.add_argument("--prompt", default=None, help="answer this prompt and exit (otherwise read prompts from stdin)")
     p.add_argument("--max-new-tokens", type=int, default=128)
     p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--top-k", type=int, default=0, help="draw from the K likeliest tokens only (0: all)")
+    p.add_argument("--top-p", type=float, default=1.0, help="draw from the likeliest tokens that make up this share of the probability")
+    p.add_argument("--min-p", type=float, default=0.0, help="leave out tokens less likely than this share of the likeliest one")
+    p.add_argument("--seed", type=int, default=0)
     a = p.parse_args(argv)
     import torch
 
@@ -62,7 +52,7 @@ def main(argv, command: str = "chat") -> int:
 
     def answer(text: str) -> str:
         ids = tok.apply_chat_template_and_encode([{"role": "user", "content": text}], add_generation_prompt=True)
-        return tok.decode(generate(tr, tok, ids, a.max_new_tokens, a.temperature), skip_special_tokens=True)
+        return tok.decode(generate(tr, tok, ids, a.max_new_tokens, a.temperature, a.seed, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p), skip_special_tokens=True)
 
     if a.prompt is not None:
         print(answer(a.prompt))

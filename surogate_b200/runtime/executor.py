@@ -74,6 +74,8 @@ class ExecContext:
         self.extras: Dict[str, Any] = {}
         # chunked-sequence training: the attention op reads / extends the per-layer key-value prefix kept here
         self.chunk: Optional["ChunkState"] = None
+        # answering: the attention ops append to the paged key/value cache and read it (generation.CacheStep)
+        self.kv: Any = None
         # values that cross layer boundaries outside the block interface, and the gradients flowing back to their producers
         self.shared: Dict[str, torch.Tensor] = {}
         self.shared_grad: Dict[str, torch.Tensor] = {}
@@ -289,6 +291,7 @@ class Executor:
         self.lora = lora
         self._liveness: Dict[int, Dict[str, int]] = {}
         self._programs: Dict[Any, Any] = {}
+        self._before_head: Optional[Tuple[List[OpNode], OpNode]] = None   # last_logits: the top-level ops before the LM head, and the head
         self._saved_sets: Dict[str, Set[str]] = {}
         for bt, bwd in self.cm.block_bwd.items():
             self._saved_sets[bt] = set(bwd.meta["saved"])
@@ -479,6 +482,28 @@ class Executor:
         if self.timer is not None:
             self.timer.mark("forward")
         return ctx, [env[o] for o in g.outputs]
+
+    def last_logits(self, token_ids, position_ids, last, kv=None) -> torch.Tensor:
+        """fp32 logits [rows, V] of the position ``last[row]`` (int64) of each row: the forward graph up to the LM head, and the head's product
+        for one position a row.  ``kv``: the attention layers work on a paged cache (generation.CacheStep)."""
+        ctx = self.new_context(token_ids, False)
+        ctx.kv = kv
+        ctx.phase = "fwd"
+        g = self.cm.fwd
+        if self._before_head is None:
+            i = self._op_index(g, "fused_lm_head_loss")
+            self._before_head = (g.ops[:i], g.ops[i])
+        ops, head = self._before_head
+        env = {"token_ids": token_ids, "position_ids": position_ids}
+        self.store.group_start("embedding", "fwd")
+        self.run_graph(g, env, ctx, {head.inputs[0]}, ops=ops)
+        x = env[head.inputs[0]]
+        if not torch.is_tensor(x):
+            x = x.hp if getattr(x, "hp", None) is not None else x.dequantize()
+        x = x.reshape(token_ids.shape[0], token_ids.shape[1], -1)[torch.arange(token_ids.shape[0], device=last.device), last]
+        out = self.backend.head_logits(x, self.store.get(head.inputs[1]))
+        cap = float(head.attrs.get("softcap") or 0.0)
+        return cap * torch.tanh(out / cap) if cap else out
 
     def backward(self, ctx: ExecContext) -> None:
         g, bg = self.cm.fwd, self.cm.bwd

@@ -308,7 +308,12 @@ class CudaOps(RefOps):
         if ctx.chunk is not None and self._chunk_native_ok(ctx, op.attrs, qkv):
             return self._chunk_attention_native(ctx, op, qkv)
 
-        if ctx.chunk is None and att_ops.native_supported(op.attrs, qkv, ctx) and self.attention_impl in ("auto", "native"):
+        if ctx.kv is not None and not ctx.kv.prompt:
+            return super().flash_attention(ctx, op, qkv)                  # one token a row over the paged cache
+        if ctx.kv is not None and att_ops.native_supported(op.attrs, qkv, ctx) and self.attention_impl in ("auto", "native"):
+            self._cached_attention(ctx, op.attrs, qkv)
+            return att_ops.forward(self.ext, op.attrs, qkv, ctx)
+        if ctx.chunk is None and ctx.kv is None and att_ops.native_supported(op.attrs, qkv, ctx) and self.attention_impl in ("auto", "native"):
             return att_ops.forward(self.ext, op.attrs, qkv, ctx)
         return super().flash_attention(ctx, op, qkv)  # incl. chunked sequences: blockwise PyTorch attention against the key/value prefix
 
@@ -322,6 +327,11 @@ class CudaOps(RefOps):
         return super().flash_attention_backward(ctx, op, d_att, qkv, att, lse)
 
     # ------------------------------------------------------------------ LM head + loss
+    def head_logits(self, x, w):
+        if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or w.shape[1] % 8:
+            return super().head_logits(x, w)
+        return gemm(x.contiguous(), w, out_dtype=torch.float32)
+
     def fused_lm_head_loss(self, ctx, op, x, w, targets):
         """Chunked over rows: logits chunk by GEMM (bf16), cross-entropy forward+backward in place, then the
         dgrad / wgrad GEMMs consume the in-place d_logits.  The full [tokens, vocab] matrix never exists."""

@@ -93,7 +93,9 @@ class RefOps:
         for key in op.attrs.get("shared_in", ()):
             kw[key] = ctx.shared[key]
         with torch.no_grad():
-            out = TORCH_FNS[op.attrs["fn"]](*ins, **kw)
+            out = self._cached_attention(ctx, kw, ins[0], ins[1] if len(ins) > 1 else None) if ctx.kv is not None and op.attrs["fn"] == "attention_general" else None
+            if out is None:
+                out = TORCH_FNS[op.attrs["fn"]](*ins, **kw)
         outs = out if isinstance(out, tuple) else (out,)
         for key, idx in op.attrs.get("shared_out", ()):
             ctx.shared[key] = outs[idx]
@@ -307,6 +309,17 @@ class RefOps:
         x = qkv.reshape(B, T, Hq + 2 * Hkv, D)
         return x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:]
 
+    # ------------------------------------------------------------------ attention on a paged key/value cache (answering)
+    def _cached_attention(self, ctx, a, qkv, sinks=None):
+        """The new tokens' keys and values go to the layer's pages.  One token a row: its attention over them, [B, 1, Hq * D]; a prompt: None."""
+        q, k, v = self._split_heads(qkv, a)
+        return ctx.kv.attend(ctx.layer, q, k, v, softmax_scale=a.get("softmax_scale"), window=int(a.get("window", 0) or 0), softcap=float(a.get("softcap", 0.0) or 0.0),
+                             sinks=None if sinks is None else sinks.float().contiguous())
+
+    def head_logits(self, x, w):
+        """fp32 [rows, V] of the final hidden states of a few positions."""
+        return x.float() @ w.float().t()
+
     # ------------------------------------------------------------------ attention against a key / value prefix (chunked sequences)
     @staticmethod
     def _prefix_mask(Tc, q0, k0, kn, a, device):
@@ -383,6 +396,10 @@ class RefOps:
         if ctx.chunk is not None:
             return self._chunk_attention(ctx, op, qkv)
         a = op.attrs
+        if ctx.kv is not None:
+            att = self._cached_attention(ctx, a, qkv)
+            if att is not None:
+                return att, None
         Hq, Hkv, D = a["num_q_heads"], a["num_kv_heads"], a["head_dim"]
         scale = a.get("softmax_scale") or 1.0 / math.sqrt(D)
         q, k, v = self._split_heads(qkv, a)

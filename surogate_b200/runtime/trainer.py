@@ -704,6 +704,17 @@ class Trainer:
         cap = float(head.attrs.get("softcap") or 0.0)
         return cap * torch.tanh(out / cap) if cap else out
 
+    def generate(self, prompts, **kw):
+        """Sampled answers to ``prompts`` (lists of token ids): for each prompt a list of ``n`` ``Completion(tokens, logprobs, finish_reason)``.
+
+        Keyword arguments: ``n=1`` completions of each prompt, ``max_new_tokens=64``, ``temperature=1.0`` (0: greedy), ``top_k=0``, ``top_p=1.0``,
+        ``min_p=0.0`` (see ``ops.sample_tokens``), ``seed=0``, ``eos_id=None`` (ends a completion), ``page_size=64`` (a multiple of 16) and
+        ``cache_dtype`` (default: the activations' type; ``torch.float8_e4m3fn`` halves the cache) of the paged key/value cache,
+        ``prompt_rows=8`` prompts in one pass.  Log-probabilities are those of the model's softmax, as ``token_logprobs`` gives them."""
+        from .generation import generate
+
+        return generate(self, prompts, **kw)
+
     @torch.no_grad()
     def validate(self, inputs, targets, position_ids=None) -> Dict[str, float]:
         self.drain_optimizer()

@@ -542,3 +542,89 @@ def test_sample_tokens_refusals():
         with pytest.raises(RuntimeError):
             _ops().sample_tokens(*args, **kw)
     assert _ops().sample_tokens(x[:0], u[:0])[0].shape == (0,)
+
+
+# ---------------------------------------------------------------------------------------------- a run of them together
+def _model(kind):
+    if kind == "qwen3":
+        return dict(architecture="Qwen3ForCausalLM", vocab_size=4096, d_model=512, n_layers=2, num_query_heads=4, num_kv_heads=2, head_size=128, d_ff=1536, tie_word_embeddings=True)
+    if kind == "llama":
+        return dict(architecture="LlamaForCausalLM", vocab_size=4096, d_model=512, n_layers=2, num_query_heads=8, num_kv_heads=2, head_size=64, d_ff=1536)
+    if kind == "moe":
+        return dict(architecture="Qwen3MoeForCausalLM", vocab_size=4096, d_model=512, n_layers=2, num_query_heads=4, num_kv_heads=2, head_size=128, num_experts=8,
+                    num_experts_per_tok=2, moe_d_ff=256)
+    return dict(architectures=["GptOssForCausalLM"], model_type="gpt_oss", vocab_size=4096, hidden_size=512, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2,
+                head_dim=64, intermediate_size=256, num_local_experts=4, num_experts_per_tok=2, sliding_window=32, max_position_embeddings=4096, rms_norm_eps=1e-5,
+                rope_theta=150000.0, layer_types=["sliding_attention", "full_attention"], tie_word_embeddings=False)
+
+
+@pytest.mark.parametrize("kind", ["qwen3", "llama", "moe", "gpt_oss"])
+def test_generate_agrees_with_scoring(kind):
+    """``Trainer.generate`` on the cache against ``token_logprobs`` of the finished rows.  Two bf16 passes over two layers: some sixteen
+    independent roundings of 2^-9 leave 1 % on the hidden state, so 0.005 on logits of spread 0.5; six times that, and half a step (2^-8) of bf16
+    logits below 2 on the scoring side, stay below 0.05.  Routed experts may be chosen differently for single tokens; there the mean is held."""
+    import numpy as np
+
+    from surogate_b200.runtime import generation
+    from surogate_b200.runtime.trainer import Trainer, TrainerConfig
+
+    tr = Trainer(TrainerConfig(model=_model(kind), batch_size=4, seq_len=256, recipe="bf16"), device=torch.device("cuda:0"))
+    tr.init_weights(seed=0)
+    assert generation.cache_layout(tr.cm, tr.device) is not None
+    g = np.random.default_rng(0)
+    prompts = [g.integers(0, 4096, n).tolist() for n in (1, 100, 128, 213)]
+    before = _ops().ext().launch_count()
+    outs = tr.generate(prompts, n=3, max_new_tokens=40, temperature=1.0, top_p=0.9, seed=3, page_size=32, prompt_rows=3)
+    assert _ops().ext().launch_count() > before + 40 * 2 * 3
+    _no_errors()
+    for p, cs in zip(prompts, outs):
+        assert len({tuple(c.tokens) for c in cs}) == 3
+        rows = np.zeros((3, 256), np.int32)
+        for i, c in enumerate(cs):
+            rows[i, :len(p) + 40] = p + c.tokens
+        tgt = np.roll(rows, -1, axis=1)
+        want = tr.token_logprobs(np.vstack([rows, rows[:1]]), np.vstack([tgt, tgt[:1]]))[:3, len(p) - 1:len(p) + 39].cpu()
+        err = (torch.tensor([c.logprobs for c in cs]) - want).abs()
+        assert (err.max() if kind in ("qwen3", "llama") else err.mean()) < 0.05, err.max()
+    again = tr.generate(prompts, n=3, max_new_tokens=40, temperature=1.0, top_p=0.9, seed=3, page_size=32, prompt_rows=3)
+    if kind in ("qwen3", "llama"):
+        assert [c.tokens for cs in again for c in cs] == [c.tokens for cs in outs for c in cs]
+    small = tr.generate(prompts[:2], n=2, max_new_tokens=8, temperature=0.0, cache_dtype=E4M3)
+    assert all(len(c.tokens) == 8 and all(math.isfinite(x) for x in c.logprobs) for cs in small for c in cs)
+    _no_errors()
+
+
+def test_decode_step_of_a_forked_group_on_one_cache():
+    """Append, fork, diverge, compact, attend: one prompt's three completions on two layers of an e4m3 cache against caches that were never shared."""
+    L, H, D, P = 2, 2, 64, 16
+    g = torch.Generator().manual_seed(0)
+    shared, alone = (_ops().PagedKVCache(L, 40, P, H, D, 4, dtype=E4M3, device=DEV) for _ in range(2))
+    prompt = torch.randn(L, 2, 1, 21, H, D, generator=g).to(DEV).bfloat16()
+    new = torch.randn(30, L, 2, 3, 1, H, D, generator=g).to(DEV).bfloat16()
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    shared.reserve({0: 21})
+    for s in range(3):
+        alone.reserve({s: 21})
+    for layer in range(L):
+        shared.append(layer, prompt[layer, 0], prompt[layer, 1], shared.table([0]), zero)
+        for s in range(3):
+            alone.append(layer, prompt[layer, 0], prompt[layer, 1], alone.table([s]), zero)
+    shared.fork(0, [1, 2])
+    q = torch.randn(3, 4, D, generator=g).to(DEV).bfloat16()
+    for t in range(30):
+        start = torch.full((3,), 21 + t, dtype=torch.int32, device=DEV)
+        for c in (shared, alone):
+            c.reserve({0: 1, 1: 1, 2: 1})
+            for layer in range(L):
+                c.append(layer, new[t, layer, 0], new[t, layer, 1], c.table([0, 1, 2]), start)
+        if t == 15:
+            shared.fork(2, [3])
+            shared.free(2)
+            shared.fork(3, [2])
+            shared.free(3)
+            shared.compact()
+        for layer in range(L):
+            a, b = (c.attend(layer, q, c.table([0, 1, 2]), start + 1) for c in (shared, alone))
+            assert torch.equal(a, b)
+    assert shared.free_pages > alone.free_pages
+    _no_errors()
