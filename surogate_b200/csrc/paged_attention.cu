@@ -35,13 +35,18 @@ namespace sg {
 namespace {
 
 constexpr int kTile = 64, kWarps = 4, kStep = 16;   // keys a tile, warps a block, keys a warp and tile
+constexpr int RING_BYTES = 16384;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(valid ? 8 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { cp_async<16>(dst, src); }
+// zeros where not `valid`
+template <int N> __device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool valid) {
+    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -55,12 +60,17 @@ __device__ __forceinline__ uint2 lds8(uint32_t a) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ float lds4(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// d += a b: rows 0-7 of a in a0, a2, rows 8-15 in a1, a3
+// d[16 x 8] += a[16 x 16] b[16 x 8]
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if (BF16)
@@ -70,18 +80,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same where rows 8-15 of a are zero: only rows 0-7 of d are kept
-template <bool BF16>
-__device__ __forceinline__ void mma(float (&d)[2], uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
-    float z0, z1;
-    const uint32_t zero = 0;
-    const float fz = 0.f;
-    if (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
-            : "+f"(d[0]), "+f"(d[1]), "=f"(z0), "=f"(z1) : "r"(a0), "r"(zero), "r"(a2), "r"(b0), "r"(b1), "f"(fz));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
-            : "+f"(d[0]), "+f"(d[1]), "=f"(z0), "=f"(z1) : "r"(a0), "r"(zero), "r"(a2), "r"(b0), "r"(b1), "f"(fz));
+// An 8 x 8 matrix of 16-bit elements, two of a row in each lane, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -104,17 +107,19 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
 template <int KT, int D, int ROWS> struct Shape {
     static constexpr int ES = KT == kKvE4m3 ? 1 : 2;               // bytes of a cached element
     static constexpr bool BF16 = KT == kKvBf16;                    // operand type of the products: bf16, else fp16
+    static constexpr int HT = ROWS / 8;                            // groups of eight query heads
     static constexpr int KCH = D * ES / 64;                        // 16-byte pieces of a key row for each of the four lanes that share it
     static constexpr int VB = D * ES >= 128 ? 16 : 8;              // bytes of a piece of a value row, shared by eight lanes
     static constexpr int VCH = D * ES / (8 * VB);
     static constexpr int E = VB / ES;                              // elements of that piece
-    static constexpr int KBYTES = 2 * KCH * 512, VBYTES = 4 * VCH * VB * 32, SBYTES = KT == kKvE4m3 ? 4 * 8 * 32 : 0;
+    static constexpr int KBYTES = 2 * KCH * 512, VBYTES = 4 * VCH * VB * 32, SBYTES = KT == kKvE4m3 ? 4 * 4 * 32 : 0;
     static constexpr int STAGE = KBYTES + VBYTES + SBYTES;
-    static constexpr int STAGES = 24576 / STAGE > 8 ? 8 : 24576 / STAGE < 3 ? 3 : 24576 / STAGE;
+    static constexpr int STAGES = RING_BYTES / STAGE > 8 ? 8 : RING_BYTES / STAGE < 2 ? 2 : RING_BYTES / STAGE;
     static constexpr int RING = STAGE * STAGES;                    // of one warp; holds its ROWS x D fp32 outputs when warps meet
-    static constexpr int NT = D / 8;                               // n-tiles of the output
-    static constexpr int NACC = ROWS == 16 ? 4 : 2;
+    static constexpr int MT = D / 16;                              // tiles of 16 outputs
     static constexpr int SMEM = kWarps * RING;
+    static constexpr int FIT = 230000 / (SMEM + 2048);             // blocks that an SM's shared memory holds
+    static constexpr int PER_SM = FIT > 3 ? 3 : FIT;
     static_assert(RING >= ROWS * D * 4, "the ring holds a warp's outputs");
 };
 
@@ -144,18 +149,23 @@ template <> __device__ __forceinline__ __half from_float<__half>(float x) { retu
 template <int KT, typename QT, int D, int ROWS>
 struct Piece {
     using S = Shape<KT, D, ROWS>;
-    static constexpr bool HI = ROWS == 16;
-    // weights are carried as 2^15 times themselves where they become fp16, whose smallest step is 2^-24
-    static constexpr float kShift = S::BF16 ? 0.f : 15.f;
+    // weights are carried as 2^7 times themselves where they become fp16, whose smallest step is 2^-24; they are below 2^(kSlack) before
+    static constexpr float kShift = S::BF16 ? 0.f : 7.f, kSlack = 8.f;
 
     // Tiles [tb, te) of row b (tile numbers of the row's positions) and head group vh.  slot < 0: the whole row; its result is written.  Else the piece is.
     static __device__ void run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, uint8_t* smem, float2 (*sh_ml)[16]) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         const int G = p.Hq / p.kv.heads, kvh = vh / groups, h0 = kvh * G + (vh - kvh * groups) * ROWS, nrows = min(ROWS, kvh * G + G - h0);
         const int lo = first_key(p, n), steps = te - tb;
-        const uint32_t ring = smem_u32(smem) + warp * S::RING;
-        const char* kv0 = static_cast<const char*>(p.kv.data) + static_cast<int64_t>(kvh) * p.kv.head_stride * S::ES;
+        const uint32_t ring = smem_u32(smem) + warp * S::RING + lane * 16;
         const int* table = p.table + b * p.table_stride;
+        // Row r of a product's 16 keys is key 4 (r % 8 / 2) + r % 2, + 2 for r >= 8: so the four rows whose values a lane pairs (2c, 2c+1, 2c+8, 2c+9) are
+        // the keys 4c .. 4c+3, and the two rows whose keys it loads (g, g+8) are k0 and k0 + 2.
+        const int k0 = 4 * (g >> 1) + (g & 1);
+        const int64_t ts = p.kv.tok_stride * S::ES;
+        const char* k_lane = static_cast<const char*>(p.kv.data) + kvh * p.kv.head_stride * S::ES + k0 * ts + c * 16;
+        const char* v_lane = static_cast<const char*>(p.kv.data) + (kvh * p.kv.head_stride + p.kv.kv_stride) * S::ES + 4 * c * ts + g * S::VB;
+        const float* s_lane = KT == kKvE4m3 ? p.kv.scales + kvh * p.kv.s_head_stride + k0 : nullptr;
 
         // page of the warp's keys in step base + lane; -1: none of them counts
         auto load_pages = [&](int base) {
@@ -170,63 +180,74 @@ struct Piece {
         };
         int pages = load_pages(0), pages_next = load_pages(32);
         unsigned have = 0;            // bit i % 32: step i has a page
+        int next_t0 = tb * kTile + warp * kStep, next_place = next_t0 % p.kv.page_size, next_i = 0;   // the step that is requested next
+        const int place_step = kTile % p.kv.page_size;
+        uint32_t next_dst = ring;
 
-        auto issue = [&](int i) {
-            if ((i & 31) == 0 && i > 0) {
+        auto issue = [&]() {
+            if ((next_i & 31) == 0 && next_i > 0) {
                 pages = pages_next;
-                pages_next = load_pages(i + 32);
+                pages_next = load_pages(next_i + 32);
             }
-            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-            have = (have & ~(1u << (i & 31))) | (page >= 0 ? 1u << (i & 31) : 0u);
-            if (page < 0) return;
-            const int t0 = (tb + i) * kTile + warp * kStep, place = t0 % p.kv.page_size;
-            const uint32_t dst = ring + (i % S::STAGES) * S::STAGE;
-            const char* kb = kv0 + (page * p.kv.page_stride + place * p.kv.tok_stride) * S::ES;
-            const char* vb = kb + p.kv.kv_stride * S::ES;
+            const int page = __shfl_sync(0xffffffffu, pages, next_i & 31);
+            have = (have & ~(1u << (next_i & 31))) | (page >= 0 ? 1u << (next_i & 31) : 0u);
+            if (page >= 0) {
+                const int64_t at = (page * p.kv.page_stride + next_place * p.kv.tok_stride) * S::ES;
+                const char* kp = k_lane + at;
+                const char* vp = v_lane + at;
+                const uint32_t kd = next_dst, vd = S::VB == 16 ? next_dst + S::KBYTES : next_dst - lane * 8 + S::KBYTES;
+                if (next_t0 >= lo && next_t0 + kStep <= n) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int k = t * 8 + g;
-                const bool ok = t0 + k >= lo && t0 + k < n;
-                const char* src = kb + k * p.kv.tok_stride * S::ES + c * 16;
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int j = 0; j < S::KCH; ++j) cp_async16(dst + (t * S::KCH + j) * 512 + lane * 16, ok ? src + j * 64 : kv0, ok);
-            }
+                        for (int j = 0; j < S::KCH; ++j) cp_async16(kd + (t * S::KCH + j) * 512, kp + 2 * t * ts + j * 64);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int k = 2 * c + (t & 1) + (t >> 1) * 8;
-                const bool ok = t0 + k >= lo && t0 + k < n;
-                const char* src = vb + k * p.kv.tok_stride * S::ES + g * S::VB;
+                    for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int j = 0; j < S::VCH; ++j) {
-                    const uint32_t d = dst + S::KBYTES + (t * S::VCH + j) * (32 * S::VB) + lane * S::VB;
-                    if (S::VB == 16) cp_async16(d, ok ? src + j * 8 * S::VB : kv0, ok);
-                    else cp_async8(d, ok ? src + j * 8 * S::VB : kv0, ok);
+                        for (int j = 0; j < S::VCH; ++j) cp_async<S::VB>(vd + (t * S::VCH + j) * (32 * S::VB), vp + t * ts + j * 8 * S::VB);
+                } else {              // keys outside the row or its window become zeros
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const bool ok = next_t0 + k0 + 2 * t >= lo && next_t0 + k0 + 2 * t < n;
+#pragma unroll
+                        for (int j = 0; j < S::KCH; ++j) cp_async_if<16>(kd + (t * S::KCH + j) * 512, ok ? kp + 2 * t * ts + j * 64 : k_lane, ok);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const bool ok = next_t0 + 4 * c + t >= lo && next_t0 + 4 * c + t < n;
+#pragma unroll
+                        for (int j = 0; j < S::VCH; ++j) cp_async_if<S::VB>(vd + (t * S::VCH + j) * (32 * S::VB), ok ? vp + t * ts + j * 8 * S::VB : v_lane, ok);
+                    }
+                }
+                if (KT == kKvE4m3) {
+                    const float* sp = s_lane + page * p.kv.s_page_stride + next_place;
+                    const uint32_t sd = next_dst - lane * 12 + S::KBYTES + S::VBYTES;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) cp_async<4>(sd + t * 128, sp + (t >> 1) * p.kv.s_kv_stride + (t & 1) * 2);
                 }
             }
-            if (KT == kKvE4m3) {
-                const float* sc = p.kv.scales + page * p.kv.s_page_stride + kvh * p.kv.s_head_stride + place + 2 * c;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    cp_async8(dst + S::KBYTES + S::VBYTES + t * 256 + lane * 8, sc + (t >> 1) * p.kv.s_kv_stride + (t & 1) * 8, true);
-            }
+            ++next_i;
+            next_t0 += kTile;
+            next_place += place_step;
+            if (next_place >= p.kv.page_size) next_place -= p.kv.page_size;
+            next_dst = next_dst == ring + (S::STAGES - 1) * S::STAGE ? ring : next_dst + S::STAGE;
         };
 
 #pragma unroll
         for (int i = 0; i < S::STAGES - 1; ++i) {
-            if (i < steps) issue(i);
+            if (i < steps) issue();
             cp_commit();
         }
 
-        // the query, piece by piece as the keys lie
-        constexpr int QW = KT == kKvE4m3 ? 8 : 4;                  // words of one row for one 16-byte piece of keys
-        uint32_t q[HI ? 2 : 1][S::KCH][QW];
-        float mult[HI ? 2 : 1];                                    // what turns a product into a score
+        // the query, piece by piece as the keys lie: head g (+ 8)
+        constexpr int QW = KT == kKvE4m3 ? 8 : 4;                  // words of one head for one 16-byte piece of keys
+        uint32_t q[S::HT][S::KCH][QW];
+        float mult[S::HT][2];                                      // what turns a product with head 2c, 2c + 1 into a score
 #pragma unroll
-        for (int r = 0; r < (HI ? 2 : 1); ++r) {
+        for (int r = 0; r < S::HT; ++r) {
             const int row = g + 8 * r;
             const QT* src = static_cast<const QT*>(p.q) + b * p.q_b_stride + (h0 + (row < nrows ? row : 0)) * p.q_h_stride;
             constexpr int EL = 16 / S::ES;                         // elements of a piece
-            mult[r] = p.scale;
 #pragma unroll
             for (int j = 0; j < S::KCH; ++j) {
 #pragma unroll
@@ -236,176 +257,189 @@ struct Piece {
                     q[r][j][w] = v.x; q[r][j][w + 1] = v.y; q[r][j][w + 2] = v.z; q[r][j][w + 3] = v.w;
                 }
             }
-            if (KT == kKvE4m3 && sizeof(QT) == 2 && !S::BF16) {
-                constexpr bool QBF = std::is_same<QT, __nv_bfloat16>::value;
-                if (QBF) {                                         // bf16 -> fp16 of the same value over a power of two
-                    float amax = 0.f;
+            float own = p.scale;
+            if (KT == kKvE4m3 && std::is_same<QT, __nv_bfloat16>::value) {   // bf16 -> fp16 of the same value over a power of two
+                float amax = 0.f;
 #pragma unroll
-                    for (int j = 0; j < S::KCH; ++j)
+                for (int j = 0; j < S::KCH; ++j)
 #pragma unroll
-                        for (int w = 0; w < QW; ++w) {
-                            const float2 f = unpack2<true>(q[r][j][w]);
-                            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-                        }
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 100);
-                    const float down = __uint_as_float((127 - e) << 23);
-                    mult[r] *= __uint_as_float((127 + e) << 23);
+                    for (int w = 0; w < QW; ++w) {
+                        const float2 f = unpack2<true>(q[r][j][w]);
+                        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 100);
+                const float down = __uint_as_float((127 - e) << 23);
+                own *= __uint_as_float((127 + e) << 23);
 #pragma unroll
-                    for (int j = 0; j < S::KCH; ++j)
+                for (int j = 0; j < S::KCH; ++j)
 #pragma unroll
-                        for (int w = 0; w < QW; ++w) {
-                            const float2 f = unpack2<true>(q[r][j][w]);
-                            q[r][j][w] = pack2<false>(f.x * down, f.y * down);
-                        }
-                }
+                    for (int w = 0; w < QW; ++w) {
+                        const float2 f = unpack2<true>(q[r][j][w]);
+                        q[r][j][w] = pack2<false>(f.x * down, f.y * down);
+                    }
             }
-            if (p.softcap == 0.f) mult[r] *= kLog2e;
+            if (p.softcap == 0.f) own *= kLog2e;
+            mult[r][0] = __shfl_sync(0xffffffffu, own, 8 * c);     // lane 4 * head holds that head's
+            mult[r][1] = __shfl_sync(0xffffffffu, own, 8 * c + 4);
         }
         const float cap = p.softcap, inv_cap2 = cap != 0.f ? 2.f * kLog2e / cap : 0.f, cap2 = cap * kLog2e;
 
-        float o[S::NT][S::NACC];
-        float m[HI ? 2 : 1], l[HI ? 2 : 1];
+        // o[m][r]: outputs of two elements of the head and of heads 8 r + 2c, + 1: [0], [1] the first element's, [2], [3] the second's
+        float o[S::MT][S::HT][4];
+        // Weights are relative to 2^top, which follows the scores' maximum only when they exceed it by kSlack: most steps need no maximum over lanes.
+        float top[S::HT][2], l[S::HT][2];
 #pragma unroll
-        for (int i = 0; i < S::NT; ++i)
+        for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-            for (int k = 0; k < S::NACC; ++k) o[i][k] = 0.f;
+            for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-        for (int r = 0; r < (HI ? 2 : 1); ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+                for (int k = 0; k < 4; ++k) o[i][r][k] = 0.f;
+#pragma unroll
+        for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) { top[r][k] = -INFINITY; l[r][k] = 0.f; }
 
-        for (int i = 0; i < steps; ++i) {
-            if (i + S::STAGES - 1 < steps) issue(i + S::STAGES - 1);
+        uint32_t st = ring;
+        int t0 = tb * kTile + warp * kStep;
+        for (int i = 0; i < steps; ++i, t0 += kTile) {
+            if (i + S::STAGES - 1 < steps) issue();
             cp_commit();
             cp_wait<S::STAGES - 1>();
+            const uint32_t at = st;
+            st = st == ring + (S::STAGES - 1) * S::STAGE ? ring : st + S::STAGE;
             if (!((have >> (i & 31)) & 1)) continue;
-            const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
 
-            // scores of 16 keys: s[t][.] columns are keys t * 8 + 2c, + 1
-            float s[2][S::NACC];
+            // scores of 16 keys: s[r][0], [1] are key k0 with heads 8 r + 2c, + 1, s[r][2], [3] key k0 + 2
+            float s[S::HT][4], s2[S::HT][4];                       // two sums, so that products do not wait for one another
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-                for (int k = 0; k < S::NACC; ++k) s[t][k] = 0.f;
+                for (int k = 0; k < 4; ++k) s[r][k] = s2[r][k] = 0.f;
 #pragma unroll
-                for (int j = 0; j < S::KCH; ++j) {
-                    const uint4 kk = lds16(st + (t * S::KCH + j) * 512 + lane * 16);
-                    if (KT != kKvE4m3) {
-                        mma<S::BF16>(s[t], q[0][j][0], q[HI][j][0], q[0][j][1], q[HI][j][1], kk.x, kk.y);
-                        mma<S::BF16>(s[t], q[0][j][2], q[HI][j][2], q[0][j][3], q[HI][j][3], kk.z, kk.w);
-                    } else {
-                        const uint32_t kw[4] = {kk.x, kk.y, kk.z, kk.w};
+            for (int j = 0; j < S::KCH; ++j) {
+                const uint4 ka = lds16(at + j * 512), kb = lds16(at + (S::KCH + j) * 512);
+                if (KT != kKvE4m3) {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            mma<false>(s[t], q[0][j][(2 * w) % QW], q[HI][j][(2 * w) % QW], q[0][j][(2 * w + 1) % QW], q[HI][j][(2 * w + 1) % QW],
-                                       e4m3x2_to_f16x2(static_cast<uint16_t>(kw[w])), e4m3x2_to_f16x2(static_cast<uint16_t>(kw[w] >> 16)));
+                    for (int r = 0; r < S::HT; ++r) {
+                        mma<S::BF16>(s[r], ka.x, kb.x, ka.y, kb.y, q[r][j][0], q[r][j][1]);
+                        mma<S::BF16>(s2[r], ka.z, kb.z, ka.w, kb.w, q[r][j][2], q[r][j][3]);
+                    }
+                } else {
+                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w])), a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w] >> 16));
+                        const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w])), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w] >> 16));
+#pragma unroll
+                        for (int r = 0; r < S::HT; ++r) mma<false>((w & 1) ? s2[r] : s[r], a0, a1, a2, a3, q[r][j][(2 * w) % QW], q[r][j][(2 * w + 1) % QW]);
                     }
                 }
             }
-            float lv[2][2];                                        // log2 of the values' scales
+            float lv[2] = {0.f, 0.f};                              // log2 of the two keys' value scales
             if (KT == kKvE4m3) {
+                const uint32_t sa = at - lane * 12 + S::KBYTES + S::VBYTES;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const uint2 ks = lds8(st + S::KBYTES + S::VBYTES + t * 256 + lane * 8), vs = lds8(st + S::KBYTES + S::VBYTES + (2 + t) * 256 + lane * 8);
+                    const float ks = lds4(sa + t * 128);
 #pragma unroll
-                    for (int k = 0; k < S::NACC; ++k) s[t][k] *= __uint_as_float((k & 1) ? ks.y : ks.x);
-                    lv[t][0] = __log2f(fmaxf(__uint_as_float(vs.x), 0x1p-100f));
-                    lv[t][1] = __log2f(fmaxf(__uint_as_float(vs.y), 0x1p-100f));
+                    for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
+                    lv[t] = __log2f(fmaxf(lds4(sa + (2 + t) * 128), 0x1p-100f));
                 }
             }
-            const int t0 = (tb + i) * kTile + warp * kStep;
             const bool full = t0 >= lo && t0 + kStep <= n;
-            float mx[HI ? 2 : 1];
+            bool above = false;
 #pragma unroll
-            for (int r = 0; r < (HI ? 2 : 1); ++r) mx[r] = -INFINITY;
+            for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int k = 0; k < S::NACC; ++k) {
-                    float x = s[t][k] * mult[k >> 1];
+                for (int k = 0; k < 4; ++k) {
+                    float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
                     if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
-                    const int key = t0 + t * 8 + 2 * c + (k & 1);
-                    if (!full && (key < lo || key >= n)) x = -INFINITY;
-                    s[t][k] = x;
-                    mx[k >> 1] = fmaxf(mx[k >> 1], KT == kKvE4m3 ? (x == -INFINITY ? x : x + lv[t][k & 1]) : x);
+                    if (!full) {
+                        const int key = t0 + k0 + (k & 2);
+                        if (key < lo || key >= n) { x = -INFINITY; if (KT == kKvE4m3) lv[k >> 1] = 0.f; }
+                    }
+                    s[r][k] = x;
+                    above |= x + lv[k >> 1] > top[r][k & 1] + kSlack;
                 }
-            bool grew = false;
-            float fac[HI ? 2 : 1];
+            if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-            for (int r = 0; r < (HI ? 2 : 1); ++r) {
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                const float mn = fmaxf(m[r], mx[r]);
-                grew |= mn > m[r];
-                fac[r] = mn == -INFINITY ? 1.f : ex2(m[r] - mn);
-                m[r] = mn;
+                for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float mx = fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        mx = fmaxf(mx, top[r][h]);
+                        const float f = mx == -INFINITY ? 1.f : ex2(top[r][h] - mx);
+                        top[r][h] = mx;
+                        l[r][h] *= f;
+#pragma unroll
+                        for (int m = 0; m < S::MT; ++m) { o[m][r][h] *= f; o[m][r][2 + h] *= f; }
+                    }
             }
-            if (__any_sync(0xffffffffu, grew)) {
+            // weights, transposed to the right operand of the second product: rows of eight keys
+            uint32_t ph[S::HT][2], pl[S::HT][2];
 #pragma unroll
-                for (int r = 0; r < (HI ? 2 : 1); ++r) l[r] *= fac[r];
+            for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-                for (int nt = 0; nt < S::NT; ++nt)
-#pragma unroll
-                    for (int k = 0; k < S::NACC; ++k) o[nt][k] *= fac[k >> 1];
-            }
-            // weights, as the left operand of the second product: keys 2c, 2c+1 of the first eight (a0, a1), of the second (a2, a3)
-            uint32_t ph[2][HI ? 2 : 1], pl[2][HI ? 2 : 1];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < (HI ? 2 : 1); ++r) {
-                    const float mr = m[r] == -INFINITY ? 0.f : m[r];
-                    const float e0 = ex2(s[t][2 * r] - mr), e1 = ex2(s[t][2 * r + 1] - mr);
-                    l[r] += e0 + e1;
+                for (int t = 0; t < 2; ++t) {
+                    const float m0 = top[r][0] == -INFINITY ? 0.f : top[r][0], m1 = top[r][1] == -INFINITY ? 0.f : top[r][1];
+                    const float x0 = s[r][2 * t] - m0, x1 = s[r][2 * t + 1] - m1;
+                    const float e0 = ex2(x0), e1 = ex2(x1);
+                    l[r][0] += e0;
+                    l[r][1] += e1;
                     float w0 = e0, w1 = e1;
                     if (KT == kKvE4m3) {
-                        w0 = s[t][2 * r] == -INFINITY ? 0.f : ex2(s[t][2 * r] - mr + lv[t][0] + kShift);
-                        w1 = s[t][2 * r + 1] == -INFINITY ? 0.f : ex2(s[t][2 * r + 1] - mr + lv[t][1] + kShift);
+                        w0 = ex2(x0 + (lv[t] + kShift));
+                        w1 = ex2(x1 + (lv[t] + kShift));
                     } else if (kShift != 0.f) {
-                        w0 *= 32768.f;
-                        w1 *= 32768.f;
+                        w0 *= 128.f;
+                        w1 *= 128.f;
                     }
-                    ph[t][r] = pack2<S::BF16>(w0, w1);
+                    ph[r][t] = pack2<S::BF16>(w0, w1);
                     if (KT != kKvE4m3) {
-                        const float2 back = unpack2<S::BF16>(ph[t][r]);
-                        pl[t][r] = pack2<S::BF16>(w0 - back.x, w1 - back.y);
+                        const float2 back = unpack2<S::BF16>(ph[r][t]);
+                        pl[r][t] = transpose8(pack2<S::BF16>(w0 - back.x, w1 - back.y));
                     }
+                    ph[r][t] = transpose8(ph[r][t]);
                 }
-            // o += weights . values; the lane's piece of the value rows is column g of E n-tiles
+            // o += values . weights; a lane's piece of the value rows is row g (and g + 8: the next element) of E / 2 tiles
 #pragma unroll
             for (int j = 0; j < S::VCH; ++j) {
                 uint32_t v[4][S::VB / 4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const uint32_t a = st + S::KBYTES + (t * S::VCH + j) * (32 * S::VB) + lane * S::VB;
                     if (S::VB == 16) {
-                        const uint4 x = lds16(a);
+                        const uint4 x = lds16(at + S::KBYTES + (t * S::VCH + j) * 512);
                         v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
                     } else {
-                        const uint2 x = lds8(a);
+                        const uint2 x = lds8(at - lane * 8 + S::KBYTES + (t * S::VCH + j) * 256);
                         v[t][0] = x.x; v[t][1] = x.y;
                     }
                 }
 #pragma unroll
                 for (int w = 0; w < S::VB / 4; ++w) {
                     if (KT != kKvE4m3) {
+                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+                        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t sel = x ? 0x7632 : 0x5410;
-                            const uint32_t b0 = __byte_perm(v[0][w], v[1][w], sel), b1 = __byte_perm(v[2][w], v[3][w], sel);
-                            float (&acc)[S::NACC] = o[j * S::E + 2 * w + x];
-                            mma<S::BF16>(acc, ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], b0, b1);
-                            mma<S::BF16>(acc, pl[0][0], pl[0][HI], pl[1][0], pl[1][HI], b0, b1);
+                        for (int r = 0; r < S::HT; ++r) {
+                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
                         }
                     } else {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const uint32_t sel = x ? 0x7362 : 0x5140;
-                            const uint32_t b0 = __byte_perm(v[0][w], v[1][w], sel), b1 = __byte_perm(v[2][w], v[3][w], sel);
-                            mma<false>(o[j * S::E + 4 * w + 2 * x], ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], e4m3x2_to_f16x2(static_cast<uint16_t>(b0)),
-                                       e4m3x2_to_f16x2(static_cast<uint16_t>(b1)));
-                            mma<false>(o[j * S::E + 4 * w + 2 * x + 1], ph[0][0], ph[0][HI], ph[1][0], ph[1][HI], e4m3x2_to_f16x2(static_cast<uint16_t>(b0 >> 16)),
-                                       e4m3x2_to_f16x2(static_cast<uint16_t>(b1 >> 16)));
+                            const uint32_t u = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
+                            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(u)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(u >> 16));
+                            const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
+#pragma unroll
+                            for (int r = 0; r < S::HT; ++r) mma<false>(o[j * S::E / 2 + 2 * w + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
                         }
                     }
                 }
@@ -415,26 +449,32 @@ struct Piece {
 
         // the four warps meet
 #pragma unroll
-        for (int r = 0; r < (HI ? 2 : 1); ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (c == 0) sh_ml[warp][g + 8 * r] = make_float2(m[r], l[r]);
-        }
+        for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[r][h] += __shfl_xor_sync(0xffffffffu, l[r][h], x);
+                if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(top[r][h], l[r][h]);
+            }
         __syncthreads();
         float* mine = reinterpret_cast<float*>(smem + warp * S::RING);
 #pragma unroll
-        for (int r = 0; r < (HI ? 2 : 1); ++r) {
-            float mm = -INFINITY;
+        for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][g + 8 * r].x);
-            const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - mm);
+            for (int h = 0; h < 2; ++h) {
+                const int head = 8 * r + 2 * c + h;
+                float mm = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < S::VCH; ++j)
+                for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][head].x);
+                const float f = top[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
 #pragma unroll
-                for (int col = 0; col < 2; ++col)
+                for (int j = 0; j < S::VCH; ++j)
 #pragma unroll
-                    for (int e = 0; e < S::E; ++e) mine[(g + 8 * r) * D + (j * 8 + 2 * c + col) * S::E + e] = o[j * S::E + e][2 * r + col] * f;
-        }
+                    for (int e = 0; e < S::E; e += 2) {
+                        const float (&acc)[4] = o[(j * S::E + e) / 2][r];
+                        *reinterpret_cast<float2*>(mine + head * D + (j * 8 + g) * S::E + e) = make_float2(acc[h] * f, acc[2 + h] * f);
+                    }
+            }
         __syncthreads();
         for (int x = threadIdx.x; x < nrows * D; x += kWarps * 32) {
             const int row = x / D, d = x - row * D;
@@ -460,7 +500,7 @@ struct Piece {
     static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float acc) {
         float total = ll;
         if (p.sinks) total += ex2(p.sinks[h] * kLog2e - mm);       // infinite where the sink outweighs all keys by 2^128: the output is 0
-        const float y = mm == -INFINITY ? 0.f : acc * (S::BF16 ? 1.f : 0x1p-15f) / total;
+        const float y = mm == -INFINITY ? 0.f : acc * (S::BF16 ? 1.f : 0x1p-7f) / total;
         static_cast<QT*>(p.out)[(static_cast<int64_t>(b) * p.Hq + h) * D + d] = from_float<QT>(y);
         if (d == 0 && p.lse) p.lse[static_cast<int64_t>(b) * p.Hq + h] = mm == -INFINITY ? -INFINITY : mm * kLn2 + logf(ll);
     }
@@ -480,7 +520,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(Page
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  A block's first and
 // last piece may be part of a row; each goes to a slot of its own.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) paged_attention_shared_kernel(PagedAttention p, Cut cut, int groups) {
+__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) paged_attention_shared_kernel(PagedAttention p, Cut cut, int groups) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float2 sh_ml[kWarps][16];
     __shared__ long long sh_sum[kWarps];
@@ -622,6 +662,14 @@ const char* launch_dim(const PagedAttention& p, const PagedAttentionPlan& plan, 
 
 }  // namespace
 
+namespace {
+template <int KT> int blocks_per_sm(int dim, int rows) {
+    if (dim == 64) return rows == 16 ? Shape<KT, 64, 16>::PER_SM : Shape<KT, 64, 8>::PER_SM;
+    if (dim == 128) return rows == 16 ? Shape<KT, 128, 16>::PER_SM : Shape<KT, 128, 8>::PER_SM;
+    return Shape<KT, 256, 8>::PER_SM;
+}
+}  // namespace
+
 PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_type, int64_t max_keys, int num_sms) {
     PagedAttentionPlan plan{};
     const int G = Hq / Hkv;
@@ -631,7 +679,8 @@ PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_
     plan.head_groups = (G + plan.rows - 1) / plan.rows;
     const int64_t pairs = static_cast<int64_t>(B) * Hkv * plan.head_groups, tiles = (max_keys + kTile - 1) / kTile;
     plan.whole = tiles <= 8;
-    plan.blocks = static_cast<int>(pairs * tiles < 2 * num_sms ? (pairs * tiles > 0 ? pairs * tiles : 1) : 2 * num_sms);
+    const int most = num_sms * (kv_type == kKvE4m3 ? blocks_per_sm<kKvE4m3>(dim, plan.rows) : blocks_per_sm<kKvBf16>(dim, plan.rows));
+    plan.blocks = static_cast<int>(pairs * tiles < most ? (pairs * tiles > 0 ? pairs * tiles : 1) : most);
     plan.workspace_floats = plan.whole ? 0 : 2 * (static_cast<int64_t>(B) + 2) + static_cast<int64_t>(plan.blocks) * 2 * plan.rows * (dim + 2);
     return plan;
 }
