@@ -63,8 +63,8 @@ sg::KvPages pages_of(const Tensor& kv, const OptTensor& scales) {
         TORCH_CHECK(s.device() == kv.device() && s.scalar_type() == at::kFloat && s.dim() == 4 && s.size(0) == kv.size(0) && s.size(1) == 2 && s.size(2) == kv.size(2) &&
                         s.size(3) == kv.size(3),
                     "scales must be fp32 [pages, 2, kv heads, page size] on the cache's device");
-        TORCH_CHECK(s.stride(3) == 1 && aligned(s.data_ptr(), 8) && s.stride(0) % 2 == 0 && s.stride(1) % 2 == 0 && s.stride(2) % 2 == 0,
-                    "scales: the places of a page must be contiguous and 8-byte aligned");
+        TORCH_CHECK(s.stride(3) == 1 && aligned(s.data_ptr(), 16) && s.stride(0) % 4 == 0 && s.stride(1) % 4 == 0 && s.stride(2) % 4 == 0,
+                    "scales: the places of a page must be contiguous and 16-byte aligned");
         k.scales = s.data_ptr<float>();
         k.s_page_stride = s.stride(0);
         k.s_kv_stride = s.stride(1);

@@ -38,18 +38,6 @@ constexpr int kTile = 64, kWarps = 4, kStep = 16;   // keys a tile, warps a bloc
 constexpr int RING_BYTES = 16384;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { cp_async<16>(dst, src); }
-// zeros where not `valid`
-template <int N> __device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool valid) {
-    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -112,15 +100,27 @@ template <int KT, int D, int ROWS> struct Shape {
     static constexpr int VB = D * ES >= 128 ? 16 : 8;              // bytes of a piece of a value row, shared by eight lanes
     static constexpr int VCH = D * ES / (8 * VB);
     static constexpr int E = VB / ES;                              // elements of that piece
-    static constexpr int KBYTES = 2 * KCH * 512, VBYTES = 4 * VCH * VB * 32, SBYTES = KT == kKvE4m3 ? 4 * 4 * 32 : 0;
-    static constexpr int STAGE = KBYTES + VBYTES + SBYTES;
+    static constexpr int ROWB = D * ES;                            // bytes of a row
+    static constexpr int PITCH = ROWB < 128 ? ROWB : 128;          // of a row in shared memory: wider ones are copied 128 bytes at a time
+    static constexpr int BOXES = ROWB / PITCH, BOXEL = PITCH / ES, BOXBYTES = kStep * PITCH;
+    static constexpr int KBYTES = kStep * ROWB;                    // a warp's keys of one step; its values take as much
+    static constexpr int STAGE = 2 * KBYTES + (KT == kKvE4m3 ? 1024 : 0);   // swizzled tiles begin on 1024 bytes
     static constexpr int STAGES = RING_BYTES / STAGE > 8 ? 8 : RING_BYTES / STAGE < 2 ? 2 : RING_BYTES / STAGE;
-    static constexpr int RING = STAGE * STAGES;                    // of one warp; holds its ROWS x D fp32 outputs when warps meet
+    static constexpr int RING = STAGE * STAGES;                    // of one warp
     static constexpr int MT = D / 16;                              // tiles of 16 outputs
-    static constexpr int SMEM = kWarps * RING;
+    static constexpr int MEET = kWarps * ROWS * D * 4;             // where the warps' outputs meet
+    static constexpr int SMEM = 1024 + kWarps * RING + MEET;
     static constexpr int FIT = 230000 / (SMEM + 2048);             // blocks that an SM's shared memory holds
     static constexpr int PER_SM = FIT > 3 ? 3 : FIT;
-    static_assert(RING >= ROWS * D * 4, "the ring holds a warp's outputs");
+};
+
+struct Ring {            // a warp's copies under way
+    const CUtensorMap* map;
+    uint32_t base, bars;  // shared memory: all warps' rings, one barrier for each slot
+    float* meet;
+    volatile int* abort_flag;
+    int slot;             // the next step's
+    uint32_t parity;
 };
 
 struct Cut {             // where the pieces of a shared problem go
@@ -146,26 +146,53 @@ template <typename QT> __device__ __forceinline__ QT from_float(float x);
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, int c4, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+        : "memory");
+}
+
 template <int KT, typename QT, int D, int ROWS>
 struct Piece {
     using S = Shape<KT, D, ROWS>;
     // weights are carried as 2^7 times themselves where they become fp16, whose smallest step is 2^-24; they are below 2^(kSlack) before
     static constexpr float kShift = S::BF16 ? 0.f : 7.f, kSlack = 8.f;
 
+    static __device__ Ring begin(const CUtensorMap* map, uint8_t* smem, unsigned long long* bars, int* abort_flag) {
+        uint8_t* at = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~uintptr_t{1023});
+        if (threadIdx.x == 0) *abort_flag = 0;
+        if (threadIdx.x < kWarps * S::STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
+        fence_barrier_init();
+        __syncthreads();
+        return Ring{map, smem_u32(at), smem_u32(bars), reinterpret_cast<float*>(at + kWarps * S::RING), abort_flag, 0, 0};
+    }
+    static __device__ void end(const PagedAttention& p, const int* abort_flag) {
+        if (threadIdx.x == 0 && *abort_flag) atomicExch(p.error_flag, 1);
+    }
+
     // Tiles [tb, te) of row b (tile numbers of the row's positions) and head group vh.  slot < 0: the whole row; its result is written.  Else the piece is.
-    static __device__ void run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, uint8_t* smem, float2 (*sh_ml)[16]) {
+    static __device__ void run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, Ring& rg, float2 (*sh_ml)[16]) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         const int G = p.Hq / p.kv.heads, kvh = vh / groups, h0 = kvh * G + (vh - kvh * groups) * ROWS, nrows = min(ROWS, kvh * G + G - h0);
         const int lo = first_key(p, n), steps = te - tb;
-        const uint32_t ring = smem_u32(smem) + warp * S::RING + lane * 16;
+        const uint32_t ring = rg.base + warp * S::RING, bars = rg.bars + warp * S::STAGES * 8;
         const int* table = p.table + b * p.table_stride;
-        // Row r of a product's 16 keys is key 4 (r % 8 / 2) + r % 2, + 2 for r >= 8: so the four rows whose values a lane pairs (2c, 2c+1, 2c+8, 2c+9) are
-        // the keys 4c .. 4c+3, and the two rows whose keys it loads (g, g+8) are k0 and k0 + 2.
-        const int k0 = 4 * (g >> 1) + (g & 1);
-        const int64_t ts = p.kv.tok_stride * S::ES;
-        const char* k_lane = static_cast<const char*>(p.kv.data) + kvh * p.kv.head_stride * S::ES + k0 * ts + c * 16;
-        const char* v_lane = static_cast<const char*>(p.kv.data) + (kvh * p.kv.head_stride + p.kv.kv_stride) * S::ES + 4 * c * ts + g * S::VB;
-        const float* s_lane = KT == kKvE4m3 ? p.kv.scales + kvh * p.kv.s_head_stride + k0 : nullptr;
+        // Row r of a product's 16 keys is key r, or r ^ 4 where r is odd.  With the order in which the copies swizzle a row's 16-byte pieces (piece ^ row % 8),
+        // neither the lanes that read keys (row g) nor those that read values (rows 2c, 2c + 1) then meet in a bank.
+        const int k0 = (g & 1) ? g ^ 4 : g;                        // this lane's first key; its second is 8 further on
+        const int v0 = 2 * c, v1 = (2 * c ^ 4) + 1;                // rows 2c and 2c + 1, whose values it pairs; then the same 8 further on
+        uint32_t k_off[2], v_off[2];
+        if (S::ROWB >= 128) {
+            k_off[0] = k0 * 128 + ((c ^ (k0 & 7)) << 4);
+            k_off[1] = k_off[0] ^ 64;
+            v_off[0] = S::KBYTES + v0 * 128 + ((g ^ (v0 & 7)) << 4);
+            v_off[1] = S::KBYTES + v1 * 128 + ((g ^ (v1 & 7)) << 4);
+        } else {                                                   // rows of 64 bytes: piece ^ row / 2 % 4
+            k_off[0] = k_off[1] = k0 * 64 + ((c ^ ((k0 >> 1) & 3)) << 4);
+            v_off[0] = S::KBYTES + v0 * 64 + (((g >> 1) ^ ((v0 >> 1) & 3)) << 4) + (g & 1) * 8;
+            v_off[1] = S::KBYTES + v1 * 64 + (((g >> 1) ^ ((v1 >> 1) & 3)) << 4) + (g & 1) * 8;
+        }
 
         // page of the warp's keys in step base + lane; -1: none of them counts
         auto load_pages = [&](int base) {
@@ -180,64 +207,39 @@ struct Piece {
         };
         int pages = load_pages(0), pages_next = load_pages(32);
         unsigned have = 0;            // bit i % 32: step i has a page
-        int next_t0 = tb * kTile + warp * kStep, next_place = next_t0 % p.kv.page_size, next_i = 0;   // the step that is requested next
+        int next_i = 0, next_place = (tb * kTile + warp * kStep) % p.kv.page_size;   // the step that is requested next
         const int place_step = kTile % p.kv.page_size;
-        uint32_t next_dst = ring;
 
-        auto issue = [&]() {
+        // Request the next step into slot `to`.  A step without a page has coordinates outside the cache: zeros, and nothing is read.
+        auto issue = [&](int to) {
             if ((next_i & 31) == 0 && next_i > 0) {
                 pages = pages_next;
                 pages_next = load_pages(next_i + 32);
             }
             const int page = __shfl_sync(0xffffffffu, pages, next_i & 31);
             have = (have & ~(1u << (next_i & 31))) | (page >= 0 ? 1u << (next_i & 31) : 0u);
-            if (page >= 0) {
-                const int64_t at = (page * p.kv.page_stride + next_place * p.kv.tok_stride) * S::ES;
-                const char* kp = k_lane + at;
-                const char* vp = v_lane + at;
-                const uint32_t kd = next_dst, vd = S::VB == 16 ? next_dst + S::KBYTES : next_dst - lane * 8 + S::KBYTES;
-                if (next_t0 >= lo && next_t0 + kStep <= n) {
+            if (lane == 0) {
+                const uint32_t dst = ring + to * S::STAGE, bar = bars + to * 8;
+                const bool scaled = KT == kKvE4m3 && page >= 0;
+                mbar_expect_tx(bar, 2 * S::KBYTES + (scaled ? 128 : 0));
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int x = 0; x < S::BOXES; ++x) tma_load_5d(dst + x * S::BOXBYTES, rg.map, x * S::BOXEL, next_place, kvh, 0, page, bar);
 #pragma unroll
-                        for (int j = 0; j < S::KCH; ++j) cp_async16(kd + (t * S::KCH + j) * 512, kp + 2 * t * ts + j * 64);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int j = 0; j < S::VCH; ++j) cp_async<S::VB>(vd + (t * S::VCH + j) * (32 * S::VB), vp + t * ts + j * 8 * S::VB);
-                } else {              // keys outside the row or its window become zeros
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const bool ok = next_t0 + k0 + 2 * t >= lo && next_t0 + k0 + 2 * t < n;
-#pragma unroll
-                        for (int j = 0; j < S::KCH; ++j) cp_async_if<16>(kd + (t * S::KCH + j) * 512, ok ? kp + 2 * t * ts + j * 64 : k_lane, ok);
-                    }
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const bool ok = next_t0 + 4 * c + t >= lo && next_t0 + 4 * c + t < n;
-#pragma unroll
-                        for (int j = 0; j < S::VCH; ++j) cp_async_if<S::VB>(vd + (t * S::VCH + j) * (32 * S::VB), ok ? vp + t * ts + j * 8 * S::VB : v_lane, ok);
-                    }
-                }
-                if (KT == kKvE4m3) {
-                    const float* sp = s_lane + page * p.kv.s_page_stride + next_place;
-                    const uint32_t sd = next_dst - lane * 12 + S::KBYTES + S::VBYTES;
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) cp_async<4>(sd + t * 128, sp + (t >> 1) * p.kv.s_kv_stride + (t & 1) * 2);
+                for (int x = 0; x < S::BOXES; ++x) tma_load_5d(dst + S::KBYTES + x * S::BOXBYTES, rg.map, x * S::BOXEL, next_place, kvh, 1, page, bar);
+                if (scaled) {
+                    const float* sp = p.kv.scales + page * p.kv.s_page_stride + kvh * p.kv.s_head_stride + next_place;
+                    bulk_load(dst + 2 * S::KBYTES, sp, 64, bar);
+                    bulk_load(dst + 2 * S::KBYTES + 64, sp + p.kv.s_kv_stride, 64, bar);
                 }
             }
             ++next_i;
-            next_t0 += kTile;
             next_place += place_step;
             if (next_place >= p.kv.page_size) next_place -= p.kv.page_size;
-            next_dst = next_dst == ring + (S::STAGES - 1) * S::STAGE ? ring : next_dst + S::STAGE;
         };
-
+        // all slots are free here: the step that this piece begins with goes to rg.slot
 #pragma unroll
-        for (int i = 0; i < S::STAGES - 1; ++i) {
-            if (i < steps) issue();
-            cp_commit();
-        }
+        for (int i = 0; i < S::STAGES; ++i)
+            if (i < steps) issue(rg.slot + i < S::STAGES ? rg.slot + i : rg.slot + i - S::STAGES);
 
         // the query, piece by piece as the keys lie: head g (+ 8)
         constexpr int QW = KT == kKvE4m3 ? 8 : 4;                  // words of one head for one 16-byte piece of keys
@@ -301,151 +303,158 @@ struct Piece {
 #pragma unroll
             for (int k = 0; k < 2; ++k) { top[r][k] = -INFINITY; l[r][k] = 0.f; }
 
-        uint32_t st = ring;
         int t0 = tb * kTile + warp * kStep;
         for (int i = 0; i < steps; ++i, t0 += kTile) {
-            if (i + S::STAGES - 1 < steps) issue();
-            cp_commit();
-            cp_wait<S::STAGES - 1>();
-            const uint32_t at = st;
-            st = st == ring + (S::STAGES - 1) * S::STAGE ? ring : st + S::STAGE;
-            if (!((have >> (i & 31)) & 1)) continue;
-
-            // scores of 16 keys: s[r][0], [1] are key k0 with heads 8 r + 2c, + 1, s[r][2], [3] key k0 + 2
-            float s[S::HT][4], s2[S::HT][4];                       // two sums, so that products do not wait for one another
-#pragma unroll
-            for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[r][k] = s2[r][k] = 0.f;
-#pragma unroll
-            for (int j = 0; j < S::KCH; ++j) {
-                const uint4 ka = lds16(at + j * 512), kb = lds16(at + (S::KCH + j) * 512);
-                if (KT != kKvE4m3) {
-#pragma unroll
-                    for (int r = 0; r < S::HT; ++r) {
-                        mma<S::BF16>(s[r], ka.x, kb.x, ka.y, kb.y, q[r][j][0], q[r][j][1]);
-                        mma<S::BF16>(s2[r], ka.z, kb.z, ka.w, kb.w, q[r][j][2], q[r][j][3]);
-                    }
-                } else {
-                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w])), a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w] >> 16));
-                        const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w])), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w] >> 16));
-#pragma unroll
-                        for (int r = 0; r < S::HT; ++r) mma<false>((w & 1) ? s2[r] : s[r], a0, a1, a2, a3, q[r][j][(2 * w) % QW], q[r][j][(2 * w + 1) % QW]);
-                    }
-                }
-            }
-            float lv[2] = {0.f, 0.f};                              // log2 of the two keys' value scales
-            if (KT == kKvE4m3) {
-                const uint32_t sa = at - lane * 12 + S::KBYTES + S::VBYTES;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const float ks = lds4(sa + t * 128);
-#pragma unroll
-                    for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
-                    lv[t] = __log2f(fmaxf(lds4(sa + (2 + t) * 128), 0x1p-100f));
-                }
-            }
-            const bool full = t0 >= lo && t0 + kStep <= n;
-            bool above = false;
-#pragma unroll
-            for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
-                    if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
-                    if (!full) {
-                        const int key = t0 + k0 + (k & 2);
-                        if (key < lo || key >= n) { x = -INFINITY; if (KT == kKvE4m3) lv[k >> 1] = 0.f; }
-                    }
-                    s[r][k] = x;
-                    above |= x + lv[k >> 1] > top[r][k & 1] + kSlack;
-                }
-            if (__any_sync(0xffffffffu, above)) {
+            if (!mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag)) break;
+            const uint32_t at = ring + rg.slot * S::STAGE;
+            if ((have >> (i & 31)) & 1) {
+                // scores of 16 keys: s[r][0], [1] are key k0 with heads 8 r + 2c, + 1, s[r][2], [3] key k0 + 8
+                float s[S::HT][4], s2[S::HT][4];                       // two sums, so that products do not wait for one another
 #pragma unroll
                 for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float mx = fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]);
+                    for (int k = 0; k < 4; ++k) s[r][k] = s2[r][k] = 0.f;
 #pragma unroll
-                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                        mx = fmaxf(mx, top[r][h]);
-                        const float f = mx == -INFINITY ? 1.f : ex2(top[r][h] - mx);
-                        top[r][h] = mx;
-                        l[r][h] *= f;
-#pragma unroll
-                        for (int m = 0; m < S::MT; ++m) { o[m][r][h] *= f; o[m][r][2 + h] *= f; }
-                    }
-            }
-            // weights, transposed to the right operand of the second product: rows of eight keys
-            uint32_t ph[S::HT][2], pl[S::HT][2];
-#pragma unroll
-            for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const float m0 = top[r][0] == -INFINITY ? 0.f : top[r][0], m1 = top[r][1] == -INFINITY ? 0.f : top[r][1];
-                    const float x0 = s[r][2 * t] - m0, x1 = s[r][2 * t + 1] - m1;
-                    const float e0 = ex2(x0), e1 = ex2(x1);
-                    l[r][0] += e0;
-                    l[r][1] += e1;
-                    float w0 = e0, w1 = e1;
-                    if (KT == kKvE4m3) {
-                        w0 = ex2(x0 + (lv[t] + kShift));
-                        w1 = ex2(x1 + (lv[t] + kShift));
-                    } else if (kShift != 0.f) {
-                        w0 *= 128.f;
-                        w1 *= 128.f;
-                    }
-                    ph[r][t] = pack2<S::BF16>(w0, w1);
+                for (int j = 0; j < S::KCH; ++j) {
+                    const uint32_t kp = at + k_off[j & 1] + (j >> 1) * S::BOXBYTES;
+                    const uint4 ka = lds16(kp), kb = lds16(kp + 8 * S::PITCH);
                     if (KT != kKvE4m3) {
-                        const float2 back = unpack2<S::BF16>(ph[r][t]);
-                        pl[r][t] = transpose8(pack2<S::BF16>(w0 - back.x, w1 - back.y));
-                    }
-                    ph[r][t] = transpose8(ph[r][t]);
-                }
-            // o += values . weights; a lane's piece of the value rows is row g (and g + 8: the next element) of E / 2 tiles
-#pragma unroll
-            for (int j = 0; j < S::VCH; ++j) {
-                uint32_t v[4][S::VB / 4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (S::VB == 16) {
-                        const uint4 x = lds16(at + S::KBYTES + (t * S::VCH + j) * 512);
-                        v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
-                    } else {
-                        const uint2 x = lds8(at - lane * 8 + S::KBYTES + (t * S::VCH + j) * 256);
-                        v[t][0] = x.x; v[t][1] = x.y;
-                    }
-                }
-#pragma unroll
-                for (int w = 0; w < S::VB / 4; ++w) {
-                    if (KT != kKvE4m3) {
-                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
-                        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
                         for (int r = 0; r < S::HT; ++r) {
-                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
-                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
+                            mma<S::BF16>(s[r], ka.x, kb.x, ka.y, kb.y, q[r][j][0], q[r][j][1]);
+                            mma<S::BF16>(s2[r], ka.z, kb.z, ka.w, kb.w, q[r][j][2], q[r][j][3]);
                         }
                     } else {
+                        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t sel = x ? 0x7362 : 0x5140;
-                            const uint32_t u = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
-                            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(u)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(u >> 16));
-                            const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w])), a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w] >> 16));
+                            const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w])), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w] >> 16));
 #pragma unroll
-                            for (int r = 0; r < S::HT; ++r) mma<false>(o[j * S::E / 2 + 2 * w + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                            for (int r = 0; r < S::HT; ++r) mma<false>((w & 1) ? s2[r] : s[r], a0, a1, a2, a3, q[r][j][(2 * w) % QW], q[r][j][(2 * w + 1) % QW]);
+                        }
+                    }
+                }
+                float lv[2] = {0.f, 0.f};                              // log2 of the two keys' value scales
+                if (KT == kKvE4m3) {
+                    const uint32_t sa = at + 2 * S::KBYTES + k0 * 4;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const float ks = lds4(sa + t * 32);
+#pragma unroll
+                        for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
+                        lv[t] = __log2f(fmaxf(lds4(sa + 64 + t * 32), 0x1p-100f));
+                    }
+                }
+                const bool full = t0 >= lo && t0 + kStep <= n;
+                bool above = false;
+#pragma unroll
+                for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
+                        if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
+                        if (!full) {
+                            const int key = t0 + k0 + 4 * (k & 2);
+                            if (key < lo || key >= n) { x = -INFINITY; if (KT == kKvE4m3) lv[k >> 1] = 0.f; }
+                        }
+                        s[r][k] = x;
+                        above |= x + lv[k >> 1] > top[r][k & 1] + kSlack;
+                    }
+                if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                    for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float mx = fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]);
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                            mx = fmaxf(mx, top[r][h]);
+                            const float f = mx == -INFINITY ? 1.f : ex2(top[r][h] - mx);
+                            top[r][h] = mx;
+                            l[r][h] *= f;
+#pragma unroll
+                            for (int m = 0; m < S::MT; ++m) { o[m][r][h] *= f; o[m][r][2 + h] *= f; }
+                        }
+                }
+                // weights, transposed to the right operand of the second product: rows of eight keys
+                uint32_t ph[S::HT][2], pl[S::HT][2];
+#pragma unroll
+                for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const float m0 = top[r][0] == -INFINITY ? 0.f : top[r][0], m1 = top[r][1] == -INFINITY ? 0.f : top[r][1];
+                        const float x0 = s[r][2 * t] - m0, x1 = s[r][2 * t + 1] - m1;
+                        const float e0 = ex2(x0), e1 = ex2(x1);
+                        l[r][0] += e0;
+                        l[r][1] += e1;
+                        float w0 = e0, w1 = e1;
+                        if (KT == kKvE4m3) {
+                            w0 = ex2(x0 + (lv[t] + kShift));
+                            w1 = ex2(x1 + (lv[t] + kShift));
+                        } else if (kShift != 0.f) {
+                            w0 *= 128.f;
+                            w1 *= 128.f;
+                        }
+                        ph[r][t] = pack2<S::BF16>(w0, w1);
+                        if (KT != kKvE4m3) {
+                            const float2 back = unpack2<S::BF16>(ph[r][t]);
+                            pl[r][t] = transpose8(pack2<S::BF16>(w0 - back.x, w1 - back.y));
+                        }
+                        ph[r][t] = transpose8(ph[r][t]);
+                    }
+                // o += values . weights; a lane's piece of the value rows is row g (and g + 8: the next element) of E / 2 tiles
+#pragma unroll
+                for (int j = 0; j < S::VCH; ++j) {
+                    uint32_t v[4][S::VB / 4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t vp = at + v_off[t & 1] + (t >> 1) * 8 * S::PITCH + j * S::BOXBYTES;
+                        if (S::VB == 16) {
+                            const uint4 x = lds16(vp);
+                            v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
+                        } else {
+                            const uint2 x = lds8(vp);
+                            v[t][0] = x.x; v[t][1] = x.y;
+                        }
+                        if (!full) {                                   // what lies behind the row's end or before its window may be anything
+                            const int key = t0 + (t & 1 ? v1 : v0) + (t >> 1) * 8;
+                            if (key < lo || key >= n) {
+#pragma unroll
+                                for (int w = 0; w < S::VB / 4; ++w) v[t][w] = 0;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < S::VB / 4; ++w) {
+                        if (KT != kKvE4m3) {
+                            const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+                            const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+#pragma unroll
+                            for (int r = 0; r < S::HT; ++r) {
+                                mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                                mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t sel = x ? 0x7362 : 0x5140;
+                                const uint32_t u = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
+                                const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(u)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(u >> 16));
+                                const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
+#pragma unroll
+                                for (int r = 0; r < S::HT; ++r) mma<false>(o[j * S::E / 2 + 2 * w + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                            }
                         }
                     }
                 }
             }
+            __syncwarp();                                          // every lane has read the slot
+            if (next_i < steps) issue(rg.slot);
+            if (++rg.slot == S::STAGES) { rg.slot = 0; rg.parity ^= 1; }
         }
-        cp_wait<0>();
 
         // the four warps meet
 #pragma unroll
@@ -457,7 +466,7 @@ struct Piece {
                 if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(top[r][h], l[r][h]);
             }
         __syncthreads();
-        float* mine = reinterpret_cast<float*>(smem + warp * S::RING);
+        float* mine = rg.meet + warp * (ROWS * D);
 #pragma unroll
         for (int r = 0; r < S::HT; ++r)
 #pragma unroll
@@ -485,7 +494,7 @@ struct Piece {
             for (int w = 0; w < kWarps; ++w) {
                 const float2 v = sh_ml[w][row];
                 if (v.x != -INFINITY) ll += v.y * ex2(v.x - mm);
-                acc += reinterpret_cast<const float*>(smem + w * S::RING)[x];
+                acc += rg.meet[w * (ROWS * D) + x];
             }
             if (slot >= 0) {
                 cut.part_o[(static_cast<int64_t>(slot) * ROWS + row) * D + d] = acc;
@@ -508,21 +517,27 @@ struct Piece {
 
 // One block for each row and head group.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(PagedAttention p, int groups) {
-    extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, int groups) {
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float2 sh_ml[kWarps][16];
+    __shared__ unsigned long long sh_bars[kWarps * 8];
+    __shared__ int sh_abort;
+    Ring rg = Piece<KT, QT, D, ROWS>::begin(&map, smem, sh_bars, &sh_abort);
     const int vhs = p.kv.heads * groups, b = blockIdx.x / vhs, vh = blockIdx.x - b * vhs;
     const int n = row_keys(p, b);
     const int tb = first_key(p, n) / kTile;
-    Piece<KT, QT, D, ROWS>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, smem, sh_ml);
+    Piece<KT, QT, D, ROWS>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, rg, sh_ml);
+    Piece<KT, QT, D, ROWS>::end(p, &sh_abort);
 }
 
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  A block's first and
 // last piece may be part of a row; each goes to a slot of its own.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) paged_attention_shared_kernel(PagedAttention p, Cut cut, int groups) {
-    extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) paged_attention_shared_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, Cut cut, int groups) {
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float2 sh_ml[kWarps][16];
+    __shared__ unsigned long long sh_bars[kWarps * 8];
+    __shared__ int sh_abort;
     __shared__ long long sh_sum[kWarps];
     __shared__ int sh_b;
     __shared__ long long sh_rest;
@@ -566,7 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) pag
             u += k;
         }
     }
-    __syncthreads();
+    Ring rg = Piece<KT, QT, D, ROWS>::begin(&map, smem, sh_bars, &sh_abort);   // (a barrier of the block)
     int b = sh_b;
     long long rest = sh_rest, left = end - begin;                   // units into the row, units still to do
     bool first = true;
@@ -576,11 +591,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) pag
         const int vh = static_cast<int>(rest / tiles), t = static_cast<int>(rest - static_cast<long long>(vh) * tiles);
         const int k = static_cast<int>(min(static_cast<long long>(tiles - t), left));
         const int tb = first_key(p, n) / kTile + t;
-        Piece<KT, QT, D, ROWS>::run(p, cut, b, vh, n, tb, tb + k, groups, k == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), smem, sh_ml);
+        Piece<KT, QT, D, ROWS>::run(p, cut, b, vh, n, tb, tb + k, groups, k == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), rg, sh_ml);
         first = false;
         rest += k;
         left -= k;
     }
+    Piece<KT, QT, D, ROWS>::end(p, &sh_abort);
 }
 
 // Joins the pieces of one row and query head, and writes the outputs of empty rows.  The pieces of a row come in the order of their blocks, so
@@ -628,14 +644,39 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttentio
     }
 }
 
+// The pages as a tensor of five dimensions (element, place, head, key / value, page), copied in boxes of 16 places.  Strides may come in any order.
+const char* page_map(CUtensorMap* map, const KvPages& kv, int box_elements, int pitch) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return static_cast<Encode>(nullptr);
+        return reinterpret_cast<Encode>(ptr);
+    }();
+    if (!encode) return "paged_attention: cuTensorMapEncodeTiled is not available";
+    const uint64_t es = kv.type == kKvE4m3 ? 1 : 2;
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(kv.dim), static_cast<cuuint64_t>(kv.page_size), static_cast<cuuint64_t>(kv.heads), 2, static_cast<cuuint64_t>(kv.num_pages)};
+    // a dimension of one entry may have any stride; the map wants a multiple of 16 bytes
+    const int64_t given[4] = {kv.tok_stride, kv.head_stride, kv.kv_stride, kv.page_stride};
+    cuuint64_t strides[4];
+    for (int i = 0; i < 4; ++i) strides[i] = dims[i + 1] == 1 ? kv.dim * es : given[i] * es;
+    const cuuint32_t box[5] = {static_cast<cuuint32_t>(box_elements), kStep, 1, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, kv.data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              pitch == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? nullptr : "paged_attention: the cache's strides do not make a tensor map";
+}
+
 template <int KT, typename QT, int D, int ROWS>
 const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
     using S = Shape<KT, D, ROWS>;
     static std::atomic<uint64_t> raised_whole{0}, raised_shared{0};
+    CUtensorMap map;
+    if (const char* e = page_map(&map, p.kv, S::BOXEL, S::PITCH)) return e;
     if (plan.whole) {
         auto k = paged_attention_whole_kernel<KT, QT, D, ROWS>;
         if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
-        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, S::SMEM, s>>>(p, plan.head_groups);
+        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, S::SMEM, s>>>(map, p, plan.head_groups);
     } else {
         auto k = paged_attention_shared_kernel<KT, QT, D, ROWS>;
         if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_shared)) return "paged_attention: the shared-memory limit could not be raised";
@@ -645,7 +686,7 @@ const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, floa
         cut.prefix = reinterpret_cast<long long*>(ws);
         cut.part_ml = reinterpret_cast<float2*>(ws + 2 * (static_cast<int64_t>(p.B) + 2));
         cut.part_o = reinterpret_cast<float*>(cut.part_ml + 2 * static_cast<int64_t>(plan.blocks) * ROWS);
-        k<<<plan.blocks, kWarps * 32, S::SMEM, s>>>(p, cut, plan.head_groups);
+        k<<<plan.blocks, kWarps * 32, S::SMEM, s>>>(map, p, cut, plan.head_groups);
         if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
         paged_attention_join_kernel<KT, QT, D, ROWS><<<dim3(p.Hq, p.B), 128, 0, s>>>(p, cut, plan.head_groups);
     }
