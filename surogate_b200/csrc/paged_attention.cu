@@ -25,6 +25,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "launch_limits.h"
 #include "paged_kv.h"
@@ -35,7 +36,7 @@ namespace sg {
 namespace {
 
 constexpr int kTile = 64, kWarps = 4, kStep = 16;   // keys a tile, warps a block, keys a warp and tile
-constexpr int RING_BYTES = 16384;
+constexpr int RING_BYTES = 16384;   // of a warp, where two steps fit
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
@@ -108,16 +109,17 @@ template <int KT, int D, int ROWS> struct Shape {
     static constexpr int STAGES = RING_BYTES / STAGE > 8 ? 8 : RING_BYTES / STAGE < 2 ? 2 : RING_BYTES / STAGE;
     static constexpr int RING = STAGE * STAGES;                    // of one warp
     static constexpr int MT = D / 16;                              // tiles of 16 outputs
-    static constexpr int MEET = kWarps * ROWS * D * 4;             // where the warps' outputs meet
-    static constexpr int SMEM = 1024 + kWarps * RING + MEET;
+    static constexpr int SMEM = 1024 + kWarps * RING;
+    static_assert(RING >= ROWS * D * 4, "a warp's ring holds its outputs when the warps meet");
     static constexpr int FIT = 230000 / (SMEM + 2048);             // blocks that an SM's shared memory holds
-    static constexpr int PER_SM = FIT > 3 ? 3 : FIT;
+    static constexpr int MOST = ROWS == 8 && D <= 128 ? 3 : 2;     // of 168 registers a thread, or 255
+    static constexpr int PER_SM = FIT < MOST ? FIT : MOST;
 };
 
 struct Ring {            // a warp's copies under way
     const CUtensorMap* map;
     uint32_t base, bars;  // shared memory: all warps' rings, one barrier for each slot
-    float* meet;
+    float* meet;          // the same memory, when the copies are done and the warps' outputs meet
     volatile int* abort_flag;
     int slot;             // the next step's
     uint32_t parity;
@@ -165,7 +167,7 @@ struct Piece {
         if (threadIdx.x < kWarps * S::STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
         fence_barrier_init();
         __syncthreads();
-        return Ring{map, smem_u32(at), smem_u32(bars), reinterpret_cast<float*>(at + kWarps * S::RING), abort_flag, 0, 0};
+        return Ring{map, smem_u32(at), smem_u32(bars), reinterpret_cast<float*>(at), abort_flag, 0, 0};
     }
     static __device__ void end(const PagedAttention& p, const int* abort_flag) {
         if (threadIdx.x == 0 && *abort_flag) atomicExch(p.error_flag, 1);
@@ -291,7 +293,8 @@ struct Piece {
         // o[m][r]: outputs of two elements of the head and of heads 8 r + 2c, + 1: [0], [1] the first element's, [2], [3] the second's
         float o[S::MT][S::HT][4];
         // Weights are relative to 2^top, which follows the scores' maximum only when they exceed it by kSlack: most steps need no maximum over lanes.
-        float top[S::HT][2], l[S::HT][2];
+        // (top: 0 until then; limit: what a score, or score plus log2 of a value's scale, may be without that.)
+        float top[S::HT][2], limit[S::HT][2], l[S::HT][2];
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
 #pragma unroll
@@ -301,155 +304,174 @@ struct Piece {
 #pragma unroll
         for (int r = 0; r < S::HT; ++r)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) { top[r][k] = -INFINITY; l[r][k] = 0.f; }
+            for (int k = 0; k < 2; ++k) { top[r][k] = 0.f; limit[r][k] = -INFINITY; l[r][k] = 0.f; }
+
+        // One step: 16 keys in the slot at `at`.  Only the first and last of a row hold keys that do not count (FULL: none does).
+        auto compute = [&](auto full_tag, uint32_t at, int t0) {
+            constexpr bool FULL = decltype(full_tag)::value;
+            // scores of 16 keys: s[r][0], [1] are key k0 with heads 8 r + 2c, + 1, s[r][2], [3] key k0 + 8
+            float s[S::HT][4], s2[S::HT][4];                       // two sums, so that products do not wait for one another
+#pragma unroll
+            for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[r][k] = s2[r][k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < S::KCH; ++j) {
+                const uint32_t kp = at + k_off[j & 1] + (j >> 1) * S::BOXBYTES;
+                const uint4 ka = lds16(kp), kb = lds16(kp + 8 * S::PITCH);
+                if (KT != kKvE4m3) {
+#pragma unroll
+                    for (int r = 0; r < S::HT; ++r) {
+                        mma<S::BF16>(s[r], ka.x, kb.x, ka.y, kb.y, q[r][j][0], q[r][j][1]);
+                        mma<S::BF16>(s2[r], ka.z, kb.z, ka.w, kb.w, q[r][j][2], q[r][j][3]);
+                    }
+                } else {
+                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w])), a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w] >> 16));
+                        const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w])), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w] >> 16));
+#pragma unroll
+                        for (int r = 0; r < S::HT; ++r) mma<false>((w & 1) ? s2[r] : s[r], a0, a1, a2, a3, q[r][j][(2 * w) % QW], q[r][j][(2 * w + 1) % QW]);
+                    }
+                }
+            }
+            float lv[2] = {0.f, 0.f}, vs[2];                       // e4m3: the two keys' value scales, and log2 of them
+            if (KT == kKvE4m3) {
+                const uint32_t sa = at + 2 * S::KBYTES + k0 * 4;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float ks = lds4(sa + t * 32);
+#pragma unroll
+                    for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
+                    vs[t] = fmaxf(lds4(sa + 64 + t * 32), 0x1p-100f);
+                    lv[t] = __log2f(vs[t]);
+                }
+            }
+            if (!FULL && KT == kKvE4m3) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (t0 + k0 + 8 * t < lo || t0 + k0 + 8 * t >= n) { lv[t] = 0.f; vs[t] = 1.f; }   // not there: its scale may be anything
+            }
+            bool above = false;
+            float most[S::HT][2];
+#pragma unroll
+            for (int r = 0; r < S::HT; ++r) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
+                    if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
+                    if (!FULL) {
+                        const int key = t0 + k0 + 4 * (k & 2);
+                        if (key < lo || key >= n) x = -INFINITY;
+                    }
+                    s[r][k] = x;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    most[r][h] = KT == kKvE4m3 ? fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]) : fmaxf(s[r][h], s[r][2 + h]);
+                    above |= most[r][h] > limit[r][h];
+                }
+            }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float mx = most[r][h];
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        if (mx > (limit[r][h] == -INFINITY ? -INFINITY : top[r][h])) {
+                            const float f = limit[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mx);
+                            top[r][h] = mx;
+                            limit[r][h] = mx + kSlack;
+                            l[r][h] *= f;
+#pragma unroll
+                            for (int m = 0; m < S::MT; ++m) { o[m][r][h] *= f; o[m][r][2 + h] *= f; }
+                        }
+                    }
+            }
+            // weights, transposed to the right operand of the second product: rows of eight keys
+            uint32_t ph[S::HT][2], pl[S::HT][2];
+#pragma unroll
+            for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float e0 = ex2(s[r][2 * t] - top[r][0]), e1 = ex2(s[r][2 * t + 1] - top[r][1]);
+                    l[r][0] += e0;
+                    l[r][1] += e1;
+                    float w0 = e0, w1 = e1;
+                    if (KT == kKvE4m3) {
+                        const float f = vs[t] * 128.f;
+                        w0 *= f;
+                        w1 *= f;
+                    } else if (kShift != 0.f) {
+                        w0 *= 128.f;
+                        w1 *= 128.f;
+                    }
+                    ph[r][t] = pack2<S::BF16>(w0, w1);
+                    if (KT != kKvE4m3) {
+                        const float2 back = unpack2<S::BF16>(ph[r][t]);
+                        pl[r][t] = transpose8(pack2<S::BF16>(w0 - back.x, w1 - back.y));
+                    }
+                    ph[r][t] = transpose8(ph[r][t]);
+                }
+            // o += values . weights; a lane's piece of the value rows is row g (and g + 8: the next element) of E / 2 tiles
+#pragma unroll
+            for (int j = 0; j < S::VCH; ++j) {
+                uint32_t v[4][S::VB / 4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t vp = at + v_off[t & 1] + (t >> 1) * 8 * S::PITCH + j * S::BOXBYTES;
+                    if (S::VB == 16) {
+                        const uint4 x = lds16(vp);
+                        v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
+                    } else {
+                        const uint2 x = lds8(vp);
+                        v[t][0] = x.x; v[t][1] = x.y;
+                    }
+                    if (!FULL) {                                   // what lies behind the row's end or before its window may be anything
+                        const int key = t0 + (t & 1 ? v1 : v0) + (t >> 1) * 8;
+                        if (key < lo || key >= n) {
+#pragma unroll
+                            for (int w = 0; w < S::VB / 4; ++w) v[t][w] = 0;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < S::VB / 4; ++w) {
+                    if (KT != kKvE4m3) {
+                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+                        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+#pragma unroll
+                        for (int r = 0; r < S::HT; ++r) {
+                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                            mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t sel = x ? 0x7362 : 0x5140;
+                            const uint32_t u = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
+                            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(u)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(u >> 16));
+                            const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
+#pragma unroll
+                            for (int r = 0; r < S::HT; ++r) mma<false>(o[j * S::E / 2 + 2 * w + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+                        }
+                    }
+                }
+            }
+        };
 
         int t0 = tb * kTile + warp * kStep;
         for (int i = 0; i < steps; ++i, t0 += kTile) {
             if (!mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag)) break;
             const uint32_t at = ring + rg.slot * S::STAGE;
             if ((have >> (i & 31)) & 1) {
-                // scores of 16 keys: s[r][0], [1] are key k0 with heads 8 r + 2c, + 1, s[r][2], [3] key k0 + 8
-                float s[S::HT][4], s2[S::HT][4];                       // two sums, so that products do not wait for one another
-#pragma unroll
-                for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) s[r][k] = s2[r][k] = 0.f;
-#pragma unroll
-                for (int j = 0; j < S::KCH; ++j) {
-                    const uint32_t kp = at + k_off[j & 1] + (j >> 1) * S::BOXBYTES;
-                    const uint4 ka = lds16(kp), kb = lds16(kp + 8 * S::PITCH);
-                    if (KT != kKvE4m3) {
-#pragma unroll
-                        for (int r = 0; r < S::HT; ++r) {
-                            mma<S::BF16>(s[r], ka.x, kb.x, ka.y, kb.y, q[r][j][0], q[r][j][1]);
-                            mma<S::BF16>(s2[r], ka.z, kb.z, ka.w, kb.w, q[r][j][2], q[r][j][3]);
-                        }
-                    } else {
-                        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w])), a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(wa[w] >> 16));
-                            const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w])), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[w] >> 16));
-#pragma unroll
-                            for (int r = 0; r < S::HT; ++r) mma<false>((w & 1) ? s2[r] : s[r], a0, a1, a2, a3, q[r][j][(2 * w) % QW], q[r][j][(2 * w + 1) % QW]);
-                        }
-                    }
-                }
-                float lv[2] = {0.f, 0.f};                              // log2 of the two keys' value scales
-                if (KT == kKvE4m3) {
-                    const uint32_t sa = at + 2 * S::KBYTES + k0 * 4;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const float ks = lds4(sa + t * 32);
-#pragma unroll
-                        for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
-                        lv[t] = __log2f(fmaxf(lds4(sa + 64 + t * 32), 0x1p-100f));
-                    }
-                }
-                const bool full = t0 >= lo && t0 + kStep <= n;
-                bool above = false;
-#pragma unroll
-                for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
-                        if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
-                        if (!full) {
-                            const int key = t0 + k0 + 4 * (k & 2);
-                            if (key < lo || key >= n) { x = -INFINITY; if (KT == kKvE4m3) lv[k >> 1] = 0.f; }
-                        }
-                        s[r][k] = x;
-                        above |= x + lv[k >> 1] > top[r][k & 1] + kSlack;
-                    }
-                if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-                    for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float mx = fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]);
-#pragma unroll
-                            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                            mx = fmaxf(mx, top[r][h]);
-                            const float f = mx == -INFINITY ? 1.f : ex2(top[r][h] - mx);
-                            top[r][h] = mx;
-                            l[r][h] *= f;
-#pragma unroll
-                            for (int m = 0; m < S::MT; ++m) { o[m][r][h] *= f; o[m][r][2 + h] *= f; }
-                        }
-                }
-                // weights, transposed to the right operand of the second product: rows of eight keys
-                uint32_t ph[S::HT][2], pl[S::HT][2];
-#pragma unroll
-                for (int r = 0; r < S::HT; ++r)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const float m0 = top[r][0] == -INFINITY ? 0.f : top[r][0], m1 = top[r][1] == -INFINITY ? 0.f : top[r][1];
-                        const float x0 = s[r][2 * t] - m0, x1 = s[r][2 * t + 1] - m1;
-                        const float e0 = ex2(x0), e1 = ex2(x1);
-                        l[r][0] += e0;
-                        l[r][1] += e1;
-                        float w0 = e0, w1 = e1;
-                        if (KT == kKvE4m3) {
-                            w0 = ex2(x0 + (lv[t] + kShift));
-                            w1 = ex2(x1 + (lv[t] + kShift));
-                        } else if (kShift != 0.f) {
-                            w0 *= 128.f;
-                            w1 *= 128.f;
-                        }
-                        ph[r][t] = pack2<S::BF16>(w0, w1);
-                        if (KT != kKvE4m3) {
-                            const float2 back = unpack2<S::BF16>(ph[r][t]);
-                            pl[r][t] = transpose8(pack2<S::BF16>(w0 - back.x, w1 - back.y));
-                        }
-                        ph[r][t] = transpose8(ph[r][t]);
-                    }
-                // o += values . weights; a lane's piece of the value rows is row g (and g + 8: the next element) of E / 2 tiles
-#pragma unroll
-                for (int j = 0; j < S::VCH; ++j) {
-                    uint32_t v[4][S::VB / 4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t vp = at + v_off[t & 1] + (t >> 1) * 8 * S::PITCH + j * S::BOXBYTES;
-                        if (S::VB == 16) {
-                            const uint4 x = lds16(vp);
-                            v[t][0] = x.x; v[t][1] = x.y; v[t][2 % (S::VB / 4)] = x.z; v[t][3 % (S::VB / 4)] = x.w;
-                        } else {
-                            const uint2 x = lds8(vp);
-                            v[t][0] = x.x; v[t][1] = x.y;
-                        }
-                        if (!full) {                                   // what lies behind the row's end or before its window may be anything
-                            const int key = t0 + (t & 1 ? v1 : v0) + (t >> 1) * 8;
-                            if (key < lo || key >= n) {
-#pragma unroll
-                                for (int w = 0; w < S::VB / 4; ++w) v[t][w] = 0;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int w = 0; w < S::VB / 4; ++w) {
-                        if (KT != kKvE4m3) {
-                            const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
-                            const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
-#pragma unroll
-                            for (int r = 0; r < S::HT; ++r) {
-                                mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
-                                mma<S::BF16>(o[j * S::E / 2 + w][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t sel = x ? 0x7362 : 0x5140;
-                                const uint32_t u = __byte_perm(v[0][w], v[1][w], sel), y = __byte_perm(v[2][w], v[3][w], sel);
-                                const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(u)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(u >> 16));
-                                const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
-#pragma unroll
-                                for (int r = 0; r < S::HT; ++r) mma<false>(o[j * S::E / 2 + 2 * w + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
-                            }
-                        }
-                    }
-                }
+                if (t0 >= lo && t0 + kStep <= n) compute(std::true_type{}, at, t0);
+                else compute(std::false_type{}, at, t0);
             }
             __syncwarp();                                          // every lane has read the slot
             if (next_i < steps) issue(rg.slot);
@@ -463,7 +485,7 @@ struct Piece {
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[r][h] += __shfl_xor_sync(0xffffffffu, l[r][h], x);
-                if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(top[r][h], l[r][h]);
+                if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(limit[r][h] == -INFINITY ? -INFINITY : top[r][h], l[r][h]);
             }
         __syncthreads();
         float* mine = rg.meet + warp * (ROWS * D);
@@ -475,7 +497,7 @@ struct Piece {
                 float mm = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][head].x);
-                const float f = top[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
+                const float f = limit[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
 #pragma unroll
                 for (int j = 0; j < S::VCH; ++j)
 #pragma unroll
@@ -503,6 +525,7 @@ struct Piece {
                 finish(p, b, h0 + row, d, mm, ll, acc);
             }
         }
+        fence_proxy_async();                                       // the rings are written by copies again
         __syncthreads();
     }
 
