@@ -5,12 +5,16 @@
 //   the kept mass exceeds u times the whole.  T = 0: the largest logit's lowest index.  logprob = l_token - log sum e^l, without filters.
 //
 // A row is read from HBM once, and that (size of a logit * vocabulary) is its floor.  A cluster of 1 to 8 blocks holds the row in its shared
-// memory; the passes over it (maximum; weights; the cuts; the draw) stay on the chip, the blocks exchange a few words after each.
+// memory; the passes over it (maximum; sums; the candidates) stay on the chip, and the blocks exchange a few words after each.
 //
 // * The result is a token, not a number that may be a little off, so masses are integers: weights as multiples of 2^-44 of the largest one
-//   (exponentials in fp64, relative error below 2^-44; smaller weights than 2^-45 count as nothing), whose sums do not depend on the order.
-// * Cuts need no sort: tokens are counted (and their mass summed) in 1024 bins over the logits, the bin in which the cut falls is found by a
-//   scan, and only its tokens are ranked against one another; a bin with too many is divided again, equal logits are counted by index.
+//   (exponentials in fp64 by a table of 2^(j/1024) and two terms of the series: relative error 2^-37), whose sums do not depend on the order.
+//   A wrong token takes a u within that of a boundary.
+// * Cuts need no sort.  Bounds leave a few candidates: the k largest logits are not below the k-th of the threads' own maxima; tokens lighter
+//   than (1 - top_p) / vocabulary of the whole mass make up less than 1 - top_p together, so the cut of top-p lies above them.  Up to 512
+//   candidates are ranked against one another by one block.  More (flat rows, large k) are counted, with their mass, in 1024 bins over the
+//   logits; the bin in which the cut falls is found by a scan and only its tokens are ranked; a bin with too many is divided again, equal
+//   logits are counted by index.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,13 +34,12 @@ namespace {
 
 using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = 512, kMaxCluster = 8;
+constexpr int kOwn = 64;                      // candidates a warp can note down
 constexpr int kFrac = 44;                     // weights are multiples of 2^-44
-constexpr float kRange = 46.f;                // log2 of the smallest weight that is looked at: what lies below is 0 as a multiple
-constexpr double kLog2eD = 1.4426950408889634074;
-
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+constexpr float kRange = 46.f;                // minus log2 of the smallest weight that is looked at: what lies below is 0 as a multiple
+constexpr int kTable = 1024;
+constexpr int kMost = 190 * 1024;             // bytes of a row that a block holds at most, beside 29 KB of its own
+constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 
 // fp32 as an unsigned number of the same order (-0 as +0); 0 is below all that occur
 __device__ __forceinline__ uint32_t order_key(float l) {
@@ -62,72 +65,142 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {   // inclusive
 }
 
 struct Shared {
-    double table[64];                 // 2^(j / 64)
-    u64 mass[kBins];
-    u64 list[kList], all[kList], all_q[kList];
-    uint32_t count[kBins];
+    double table[kTable];             // 2^(j / 1024)
+    float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
+    int own_i[kWarps * kOwn];
+    union {
+        struct { u64 mass[kBins]; uint32_t count[kBins]; };
+        struct { u64 all[kList], all_q[kList]; };
+    };
     u64 warp_q[kWarps];
     float warp_z[kWarps];
+    int warp_n[kWarps];               // candidates of each warp
     // what other blocks of the cluster read
-    u64 x_best, x_sum, x_cut;
+    u64 x_sum, x_cut;
     float x_z;
-    uint32_t x_min, x_max, x_listed;
+    int x_first;                      // index of place 0
+    uint32_t x_best, x_index, x_min, x_max, x_listed, x_noted;
     // results of one thread for its block
-    u64 b_before, b_total;
+    u64 b_before;
     uint32_t b_bin, b_count;
 };
 
+// 16 bytes of logits as fp32
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(const uint4& v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+    }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+};
+template <> struct Vec<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i])); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One block's part of a row.  Places count its logits from the 16-byte boundary at or before its first one; places that hold none read as -inf.
 template <typename T, bool RESIDENT>
 struct Row {
+    static constexpr int N = Vec<T>::N;
     cg::cluster_group cluster = cg::this_cluster();
     Shared& sh;
-    const T* x;                       // this block's part of the row: shared memory, or where it lies
-    int n, first, seg;                // its size, the index of its first token, tokens a warp
+    const uint4* x;                   // the boundary: in shared memory, or where the row lies
+    int off, end, nvec, seg;          // places [off, end) hold logits; vectors; vectors a warp
+    int first;                        // index of place 0
     int blocks, rank, warp, lane;
     float lmax;
     double to_log2;                   // log2(e) / T
-    double least;                     // log2 of the smallest eligible weight
-    float bin_scale, least_lo, least_hi;
+    bool steep;                       // what is not below floor_l may still be lighter than 2^-1000: a very low temperature, or infinite logits
+    double least;                     // log2 of the smallest weight that min-p lets stay
+    bool by_min_p;
+    float bin_scale;
+    float floor_l;                    // what is not below this is looked at
+    bool listed = false;              // the candidates have been noted down: passes run over them
     u64 cut = 0;                      // kept: pack() >= cut
 
     __device__ Row(Shared& s) : sh(s) {}
 
-    __device__ __forceinline__ float at(int i) const { return to_f(x[i]); }
-    __device__ __forceinline__ double log2_weight(float l) const {
-        return l == lmax ? 0. : (static_cast<double>(l) - static_cast<double>(lmax)) * to_log2;
+    // the vector `v` in global memory: whole where all of it belongs to the row's part
+    __device__ __forceinline__ uint4 from_global(const uint4* base, int v) const {
+        if (v * N >= off && v * N + N <= end) return __ldg(base + v);
+        alignas(16) T e[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = v * N + j;
+            e[j] = i >= off && i < end ? reinterpret_cast<const T*>(base)[i] : static_cast<T>(-INFINITY);
+        }
+        return *reinterpret_cast<const uint4*>(e);
     }
+    __device__ __forceinline__ uint4 vec(int v) const { return RESIDENT ? x[v] : from_global(x, v); }
+
+    __device__ __forceinline__ double log2_weight(float l) const { return l == lmax ? 0. : (static_cast<double>(l) - static_cast<double>(lmax)) * to_log2; }
     // Coarse log2 of a weight in fp32: never increases as l falls
     __device__ __forceinline__ float coarse(float l) const { return l == lmax ? 0.f : (l - lmax) * bin_scale; }
-    __device__ __forceinline__ bool eligible(float l) const {
-        const float t = coarse(l);
-        if (t > least_hi) return true;
-        if (!(t >= least_lo)) return false;                       // NaN and -inf as well
-        return log2_weight(l) >= least;
+    __device__ __forceinline__ int bin_of(float l) const { return max(0, min(kBins - 1, static_cast<int>(-coarse(l) * (kBins / kRange)))); }
+    __device__ __forceinline__ bool eligible(float l) const { return !by_min_p || log2_weight(l) >= least; }
+    // A logit that surely is not above one with this log2 of its weight
+    __device__ __forceinline__ float logit_below(double log2_w) const {
+        const double l = static_cast<double>(lmax) + log2_w * 1.000001 / to_log2;
+        return fmaxf(__double2float_rd(l - fabs(l) * 1e-6), -3.402823466e38f);        // (-inf never counts; NaN, from infinities: the lowest number)
     }
-    // 2^t as a multiple of 2^-44, t <= 0: t = i / 64 + r, 2^r by its series to the fourth power (|r| <= 2^-7: 4e-14)
+    // 2^log2_weight as a multiple of 2^-44, for l >= floor_l: t = i / 1024 + r, 2^r = 1 + r (ln 2 + r ln2^2 / 2).  Adding 256 to it as an fp64
+    // leaves the multiple in the lowest bits.
     __device__ __forceinline__ u64 weight(float l) const {
-        const double t = log2_weight(l);
-        if (!(t >= -45.)) return 0;
-        const double big = 6755399441055744. / 64.;               // 1.5 * 2^52 / 64: adding it rounds to multiples of 1 / 64
-        const double m = t + big;
-        const int i = static_cast<int>(__double_as_longlong(m) & 0xffffffff);
-        const double r = t - (m - big);
-        double y = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);   // ln2^4 / 24, ln2^3 / 6, ln2^2 / 2, ln2
-        y = fma(r, y, 2.402265069591007e-1);
-        y = fma(r, y, 6.931471805599453e-1);
-        const double e = sh.table[i & 63];
-        const double v = fma(e * r, y, e);                        // 2^(t - floor(i / 64)), in [0.99, 2.01)
-        const long long bits = __double_as_longlong(v);
-        const int shift = 52 - kFrac - static_cast<int>((bits >> 52) - 1023) - (i >> 6);   // 1 .. 54
-        const u64 mant = (static_cast<u64>(bits) & 0xfffffffffffffull) | 0x10000000000000ull;
-        return (mant + (1ull << (shift - 1))) >> shift;
+        const double d = static_cast<double>(l) - static_cast<double>(lmax);
+        if (steep) {
+            if (l == lmax) return 1ull << kFrac;
+            if (!(d * to_log2 >= -60.)) return 0;
+        }
+        const double big = 6755399441055744. / kTable;            // 1.5 * 2^52 / 1024: adding it rounds to multiples of 1 / 1024
+        const double m = fma(d, to_log2, big);
+        const int i = __double2loint(m);
+        const double r = fma(d, to_log2, big - m);
+        const double e = sh.table[i & (kTable - 1)];
+        const double v = fma(e * r, fma(r, kLn2D * kLn2D / 2, kLn2D), e);
+        const double w = __hiloint2double(__double2hiint(v) + ((i >> 10) << 20), __double2loint(v));
+        return static_cast<u64>(__double_as_longlong(w + 256.)) - 0x4070000000000000ull;
     }
 
-    template <typename F> __device__ __forceinline__ void each(F f) const {                      // all tokens of the block
-        for (int i = threadIdx.x; i < n; i += kThreads) f(i, at(i));
+    // f(place, logit) for the tokens that are not below floor_l, each warp its own in the order of their indices, lanes apart
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        if (listed) {
+            for (int i = lane; i < sh.warp_n[warp]; i += 32) f(sh.own_i[warp * kOwn + i], sh.own_l[warp * kOwn + i]);
+            return;
+        }
+        const int b = min(nvec, (warp + 1) * seg);
+        for (int v = warp * seg + lane; v < b; v += 32) {
+            float l[N], most;
+            Vec<T>::get(vec(v), l);
+            most = l[0];
+#pragma unroll
+            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+            if (!(most >= floor_l)) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (l[j] >= floor_l) f(v * N + j, l[j]);
+        }
     }
+    __device__ __forceinline__ u64 order(int place, float l) const { return pack(l, first + place); }
 
-    // Sum over the block of one number a thread, and the sum before each warp's, in sh.warp_q; every thread gets the block's
+    // Sum over the block of one number a lane (a thread's share), the warps' own sums in sh.warp_q; every thread gets the block's
     __device__ u64 block_sums(u64 v) {
         v = warp_sum(v);
         __syncthreads();
@@ -138,9 +211,19 @@ struct Row {
         for (int w = 0; w < kWarps; ++w) total += sh.warp_q[w];
         return total;
     }
+    // The thread of the block in whose share the running sum first exceeds `target`: given the sum before its share by hit(before)
+    template <typename F> __device__ void block_find(u64 v, u64 target, F hit) {
+        const u64 upto = warp_scan(v, lane);
+        __syncthreads();
+        if (lane == 31) sh.warp_q[warp] = upto;
+        __syncthreads();
+        u64 before = upto - v;
+        for (int w = 0; w < warp; ++w) before += sh.warp_q[w];
+        if (before <= target && target < before + v) hit(before);
+    }
 
-    // The token (index in the row) at which the sum of q(i, l) over the tokens of the row, in the order of the indices, first exceeds what `aim` makes
-    // of the whole sum; `mine` is the warp's own sum.  Given to the one warp that holds it by `found(index, logit)`.
+    // The token at which the sum of q(place, logit) over the tokens of the row, in the order of the indices, first exceeds what `aim` makes of
+    // the whole sum; `mine` is this lane's part of its warp's sum.  One thread of the cluster gets it by found(place, logit).
     template <typename Q, typename A, typename F> __device__ void locate(Q q, u64 mine, A aim, F found) {
         const u64 own = block_sums(mine);
         if (threadIdx.x == 0) sh.x_sum = own;
@@ -151,36 +234,80 @@ struct Row {
             if (r < rank) before += v;
             total += v;
         }
-        const u64 target = aim(total);
-        for (int w = 0; w < warp; ++w) before += sh.warp_q[w];
-        if (before <= target && target < before + sh.warp_q[warp]) {       // one warp of the cluster
-            const int a = warp * seg, b = min(n, a + seg), sub = (b - a + 31) / 32;
-            const int la = min(b, a + lane * sub), lb = min(b, la + sub);
-            u64 s = 0;
-            for (int i = la; i < lb; ++i) s += q(i, at(i));
-            const u64 upto = before + warp_scan(s, lane);
-            const int who = __ffs(__ballot_sync(0xffffffffu, upto > target)) - 1;
-            before = __shfl_sync(0xffffffffu, upto - s, who);
-            const int wa = min(b, a + who * sub), wb = min(b, wa + sub);
-            for (int base = wa; base < wb; base += 32) {
-                const int i = base + lane;
-                const float l = i < wb ? at(i) : 0.f;
-                const u64 v = i < wb ? q(i, l) : 0;
-                const u64 through = before + warp_scan(v, lane);
-                const unsigned hit = __ballot_sync(0xffffffffu, through > target);
-                if (hit) {
-                    if (lane == __ffs(hit) - 1) found(i, l);
-                    break;
-                }
-                before = __shfl_sync(0xffffffffu, through, 31);
-            }
+        u64 target = aim(total);
+        if (target < before || target >= before + own) return;            // another block's
+        target -= before;
+        int w = 0;
+        while (target >= sh.warp_q[w]) target -= sh.warp_q[w++];            // the warp's tokens, over the whole block
+        if (listed) {
+            const int i = threadIdx.x, place = i < kOwn ? sh.own_i[w * kOwn + i] : 0;
+            const float l = i < kOwn ? sh.own_l[w * kOwn + i] : 0.f;
+            block_find(i < sh.warp_n[w] ? q(place, l) : 0, target, [&](u64) { found(place, l); });
+            return;
         }
-    }
-    template <typename Q> __device__ __forceinline__ u64 warp_part(Q q) const {   // sum of q over the warp's own tokens
+        const int a = w * seg, b = min(nvec, a + seg), per = (b - a + kThreads - 1) / kThreads, va = min(b, a + static_cast<int>(threadIdx.x) * per), vb = min(b, va + per);
+        auto share = [&](auto f) {
+            for (int v = va; v < vb; ++v) {
+                float l[N];
+                Vec<T>::get(vec(v), l);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (l[j] >= floor_l) f(v * N + j, l[j]);
+            }
+        };
         u64 s = 0;
-        const int a = warp * seg, b = min(n, a + seg);
-        for (int i = a + lane; i < b; i += 32) s += q(i, at(i));
-        return s;
+        share([&](int i, float l) { s += q(i, l); });
+        block_find(s, target, [&](u64 upto) {
+            bool done = false;
+            share([&](int i, float l) {
+                upto += q(i, l);
+                if (!done && upto > target) { done = true; found(i, l); }
+            });
+        });
+    }
+
+    // Notes down the candidates; true if all warps of the cluster have room for theirs.  `total`: all of them.
+    __device__ bool note_down(int& total) {
+        int n = 0;
+        const int b = min(nvec, (warp + 1) * seg);
+        for (int base = warp * seg; base < b; base += 32) {
+            float l[N];
+            int c = 0;
+            if (base + lane < b) {
+                Vec<T>::get(vec(base + lane), l);
+#pragma unroll
+                for (int j = 0; j < N; ++j) c += l[j] >= floor_l;
+            }
+            if (!__any_sync(0xffffffffu, c)) continue;
+            int upto = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            int at = n + upto - c;
+            if (c) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (l[j] >= floor_l) {
+                        if (at < kOwn) { sh.own_l[warp * kOwn + at] = l[j]; sh.own_i[warp * kOwn + at] = (base + lane) * N + j; }
+                        ++at;
+                    }
+            }
+            n += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) sh.warp_n[warp] = n;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t sum = 0;
+            for (int w = 0; w < kWarps; ++w) sum = sh.warp_n[w] > kOwn || sum >= 0x10000000u ? 0x10000000u : sum + sh.warp_n[w];
+            sh.x_noted = sum;
+        }
+        cluster.sync();
+        uint32_t sum = 0;
+        for (int r = 0; r < blocks; ++r) sum += *cluster.map_shared_rank(&sh.x_noted, r);
+        total = static_cast<int>(sum);
+        return sum < 0x10000000u;
     }
 
     __device__ void clear_bins() {
@@ -217,7 +344,7 @@ struct Row {
             if (w < warp) before += sh.warp_q[w];
             total += sh.warp_q[w];
         }
-        if (fraction >= 0.) target = max(1ull, min(total, static_cast<u64>(ceil(fraction * static_cast<double>(total)))));
+        if (fraction >= 0.) target = share_of(fraction, total);
         const bool inside = total >= target;
         if (inside) {
 #pragma unroll
@@ -230,33 +357,35 @@ struct Row {
         cluster.sync();                                            // nobody reads these bins any more
         return inside;
     }
+    // The least mass that a prefix must reach to be `fraction` of the whole
+    static __device__ __forceinline__ u64 share_of(double fraction, u64 total) {
+        return max(1ull, min(total, static_cast<u64>(ceil(fraction * static_cast<double>(total)))));
+    }
 
     // Ranks the tokens for which `in` holds (at most kList in the cluster) against one another; sets the cut.
     template <bool MASS, typename In> __device__ void cut_in_list(In in, u64 base, u64 target) {
+        u64* list = reinterpret_cast<u64*>(sh.all);                // (the bins are done with)
         if (threadIdx.x == 0) sh.x_listed = 0;
         __syncthreads();
         each([&](int i, float l) {
-            if (in(i, l)) sh.list[min(atomicAdd(&sh.x_listed, 1u), static_cast<uint32_t>(kList - 1))] = pack(l, first + i);
+            if (in(i, l)) list[min(atomicAdd(&sh.x_listed, 1u), static_cast<uint32_t>(kList - 1))] = order(i, l);
         });
         __syncthreads();
         cluster.sync();
-        int total = 0;
-        for (int r = 0; r < blocks; ++r) {
-            const int c = min(static_cast<int>(*cluster.map_shared_rank(&sh.x_listed, r)), kList - total);
-            const u64* from = cluster.map_shared_rank(sh.list, r);
-            for (int i = threadIdx.x; i < c; i += kThreads) {
-                const u64 v = from[i];
-                sh.all[total + i] = v;
-                sh.all_q[total + i] = MASS ? weight(key_value(static_cast<uint32_t>(v >> 32))) : 1;
-            }
-            total += c;
-        }
+        // every warp of the cluster takes tokens of its own block and meets all lists, which stay where they are
+        const int own = min(static_cast<int>(sh.x_listed), kList);
+        for (int i = threadIdx.x; i < own; i += kThreads) sh.all_q[i] = MASS ? weight(key_value(static_cast<uint32_t>(list[i] >> 32))) : 1;
         __syncthreads();
-        for (int i = rank * kWarps + warp; i < total; i += blocks * kWarps) {
-            const u64 me = sh.all[i];
+        cluster.sync();
+        for (int i = warp; i < own; i += kWarps) {
+            const u64 me = list[i];
             u64 s = 0;
-            for (int j = lane; j < total; j += 32)
-                if (sh.all[j] > me) s += sh.all_q[j];
+            for (int r = 0; r < blocks; ++r) {
+                const int c = min(static_cast<int>(*cluster.map_shared_rank(&sh.x_listed, r)), kList);
+                const u64 *from = cluster.map_shared_rank(list, r), *q = cluster.map_shared_rank(sh.all_q, r);
+                for (int j = lane; j < c; j += 32)
+                    if (from[j] > me) s += q[j];
+            }
             s = base + warp_sum(s);
             if (s < target && target <= s + sh.all_q[i] && lane < blocks) *cluster.map_shared_rank(&sh.x_cut, lane) = me;
         }
@@ -264,14 +393,20 @@ struct Row {
         cut = sh.x_cut;
     }
 
-    // Keeps the tokens, in the order of falling logit, before which less than `target` has come: tokens, or mass (a share of the whole).  The bins of
-    // the first division are in sh already.
+    // Keeps the tokens, in the order of falling logit, before which less than `target` has come: tokens, or mass (a share of the whole).
     template <bool MASS> __device__ void find_cut(double fraction, u64 target) {
+        const u64 old = cut;
+        auto stays = [&](int i, float l) { return order(i, l) >= old; };
+        clear_bins();
+        each([&](int i, float l) {
+            if (!eligible(l) || !stays(i, l)) return;
+            const int bin = bin_of(l);
+            atomicAdd(&sh.count[bin], 1u);
+            if (MASS) atomicAdd(&sh.mass[bin], weight(l));
+        });
         if (!find_bin<MASS>(fraction, 0, target)) return;          // fewer tokens than that: all stay
         u64 base = sh.b_before;
         uint32_t bin = sh.b_bin, cnt = sh.b_count;
-        const u64 old = cut;
-        auto stays = [&](int i, float l) { return pack(l, first + i) >= old; };
         auto in_bin = [&](int i, float l) { return bin_of(l) == static_cast<int>(bin) && eligible(l) && stays(i, l); };
         if (cnt <= kList) return cut_in_list<MASS>(in_bin, base, target);
         // a crowded bin: divide the interval of its logits' keys
@@ -292,12 +427,12 @@ struct Row {
             lo = min(lo, *cluster.map_shared_rank(&sh.x_min, r));
             hi = max(hi, *cluster.map_shared_rank(&sh.x_max, r));
         }
+        auto within = [&](int i, float l) {
+            const uint32_t k = order_key(l);
+            return k >= lo && k <= hi && eligible(l) && stays(i, l);
+        };
         while (lo < hi) {
             const int shift = max(0, 32 - __clz(hi - lo) - 10);
-            auto within = [&](int i, float l) {
-                const uint32_t k = order_key(l);
-                return l == l && k >= lo && k <= hi && eligible(l) && stays(i, l);
-            };
             clear_bins();
             each([&](int i, float l) {
                 if (!within(i, l)) return;
@@ -312,90 +447,71 @@ struct Row {
             const uint32_t top = hi - (bin << shift);
             lo = max(lo, top - min(top, (1u << shift) - 1));
             hi = top;
-            if (cnt <= kList) {
-                // (`within` reads lo and hi: the new interval)
-                return cut_in_list<MASS>(within, base, target);
-            }
+            if (cnt <= kList) return cut_in_list<MASS>(within, base, target);
         }
         // equal logits: the lowest indices, as many as it takes
         const uint32_t key = lo;
         const u64 one = MASS ? weight(key_value(key)) : 1, need = (target - base + one - 1) / one;
-        auto same = [&](int i, float l) -> u64 { return l == l && order_key(l) == key && stays(i, l); };
-        locate(same, warp_part(same), [&](u64) { return need - 1; }, [&](int i, float l) {
-            for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&sh.x_cut, r) = pack(l, first + i);
+        auto same = [&](int i, float l) -> u64 { return order_key(l) == key && stays(i, l); };
+        u64 mine = 0;
+        each([&](int i, float l) { mine += same(i, l); });
+        locate(same, mine, [&](u64) { return need - 1; }, [&](int i, float l) {
+            for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&sh.x_cut, r) = order(i, l);
         });
         cluster.sync();
         cut = sh.x_cut;
     }
-    __device__ __forceinline__ int bin_of(float l) const { return min(kBins - 1, static_cast<int>(-coarse(l) * (kBins / kRange))); }
 };
 
 template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleTokens p, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens p, int slice) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ Shared sh;
     Row<T, RESIDENT> row(sh);
+    constexpr int N = Vec<T>::N;
     row.blocks = static_cast<int>(row.cluster.num_blocks());
     row.rank = static_cast<int>(row.cluster.block_rank());
     row.warp = threadIdx.x >> 5;
     row.lane = threadIdx.x & 31;
-    const int b = blockIdx.x / row.blocks;
-    row.first = row.rank * slice;
-    row.n = max(0, min(p.V, row.first + slice) - row.first);
-    row.seg = (row.n + kWarps - 1) / kWarps;
-    const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
-    const int k = p.top_k ? p.top_k[b] : p.top_k_all;
-    const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
-    if (threadIdx.x < 64) sh.table[threadIdx.x] = exp2(threadIdx.x / 64.);
+    const int b = blockIdx.x / row.blocks, begin = row.rank * slice;
+    const T* src = static_cast<const T*>(p.logits) + b * p.row_stride + begin;
+    row.off = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+    row.end = row.off + max(0, min(p.V - begin, slice));
+    row.first = begin - row.off;
+    row.nvec = (row.end + N - 1) / N;
+    row.seg = (row.nvec + kWarps - 1) / kWarps;
+    const uint4* gx = reinterpret_cast<const uint4*>(src - row.off);
+    row.x = RESIDENT ? reinterpret_cast<const uint4*>(dyn) : gx;
 
-    // the row's part, and its largest logit (lowest index); shared memory keeps the offset from a 16-byte boundary
-    const T* src = static_cast<const T*>(p.logits) + b * p.row_stride + row.first;
-    constexpr int VE = 16 / sizeof(T);
-    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
-    T* keep = reinterpret_cast<T*>(dyn) + off;
-    row.x = RESIDENT ? keep : src;
-    const int head = min(row.n, off ? VE - off : 0), nv = (row.n - head) / VE, tail = head + nv * VE;
+    // the row's part, and the largest logit that the thread meets (NaN never is)
     float best = -INFINITY;
-    int best_i = -1;
-    auto look = [&](int i, float l) {
-        if (l > best) { best = l; best_i = i; }                    // a thread's tokens come in the order of their indices; NaN never wins
-    };
-    if (static_cast<int>(threadIdx.x) < head) {
-        const T v = src[threadIdx.x];
-        if (RESIDENT) keep[threadIdx.x] = v;
-        look(threadIdx.x, to_f(v));
-    }
-    constexpr int DEPTH = 4;
-    for (int base = threadIdx.x; base < nv; base += kThreads * DEPTH) {
+    constexpr int DEPTH = 5;
+    for (int base = threadIdx.x; base < row.nvec; base += kThreads * DEPTH) {
         uint4 v[DEPTH];
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
-            if (base + d * kThreads < nv) v[d] = __ldg(reinterpret_cast<const uint4*>(src + head) + base + d * kThreads);
+            if (base + d * kThreads < row.nvec) v[d] = row.from_global(gx, base + d * kThreads);
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            const int i = base + d * kThreads;
-            if (i >= nv) break;
-            if (RESIDENT) reinterpret_cast<uint4*>(keep + head)[i] = v[d];
-            const T* e = reinterpret_cast<const T*>(&v[d]);
+            if (base + d * kThreads >= row.nvec) break;
+            if (RESIDENT) reinterpret_cast<uint4*>(dyn)[base + d * kThreads] = v[d];
+            float l[N];
+            Vec<T>::get(v[d], l);
 #pragma unroll
-            for (int j = 0; j < VE; ++j) look(head + i * VE + j, to_f(e[j]));
+            for (int j = 0; j < N; ++j) best = fmaxf(best, l[j]);
         }
     }
-    if (tail + static_cast<int>(threadIdx.x) < row.n) {
-        const int i = tail + threadIdx.x;
-        const T v = src[i];
-        if (RESIDENT) keep[i] = v;
-        look(i, to_f(v));
-    }
-    u64 top = best_i >= 0 ? pack(best, row.first + best_i) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (row.lane == 0) sh.warp_q[row.warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max(top, sh.warp_q[w]);
-    if (threadIdx.x == 0) sh.x_best = top;
+    const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
+    const int k = p.top_k ? p.top_k[b] : p.top_k_all;
+    const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
+    const bool greedy = !(temp > 0.f), use_k = !greedy && k > 0 && k < p.V, use_p = !greedy && top_p < 1.f, use_m = !greedy && min_p > 0.f;
+    if (!greedy)
+        for (int i = threadIdx.x; i < kTable; i += kThreads) sh.table[i] = exp2(i * (1. / kTable));
+    uint32_t top = __reduce_max_sync(0xffffffffu, best == -INFINITY ? 0u : order_key(best));
+    if (threadIdx.x == 0) { sh.x_best = 0; sh.x_index = 0xffffffffu; sh.x_first = row.first; }
     row.clear_bins();
+    if (row.lane == 0) atomicMax(&sh.x_best, top);
+    __syncthreads();
     row.cluster.sync();
     for (int r = 0; r < row.blocks; ++r) top = max(top, *row.cluster.map_shared_rank(&sh.x_best, r));
     if (top == 0) {                                                // nothing above -inf: nothing to draw
@@ -403,77 +519,175 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleTokens p,
         row.cluster.sync();
         return;
     }
-    row.lmax = key_value(static_cast<uint32_t>(top >> 32));
-    const int imax = static_cast<int>(0xffffffffu - static_cast<uint32_t>(top));
-    const bool greedy = !(temp > 0.f), use_k = !greedy && k > 0 && k < p.V, use_p = !greedy && top_p < 1.f;
-    row.to_log2 = greedy ? 0. : kLog2eD / static_cast<double>(temp);
+    row.lmax = key_value(top);
+    row.to_log2 = greedy ? 1. : kLog2eD / static_cast<double>(temp);
+    row.steep = !(fabs(static_cast<double>(row.lmax)) * row.to_log2 < 1e8);
     row.bin_scale = static_cast<float>(row.to_log2);
-    row.least = !greedy && min_p > 0.f ? max(-45., log2(static_cast<double>(fminf(min_p, 1.f)))) : -45.;
-    row.least_lo = static_cast<float>(row.least) * 1.0001f - 1e-6f;
-    row.least_hi = static_cast<float>(row.least) * 0.9999f + 1e-6f;
+    row.by_min_p = use_m;
+    row.least = use_m ? log2(static_cast<double>(fminf(min_p, 1.f))) : -kRange;
+    const float lowest = row.logit_below(-kRange);
+    row.floor_l = use_m ? row.logit_below(fmax(row.least, -static_cast<double>(kRange))) : lowest;
 
-    // the sum for the log-probability, and with it what the first cut (or the draw) needs
+    // the sum for the log-probability, and with it what the draw, or the bound for top-p's candidates, needs
+    const bool need_mass = !greedy && !use_k, z_is_mass = need_mass && temp == 1.f && !(min_p > 0.f);
+    const float k2e = static_cast<float>(kLog2eD);
     float z = 0.f;
-    auto add_z = [&](float l) { z += l == row.lmax ? 1.f : exp2f((l - row.lmax) * static_cast<float>(kLog2eD)); };
-    u64 drawn = 0;
-    auto kept_weight = [&](int i, float l) -> u64 { return row.eligible(l) && pack(l, row.first + i) >= row.cut ? row.weight(l) : 0; };
-    if (greedy) {
-        row.each([&](int, float l) { if (l == l) add_z(l); });
-    } else if (!use_k && !use_p) {
-        const int a = row.warp * row.seg, e = min(row.n, a + row.seg);
-        for (int i = a + row.lane; i < e; i += 32) {
-            const float l = row.at(i);
-            if (l != l) continue;
-            add_z(l);
-            drawn += kept_weight(i, l);
+    u64 mass = 0;
+    uint32_t at = 0xffffffffu;
+    {
+        const int e = min(row.nvec, (row.warp + 1) * row.seg);
+        for (int v = row.warp * row.seg + row.lane; v < e; v += 32) {
+            float l[N];
+            Vec<T>::get(row.vec(v), l);
+            if (!z_is_mass) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float d = l[j] == row.lmax ? 0.f : l[j] - row.lmax;      // (equal infinities)
+                    z += l[j] == l[j] ? ex2(d * k2e) : 0.f;
+                }
+            }
+            if (greedy) {
+#pragma unroll
+                for (int j = N - 1; j >= 0; --j)
+                    if (l[j] == row.lmax) at = min(at, static_cast<uint32_t>(row.first + v * N + j));
+            }
+            if (need_mass) {
+                float most = l[0];
+#pragma unroll
+                for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+                if (most >= row.floor_l) {
+                    if (!use_m) {                                  // (no branch for each logit: one below the floor is taken for the floor)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) mass += l[j] >= lowest ? row.weight(fmaxf(l[j], lowest)) : 0;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+                            if (l[j] >= row.floor_l && row.eligible(l[j])) mass += row.weight(l[j]);
+                    }
+                }
+            }
         }
-    } else {
-        row.each([&](int, float l) {
-            if (l != l) return;
-            add_z(l);
-            if (!row.eligible(l)) return;
-            const int bin = row.bin_of(l);
-            atomicAdd(&sh.count[bin], 1u);
-            if (!use_k) atomicAdd(&sh.mass[bin], row.weight(l));
-        });
     }
+    auto kept_weight = [&](int i, float l) -> u64 { return row.eligible(l) && row.order(i, l) >= row.cut ? row.weight(l) : 0; };
+    float log_z = 0.f;
+    auto aim = [&](u64 total) {
+        const double t = static_cast<double>(u > 0.f ? u : 0.f) * static_cast<double>(total);
+        return min(total - 1, static_cast<u64>(t));
+    };
+    auto found = [&](int i, float l) {
+        p.token[b] = row.first + i;
+        p.logprob[b] = (l == row.lmax ? 0.f : l - row.lmax) - log_z;
+    };
+    // the k largest logits are not below the k-th of these maxima
+    const bool by_maxima = use_k && k <= row.blocks * (kThreads / 4);
+    if (by_maxima && best >= row.floor_l) atomicAdd(&sh.count[row.bin_of(best)], 1u);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if (row.lane == 0) sh.warp_z[row.warp] = z;
-    __syncthreads();
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (row.lane == 0) {
+        sh.warp_z[row.warp] = z;
+        if (greedy) atomicMin(&sh.x_index, at);
+    }
+    const u64 own_mass = row.block_sums(mass);                     // (barriers of the block)
     if (threadIdx.x == 0) {
         float s = 0.f;
         for (int w = 0; w < kWarps; ++w) s += sh.warp_z[w];
         sh.x_z = s;
+        sh.x_sum = own_mass;
     }
-    row.cluster.sync();
+    if (by_maxima) {
+        u64 target = k;
+        if (row.template find_bin<false>(-1., 0, target)) row.floor_l = fmaxf(row.floor_l, row.logit_below(-(sh.b_bin + 1.001) * (kRange / kBins)));
+    } else {
+        __syncthreads();
+        row.cluster.sync();
+    }
+    u64 whole = 0;
     z = 0.f;
-    for (int r = 0; r < row.blocks; ++r) z += *row.cluster.map_shared_rank(&sh.x_z, r);
-
+    for (int r = 0; r < row.blocks; ++r) {
+        z += *row.cluster.map_shared_rank(&sh.x_z, r);
+        whole += *row.cluster.map_shared_rank(&sh.x_sum, r);
+        at = min(at, *row.cluster.map_shared_rank(&sh.x_index, r));
+    }
+    log_z = logf(z_is_mass ? static_cast<float>(static_cast<double>(whole) * (1. / (1ull << kFrac))) : z);
     if (greedy) {
-        if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = imax; p.logprob[b] = -logf(z); }
+        if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = static_cast<int>(at); p.logprob[b] = -log_z; }
         row.cluster.sync();
         return;
     }
-    if (use_k) row.template find_cut<false>(-1., static_cast<u64>(k));
-    if (use_p) {
-        if (use_k) {
-            row.clear_bins();
-            row.each([&](int i, float l) {
-                if (l != l || !row.eligible(l) || pack(l, row.first + i) < row.cut) return;
-                atomicAdd(&sh.count[row.bin_of(l)], 1u);
-                atomicAdd(&sh.mass[row.bin_of(l)], row.weight(l));
-            });
-        }
-        row.template find_cut<true>(fmaxf(top_p, 0.f), 0);
+    if (!use_k && !use_p) {
+        row.cluster.sync();                                        // (x_sum is written again)
+        row.locate(kept_weight, mass, aim, found);
+        row.cluster.sync();
+        return;
     }
-    if (use_k || use_p) drawn = row.warp_part(kept_weight);
-    row.locate(kept_weight, drawn,
-               [&](u64 total) {
-                   const double t = static_cast<double>(u > 0.f ? u : 0.f) * static_cast<double>(total);
-                   return min(total - 1, static_cast<u64>(t));
-               },
-               [&](int i, float l) { p.token[b] = row.first + i; p.logprob[b] = (l == row.lmax ? 0.f : l - row.lmax) - logf(z); });
+    const double share = fmax(static_cast<double>(top_p), 0.);
+    if (use_p && !use_k) {
+        // (.999: their multiples of 2^-44 are rounded, each by half a multiple at most)
+        const double light = (1. - share) * 0.999 * static_cast<double>(whole) / p.V;
+        if (light > 1000.) row.floor_l = fmaxf(row.floor_l, row.logit_below(fmin(log2(light) - kFrac, 0.)));
+    }
+    int total = 0;
+    const bool noted = row.note_down(total);
+    if (noted && total <= kList) {                                 // one block has them all, in the order of their indices, one a thread
+        const int i = threadIdx.x;
+        u64 me = 0;
+        if (row.rank == 0) {
+            uint32_t* upto = sh.count;                             // candidates through each warp of the cluster
+            if (row.warp == 0) {
+                constexpr int PER = kMaxCluster * kWarps / 32;
+                uint32_t c[PER], sum = 0;
+#pragma unroll
+                for (int x = 0; x < PER; ++x) {
+                    const int w = row.lane * PER + x, r = w / kWarps;
+                    c[x] = r < row.blocks ? *row.cluster.map_shared_rank(&sh.warp_n[w % kWarps], r) : 0;
+                    sum += c[x];
+                }
+                uint32_t through = static_cast<uint32_t>(warp_scan(sum, row.lane)) - sum;
+#pragma unroll
+                for (int x = 0; x < PER; ++x) upto[row.lane * PER + x] = through += c[x];
+            }
+            __syncthreads();
+            if (i < total) {
+                int w = 0;                                         // the first warp through which there are more than i
+#pragma unroll
+                for (int half = kMaxCluster * kWarps / 2; half > 0; half >>= 1)
+                    if (upto[w + half - 1] <= static_cast<uint32_t>(i)) w += half;
+                const Shared* from = row.cluster.map_shared_rank(&sh, w / kWarps);
+                const int at_i = w % kWarps * kOwn + i - static_cast<int>(w ? upto[w - 1] : 0);
+                const float l = from->own_l[at_i];
+                if (row.eligible(l)) me = pack(l, from->own_i[at_i] + from->x_first);
+            }
+        }
+        row.cluster.sync();                                        // the other blocks are done
+        if (row.rank != 0) return;
+        const float l = key_value(static_cast<uint32_t>(me >> 32));
+        const u64 w = me ? row.weight(l) : 0;
+        sh.all[i] = me;
+        sh.all_q[i] = w;
+        __syncthreads();
+        int ahead = 0;
+        u64 before = 0;
+        for (int j = 0; j < total; ++j)
+            if (sh.all[j] > me) { ++ahead; before += sh.all_q[j]; }
+        bool keep = me != 0 && (!use_k || ahead < k);
+        if (use_p) {
+            const u64 target = row.share_of(share, use_k ? row.block_sums(keep ? w : 0) : whole);
+            keep = keep && before < target;
+        }
+        const u64 mine = keep ? w : 0, target = aim(row.block_sums(mine));
+        row.block_find(mine, target, [&](u64) {
+            p.token[b] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(me));
+            p.logprob[b] = (l == row.lmax ? 0.f : l - row.lmax) - log_z;
+        });
+        return;
+    }
+    row.listed = noted;
+    if (use_k) row.template find_cut<false>(-1., static_cast<u64>(k));
+    if (use_p) row.template find_cut<true>(use_k ? share : -1., row.share_of(share, whole));   // without top-k the share is one of the whole row
+    u64 drawn = 0;
+    row.each([&](int i, float l) { drawn += kept_weight(i, l); });
+    row.locate(kept_weight, drawn, aim, found);
     row.cluster.sync();
 }
 
@@ -481,7 +695,7 @@ template <typename T, bool RESIDENT>
 const char* launch(const SampleTokens& p, int blocks, int slice, int smem, cudaStream_t s) {
     static std::atomic<uint64_t> raised{0};
     auto k = sample_tokens_kernel<T, RESIDENT>;
-    if (RESIDENT && !raise_smem_limit(reinterpret_cast<const void*>(k), 200 * 1024, raised)) return "sample_tokens: the shared-memory limit could not be raised";
+    if (RESIDENT && !raise_smem_limit(reinterpret_cast<const void*>(k), kMost, raised)) return "sample_tokens: the shared-memory limit could not be raised";
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -503,11 +717,11 @@ const char* launch(const SampleTokens& p, int blocks, int slice, int smem, cudaS
 template <typename T>
 const char* launch_type(const SampleTokens& p, int num_sms, cudaStream_t s) {
     // Blocks a row: enough that two blocks fit an SM (80 KB of the row each), more of them while the rows alone would leave SMs idle.
-    constexpr int64_t kFit = 80 * 1024, kMost = 190 * 1024;
+    constexpr int64_t kFit = 80 * 1024;
     int blocks = 1;
     while (blocks < kMaxCluster && (static_cast<int64_t>(p.V) * sizeof(T) > kFit * blocks || (static_cast<int64_t>(p.B) * blocks * 2 <= num_sms && p.V > 2048 * blocks))) blocks *= 2;
     const int slice = ((p.V + blocks - 1) / blocks + 15) / 16 * 16;
-    const int64_t bytes = static_cast<int64_t>(slice) * sizeof(T) + 16;
+    const int64_t bytes = static_cast<int64_t>(slice) * sizeof(T) + 32;    // (a part begins up to 15 bytes behind a 16-byte boundary)
     if (bytes <= kMost) return launch<T, true>(p, blocks, slice, static_cast<int>(bytes), s);
     return launch<T, false>(p, blocks, slice, 0, s);               // a vocabulary beyond 8 x 190 KB is read again in every pass
 }
