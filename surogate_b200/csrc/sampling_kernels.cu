@@ -8,7 +8,7 @@
 // memory; the passes over it (maximum; sums; the candidates) stay on the chip, and the blocks exchange a few words after each.
 //
 // * The result is a token, not a number that may be a little off, so masses are integers: weights as multiples of 2^-44 of the largest one
-//   (exponentials in fp64 by a table of 2^(j/1024) and two terms of the series: relative error 2^-37), whose sums do not depend on the order.
+//   (exponentials in fp64 by a table of 2^(j/64) and four terms of the series: relative error 2^-44), whose sums do not depend on the order.
 //   A wrong token takes a u within that of a boundary.
 // * Cuts need no sort.  Bounds leave a few candidates: the k largest logits are not below the k-th of the threads' own maxima; tokens lighter
 //   than (1 - top_p) / vocabulary of the whole mass make up less than 1 - top_p together, so the cut of top-p lies above them.  Up to 512
@@ -22,6 +22,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <utility>
 
 #include "launch_limits.h"
 #include "sampling.h"
@@ -37,7 +38,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = 512,
 constexpr int kOwn = 64;                      // candidates a warp can note down
 constexpr int kFrac = 44;                     // weights are multiples of 2^-44
 constexpr float kRange = 46.f;                // minus log2 of the smallest weight that is looked at: what lies below is 0 as a multiple
-constexpr int kTable = 1024;
+constexpr int kTable = 64, kCopies = 16;      // 2^(j / 64), a copy for each of 16 lanes so that none meet in a bank
 constexpr int kMost = 190 * 1024;             // bytes of a row that a block holds at most, beside 29 KB of its own
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 
@@ -65,24 +66,24 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {   // inclusive
 }
 
 struct Shared {
-    double table[kTable];             // 2^(j / 1024)
+    double table[kTable * kCopies];
+    union {
+        struct { uint32_t mass_lo[kBins], mass_hi[kBins], count[kBins]; };
+        struct { u64 list[kList], all[kList], all_q[kList]; };   // a block's candidates for a cut, and all blocks'
+    };
     float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
     int own_i[kWarps * kOwn];
-    union {
-        struct { u64 mass[kBins]; uint32_t count[kBins]; };
-        struct { u64 all[kList], all_q[kList]; };
-    };
     u64 warp_q[kWarps];
     float warp_z[kWarps];
     int warp_n[kWarps];               // candidates of each warp
     // what other blocks of the cluster read
-    u64 x_sum, x_cut;
+    u64 x_sum, x_cut, x_bins;
     float x_z;
     int x_first;                      // index of place 0
     uint32_t x_best, x_index, x_min, x_max, x_listed, x_noted;
-    // results of one thread for its block
+    // the bin found, told to all blocks
     u64 b_before;
-    uint32_t b_bin, b_count;
+    uint32_t b_bin;
 };
 
 // 16 bytes of logits as fp32
@@ -161,28 +162,56 @@ struct Row {
         const double l = static_cast<double>(lmax) + log2_w * 1.000001 / to_log2;
         return fmaxf(__double2float_rd(l - fabs(l) * 1e-6), -3.402823466e38f);        // (-inf never counts; NaN, from infinities: the lowest number)
     }
-    // 2^log2_weight as a multiple of 2^-44, for l >= floor_l: t = i / 1024 + r, 2^r = 1 + r (ln 2 + r ln2^2 / 2).  Adding 256 to it as an fp64
-    // leaves the multiple in the lowest bits.
-    __device__ __forceinline__ u64 weight(float l) const {
+    // 2^log2_weight as multiples of 2^-44, for logits that are not below the lowest floor: t = i / 64 + r, 2^r by its series to the fourth power
+    // (|r| <= 2^-7: 4e-14).  Adding 256 to it as an fp64 leaves the multiple in the lowest bits.
+    __device__ __forceinline__ u64 fast_weight(float l) const {
         const double d = static_cast<double>(l) - static_cast<double>(lmax);
-        if (steep) {
-            if (l == lmax) return 1ull << kFrac;
-            if (!(d * to_log2 >= -60.)) return 0;
-        }
-        const double big = 6755399441055744. / kTable;            // 1.5 * 2^52 / 1024: adding it rounds to multiples of 1 / 1024
+        const double big = 6755399441055744. / kTable;            // 1.5 * 2^52 / 64: adding it rounds to multiples of 1 / 64
         const double m = fma(d, to_log2, big);
         const int i = __double2loint(m);
         const double r = fma(d, to_log2, big - m);
-        const double e = sh.table[i & (kTable - 1)];
-        const double v = fma(e * r, fma(r, kLn2D * kLn2D / 2, kLn2D), e);
-        const double w = __hiloint2double(__double2hiint(v) + ((i >> 10) << 20), __double2loint(v));
+        const double e = sh.table[(i & (kTable - 1)) * kCopies + (lane & (kCopies - 1))];
+        double y = fma(r, kLn2D * kLn2D * kLn2D * kLn2D / 24, kLn2D * kLn2D * kLn2D / 6);
+        y = fma(r, y, kLn2D * kLn2D / 2);
+        y = fma(r, y, kLn2D);
+        const double v = fma(e * r, y, e);
+        const double w = __hiloint2double(__double2hiint(v) + ((i >> 6) << 20), __double2loint(v));
         return static_cast<u64>(__double_as_longlong(w + 256.)) - 0x4070000000000000ull;
     }
+    __device__ __forceinline__ u64 weight(float l) const {
+        if (steep) {
+            if (l == lmax) return 1ull << kFrac;
+            if (!((static_cast<double>(l) - static_cast<double>(lmax)) * to_log2 >= -60.)) return 0;
+        }
+        return fast_weight(l);
+    }
+    // weights of a vector's logits, 0 below `least_l` (which is not below the lowest floor): side by side, without a branch for each
+    __device__ __forceinline__ void weights(const float (&l)[N], float least_l, u64 (&w)[N]) const {
+        if (!steep) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = fast_weight(fmaxf(l[j], least_l));
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = l[j] >= least_l ? w[j] : 0;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = l[j] >= least_l ? weight(l[j]) : 0;
+        }
+    }
+    // A word of each block of the cluster: lane r has that of block r, the lanes behind the last block zero
+    template <typename V> __device__ __forceinline__ V of_rank(V* own) const { return lane < blocks ? *cluster.map_shared_rank(own, lane) : V{}; }
+    __device__ __forceinline__ u64 sum_ranks(u64 v) const {
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return __shfl_sync(0xffffffffu, v, 0);
+    }
 
-    // f(place, logit) for the tokens that are not below floor_l, each warp its own in the order of their indices, lanes apart
-    template <typename F> __device__ __forceinline__ void each(F f) const {
+    // f(place, logit, weight if WEIGH) for the tokens that are not below floor_l, each warp its own in the order of their indices, lanes apart
+    template <bool WEIGH, typename F> __device__ __forceinline__ void each(F f) const {
         if (listed) {
-            for (int i = lane; i < sh.warp_n[warp]; i += 32) f(sh.own_i[warp * kOwn + i], sh.own_l[warp * kOwn + i]);
+            for (int i = lane; i < sh.warp_n[warp]; i += 32) {
+                const float l = sh.own_l[warp * kOwn + i];
+                if (l >= floor_l) f(sh.own_i[warp * kOwn + i], l, WEIGH ? weight(l) : 0);
+            }
             return;
         }
         const int b = min(nvec, (warp + 1) * seg);
@@ -193,9 +222,11 @@ struct Row {
 #pragma unroll
             for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
             if (!(most >= floor_l)) continue;
+            u64 w[N];
+            if (WEIGH) weights(l, floor_l, w);
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (l[j] >= floor_l) f(v * N + j, l[j]);
+                if (l[j] >= floor_l) f(v * N + j, l[j], WEIGH ? w[j] : 0);
         }
     }
     __device__ __forceinline__ u64 order(int place, float l) const { return pack(l, first + place); }
@@ -228,13 +259,12 @@ struct Row {
         const u64 own = block_sums(mine);
         if (threadIdx.x == 0) sh.x_sum = own;
         cluster.sync();
-        u64 before = 0, total = 0;
-        for (int r = 0; r < blocks; ++r) {
-            const u64 v = *cluster.map_shared_rank(&sh.x_sum, r);
-            if (r < rank) before += v;
-            total += v;
-        }
-        u64 target = aim(total);
+        locate_in(q, of_rank(&sh.x_sum), own, aim, found);
+    }
+    // the same, with the blocks' sums known: lane r has that of block r; the warps' are in sh.warp_q
+    template <typename Q, typename A, typename F> __device__ void locate_in(Q q, u64 of_blocks, u64 own, A aim, F found) {
+        u64 target = aim(sum_ranks(of_blocks));
+        const u64 before = __shfl_sync(0xffffffffu, warp_scan(of_blocks, lane) - of_blocks, rank);
         if (target < before || target >= before + own) return;            // another block's
         target -= before;
         int w = 0;
@@ -242,7 +272,7 @@ struct Row {
         if (listed) {
             const int i = threadIdx.x, place = i < kOwn ? sh.own_i[w * kOwn + i] : 0;
             const float l = i < kOwn ? sh.own_l[w * kOwn + i] : 0.f;
-            block_find(i < sh.warp_n[w] ? q(place, l) : 0, target, [&](u64) { found(place, l); });
+            block_find(i < sh.warp_n[w] && l >= floor_l ? q(place, l) : 0, target, [&](u64) { found(place, l); });
             return;
         }
         const int a = w * seg, b = min(nvec, a + seg), per = (b - a + kThreads - 1) / kThreads, va = min(b, a + static_cast<int>(threadIdx.x) * per), vb = min(b, va + per);
@@ -270,127 +300,156 @@ struct Row {
     __device__ bool note_down(int& total) {
         int n = 0;
         const int b = min(nvec, (warp + 1) * seg);
-        for (int base = warp * seg; base < b; base += 32) {
-            float l[N];
-            int c = 0;
+        for (int base = warp * seg; base < b && n <= kOwn; base += 32) {
+            float l[N], most = -INFINITY;
             if (base + lane < b) {
                 Vec<T>::get(vec(base + lane), l);
 #pragma unroll
-                for (int j = 0; j < N; ++j) c += l[j] >= floor_l;
+                for (int j = 0; j < N; ++j) most = fmaxf(most, l[j]);
             }
-            if (!__any_sync(0xffffffffu, c)) continue;
-            int upto = c;
+            if (!__any_sync(0xffffffffu, most >= floor_l)) continue;
+            const bool some = most >= floor_l;
+            int at = n, mine = 0;                                  // before this lane's: all of the lanes before it
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
+            for (int j = 0; j < N; ++j) {
+                const bool in = some && l[j] >= floor_l;
+                const unsigned all = __ballot_sync(0xffffffffu, in);
+                at += __popc(all & ((1u << lane) - 1));
+                n += __popc(all);
+                mine |= in << j;
             }
-            int at = n + upto - c;
-            if (c) {
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (l[j] >= floor_l) {
-                        if (at < kOwn) { sh.own_l[warp * kOwn + at] = l[j]; sh.own_i[warp * kOwn + at] = (base + lane) * N + j; }
-                        ++at;
-                    }
-            }
-            n += __shfl_sync(0xffffffffu, upto, 31);
+            for (int j = 0; j < N; ++j)
+                if (mine >> j & 1) {
+                    if (at < kOwn) { sh.own_l[warp * kOwn + at] = l[j]; sh.own_i[warp * kOwn + at] = (base + lane) * N + j; }
+                    ++at;
+                }
         }
         if (lane == 0) sh.warp_n[warp] = n;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t sum = 0;
-            for (int w = 0; w < kWarps; ++w) sum = sh.warp_n[w] > kOwn || sum >= 0x10000000u ? 0x10000000u : sum + sh.warp_n[w];
-            sh.x_noted = sum;
+        if (warp == 0) {
+            const int c = lane < kWarps ? sh.warp_n[lane] : 0;
+            const uint32_t sum = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(min(c, kOwn)));
+            if (lane == 0) sh.x_noted = sum;
+            if (__any_sync(0xffffffffu, c > kOwn) && lane == 0) sh.x_noted = 0x10000000u;
         }
         cluster.sync();
-        uint32_t sum = 0;
-        for (int r = 0; r < blocks; ++r) sum += *cluster.map_shared_rank(&sh.x_noted, r);
-        total = static_cast<int>(sum);
+        const u64 sum = sum_ranks(of_rank(&sh.x_noted));
+        total = static_cast<int>(min(sum, u64{0x10000000u}));
         return sum < 0x10000000u;
     }
 
     __device__ void clear_bins() {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) { sh.count[i] = 0; sh.mass[i] = 0; }
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
         __syncthreads();
     }
+    // 64-bit sums of two words each, so that a native 32-bit atomic does it
+    __device__ __forceinline__ void add_mass(int bin, u64 w) {
+        const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass_lo[bin], lo);
+        const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old);
+        if (hi) atomicAdd(&sh.mass_hi[bin], hi);
+    }
     // Adds up all blocks' bins; finds the one in which the target falls (before < target <= before + bin).  With `fraction` the target is that
-    // share of the whole.  False: the whole is less than the target.  Leaves the bin, what comes before it and its tokens in b_*.
+    // share of the whole.  False: the whole is less than the target.  Leaves the bin and what comes before it in b_*.
     template <bool MASS> __device__ bool find_bin(double fraction, u64 base, u64& target) {
         __syncthreads();
         cluster.sync();
-        constexpr int PER = kBins / kThreads;
-        u64 q[PER];
-        uint32_t cnt[PER];
-        u64 s = 0;
+        // A block adds up its share of the bins (words of other blocks are slow to get, so each is fetched once); their sums are exchanged, and the
+        // block in whose share the target falls tells the others the bin.
+        constexpr int PER = kBins / kThreads;                      // (at one block a row; with more of them some threads have none)
+        const int share = kBins / blocks, bin = rank * share + threadIdx.x * PER;
+        u64 q[PER], mine = 0;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            q[k] = 0;
-            cnt[k] = 0;
-            for (int r = 0; r < blocks; ++r) {
-                const int bin = threadIdx.x * PER + k;
-                cnt[k] += cluster.map_shared_rank(sh.count, r)[bin];
-                if (MASS) q[k] += cluster.map_shared_rank(sh.mass, r)[bin];
+        for (int k = 0; k < PER; ++k) q[k] = 0;
+        if (static_cast<int>(threadIdx.x) * PER < share) {
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                if (r >= blocks) break;
+                const Shared* from = cluster.map_shared_rank(&sh, r);
+#pragma unroll
+                for (int k = 0; k < PER; ++k) q[k] += MASS ? (static_cast<u64>(from->mass_hi[bin + k]) << 32) + from->mass_lo[bin + k] : from->count[bin + k];
             }
-            if (!MASS) q[k] = cnt[k];
-            s += q[k];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) mine += q[k];
         }
-        const u64 upto = warp_scan(s, lane);
+        const u64 upto = warp_scan(mine, lane);
         if (lane == 31) sh.warp_q[warp] = upto;
         __syncthreads();
-        u64 before = base + upto - s, total = base;
+        u64 before = upto - mine, own = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) before += sh.warp_q[w];
-            total += sh.warp_q[w];
+            own += sh.warp_q[w];
         }
+        if (threadIdx.x == 0) sh.x_bins = own;
+        cluster.sync();
+        const u64 of_blocks = of_rank(&sh.x_bins), total = base + sum_ranks(of_blocks);
         if (fraction >= 0.) target = share_of(fraction, total);
-        const bool inside = total >= target;
-        if (inside) {
+        if (total < target) return false;                          // (the same in all blocks)
+        before += base + __shfl_sync(0xffffffffu, warp_scan(of_blocks, lane) - of_blocks, rank);
 #pragma unroll
-            for (int k = 0; k < PER; ++k) {
-                if (before < target && target <= before + q[k]) { sh.b_bin = threadIdx.x * PER + k; sh.b_before = before; sh.b_count = cnt[k]; }
-                before += q[k];
+        for (int k = 0; k < PER; ++k) {
+            if (before < target && target <= before + q[k]) {
+                for (int r = 0; r < blocks; ++r) {
+                    Shared* to = cluster.map_shared_rank(&sh, r);
+                    to->b_bin = bin + k;
+                    to->b_before = before;
+                }
             }
+            before += q[k];
         }
-        __syncthreads();
-        cluster.sync();                                            // nobody reads these bins any more
-        return inside;
+        cluster.sync();                                            // b_* is there, and nobody reads these bins any more
+        return true;
     }
     // The least mass that a prefix must reach to be `fraction` of the whole
     static __device__ __forceinline__ u64 share_of(double fraction, u64 total) {
         return max(1ull, min(total, static_cast<u64>(ceil(fraction * static_cast<double>(total)))));
     }
 
-    // Ranks the tokens for which `in` holds (at most kList in the cluster) against one another; sets the cut.
-    template <bool MASS, typename In> __device__ void cut_in_list(In in, u64 base, u64 target) {
-        u64* list = reinterpret_cast<u64*>(sh.all);                // (the bins are done with)
-        if (threadIdx.x == 0) sh.x_listed = 0;
+    // Ranks the tokens for which `in` holds against one another and sets the cut, if they are at most kList in the cluster.
+    template <bool MASS, typename In> __device__ bool cut_in_list(In in, u64 base, u64 target) {
+        if (threadIdx.x == 0) sh.x_listed = 0;                     // (the bins are done with: the lists take their place)
         __syncthreads();
-        each([&](int i, float l) {
-            if (in(i, l)) list[min(atomicAdd(&sh.x_listed, 1u), static_cast<uint32_t>(kList - 1))] = order(i, l);
+        each<false>([&](int i, float l, u64) {
+            if (!in(i, l)) return;
+            const uint32_t at = atomicAdd(&sh.x_listed, 1u);
+            if (at < kList) sh.list[at] = order(i, l);
         });
         __syncthreads();
         cluster.sync();
-        // every warp of the cluster takes tokens of its own block and meets all lists, which stay where they are
-        const int own = min(static_cast<int>(sh.x_listed), kList);
-        for (int i = threadIdx.x; i < own; i += kThreads) sh.all_q[i] = MASS ? weight(key_value(static_cast<uint32_t>(list[i] >> 32))) : 1;
-        __syncthreads();
-        cluster.sync();
-        for (int i = warp; i < own; i += kWarps) {
-            const u64 me = list[i];
-            u64 s = 0;
-            for (int r = 0; r < blocks; ++r) {
-                const int c = min(static_cast<int>(*cluster.map_shared_rank(&sh.x_listed, r)), kList);
-                const u64 *from = cluster.map_shared_rank(list, r), *q = cluster.map_shared_rank(sh.all_q, r);
-                for (int j = lane; j < c; j += 32)
-                    if (from[j] > me) s += q[j];
+        const uint32_t of_block = of_rank(&sh.x_listed), total = static_cast<uint32_t>(sum_ranks(of_block));
+        const bool fits = total <= kList;
+        if (fits) {                                                // all lists come to each block, whose warps take every blocks-th token
+            const uint32_t upto = static_cast<uint32_t>(warp_scan(of_block, lane));
+            int r = 0;
+            uint32_t first_of = 0;
+#pragma unroll
+            for (int x = 0; x < kMaxCluster - 1; ++x) {
+                const uint32_t y = __shfl_sync(0xffffffffu, upto, x);
+                if (threadIdx.x >= y && x + 1 < blocks) { r = x + 1; first_of = y; }
             }
-            s = base + warp_sum(s);
-            if (s < target && target <= s + sh.all_q[i] && lane < blocks) *cluster.map_shared_rank(&sh.x_cut, lane) = me;
+            if (threadIdx.x < total) {
+                const u64 v = cluster.map_shared_rank(sh.list, r)[threadIdx.x - first_of];
+                sh.all[threadIdx.x] = v;
+                sh.all_q[threadIdx.x] = MASS ? weight(key_value(static_cast<uint32_t>(v >> 32))) : 1;
+            }
+            __syncthreads();
+            for (uint32_t i = warp * blocks + rank; i < total; i += kWarps * blocks) {
+                const u64 me = sh.all[i];
+                u64 s = 0;
+                for (uint32_t j = lane; j < total; j += 32)
+                    if (sh.all[j] > me) s += sh.all_q[j];
+                s = base + warp_sum(s);
+                if (s < target && target <= s + sh.all_q[i] && lane < blocks) *cluster.map_shared_rank(&sh.x_cut, lane) = me;
+            }
         }
         cluster.sync();
-        cut = sh.x_cut;
+        if (fits) set_cut(sh.x_cut);
+        return fits;
+    }
+    __device__ __forceinline__ void set_cut(u64 c) {
+        cut = c;
+        floor_l = fmaxf(floor_l, key_value(static_cast<uint32_t>(c >> 32)));
     }
 
     // Keeps the tokens, in the order of falling logit, before which less than `target` has come: tokens, or mass (a share of the whole).
@@ -398,22 +457,21 @@ struct Row {
         const u64 old = cut;
         auto stays = [&](int i, float l) { return order(i, l) >= old; };
         clear_bins();
-        each([&](int i, float l) {
+        each<MASS>([&](int i, float l, u64 w) {
             if (!eligible(l) || !stays(i, l)) return;
-            const int bin = bin_of(l);
-            atomicAdd(&sh.count[bin], 1u);
-            if (MASS) atomicAdd(&sh.mass[bin], weight(l));
+            if (MASS) add_mass(bin_of(l), w);
+            else atomicAdd(&sh.count[bin_of(l)], 1u);
         });
         if (!find_bin<MASS>(fraction, 0, target)) return;          // fewer tokens than that: all stay
         u64 base = sh.b_before;
-        uint32_t bin = sh.b_bin, cnt = sh.b_count;
+        uint32_t bin = sh.b_bin;
         auto in_bin = [&](int i, float l) { return bin_of(l) == static_cast<int>(bin) && eligible(l) && stays(i, l); };
-        if (cnt <= kList) return cut_in_list<MASS>(in_bin, base, target);
+        if (cut_in_list<MASS>(in_bin, base, target)) return;
         // a crowded bin: divide the interval of its logits' keys
         if (threadIdx.x == 0) { sh.x_min = 0xffffffffu; sh.x_max = 0; }
         __syncthreads();
         uint32_t lo = 0xffffffffu, hi = 0;
-        each([&](int i, float l) {
+        each<false>([&](int i, float l, u64) {
             if (in_bin(i, l)) { lo = min(lo, order_key(l)); hi = max(hi, order_key(l)); }
         });
         lo = __reduce_min_sync(0xffffffffu, lo);
@@ -421,12 +479,8 @@ struct Row {
         if (lane == 0) { atomicMin(&sh.x_min, lo); atomicMax(&sh.x_max, hi); }
         __syncthreads();
         cluster.sync();
-        lo = 0xffffffffu;
-        hi = 0;
-        for (int r = 0; r < blocks; ++r) {
-            lo = min(lo, *cluster.map_shared_rank(&sh.x_min, r));
-            hi = max(hi, *cluster.map_shared_rank(&sh.x_max, r));
-        }
+        lo = __reduce_min_sync(0xffffffffu, lane < blocks ? *cluster.map_shared_rank(&sh.x_min, lane) : 0xffffffffu);
+        hi = __reduce_max_sync(0xffffffffu, of_rank(&sh.x_max));
         auto within = [&](int i, float l) {
             const uint32_t k = order_key(l);
             return k >= lo && k <= hi && eligible(l) && stays(i, l);
@@ -434,32 +488,31 @@ struct Row {
         while (lo < hi) {
             const int shift = max(0, 32 - __clz(hi - lo) - 10);
             clear_bins();
-            each([&](int i, float l) {
+            each<MASS>([&](int i, float l, u64 w) {
                 if (!within(i, l)) return;
                 const uint32_t b = (hi - order_key(l)) >> shift;
-                atomicAdd(&sh.count[b], 1u);
-                if (MASS) atomicAdd(&sh.mass[b], weight(l));
+                if (MASS) add_mass(b, w);
+                else atomicAdd(&sh.count[b], 1u);
             });
             find_bin<MASS>(-1., base, target);
             base = sh.b_before;
             bin = sh.b_bin;
-            cnt = sh.b_count;
             const uint32_t top = hi - (bin << shift);
             lo = max(lo, top - min(top, (1u << shift) - 1));
             hi = top;
-            if (cnt <= kList) return cut_in_list<MASS>(within, base, target);
+            if (cut_in_list<MASS>(within, base, target)) return;
         }
         // equal logits: the lowest indices, as many as it takes
         const uint32_t key = lo;
         const u64 one = MASS ? weight(key_value(key)) : 1, need = (target - base + one - 1) / one;
         auto same = [&](int i, float l) -> u64 { return order_key(l) == key && stays(i, l); };
         u64 mine = 0;
-        each([&](int i, float l) { mine += same(i, l); });
+        each<false>([&](int i, float l, u64) { mine += same(i, l); });
         locate(same, mine, [&](u64) { return need - 1; }, [&](int i, float l) {
             for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&sh.x_cut, r) = order(i, l);
         });
         cluster.sync();
-        cut = sh.x_cut;
+        set_cut(sh.x_cut);
     }
 };
 
@@ -505,15 +558,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     const int k = p.top_k ? p.top_k[b] : p.top_k_all;
     const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
     const bool greedy = !(temp > 0.f), use_k = !greedy && k > 0 && k < p.V, use_p = !greedy && top_p < 1.f, use_m = !greedy && min_p > 0.f;
-    if (!greedy)
-        for (int i = threadIdx.x; i < kTable; i += kThreads) sh.table[i] = exp2(i * (1. / kTable));
+    if (!greedy && threadIdx.x < kTable) {
+        const double e = exp2(threadIdx.x * (1. / kTable));
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) sh.table[threadIdx.x * kCopies + (i + threadIdx.x) % kCopies] = e;
+    }
     uint32_t top = __reduce_max_sync(0xffffffffu, best == -INFINITY ? 0u : order_key(best));
     if (threadIdx.x == 0) { sh.x_best = 0; sh.x_index = 0xffffffffu; sh.x_first = row.first; }
     row.clear_bins();
     if (row.lane == 0) atomicMax(&sh.x_best, top);
     __syncthreads();
     row.cluster.sync();
-    for (int r = 0; r < row.blocks; ++r) top = max(top, *row.cluster.map_shared_rank(&sh.x_best, r));
+    top = __reduce_max_sync(0xffffffffu, row.of_rank(&sh.x_best));
     if (top == 0) {                                                // nothing above -inf: nothing to draw
         if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = -1; p.logprob[b] = -INFINITY; }
         row.cluster.sync();
@@ -556,14 +612,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 #pragma unroll
                 for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
                 if (most >= row.floor_l) {
-                    if (!use_m) {                                  // (no branch for each logit: one below the floor is taken for the floor)
+                    u64 w[N];
+                    row.weights(l, row.floor_l, w);
 #pragma unroll
-                        for (int j = 0; j < N; ++j) mass += l[j] >= lowest ? row.weight(fmaxf(l[j], lowest)) : 0;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < N; ++j)
-                            if (l[j] >= row.floor_l && row.eligible(l[j])) mass += row.weight(l[j]);
-                    }
+                    for (int j = 0; j < N; ++j) mass += use_m && !row.eligible(l[j]) ? 0 : w[j];
                 }
             }
         }
@@ -589,11 +641,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         if (greedy) atomicMin(&sh.x_index, at);
     }
     const u64 own_mass = row.block_sums(mass);                     // (barriers of the block)
-    if (threadIdx.x == 0) {
-        float s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s += sh.warp_z[w];
-        sh.x_z = s;
-        sh.x_sum = own_mass;
+    if (row.warp == 0) {
+        float s = row.lane < kWarps ? sh.warp_z[row.lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (row.lane == 0) { sh.x_z = s; sh.x_sum = own_mass; }
     }
     if (by_maxima) {
         u64 target = k;
@@ -602,23 +654,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         __syncthreads();
         row.cluster.sync();
     }
-    u64 whole = 0;
-    z = 0.f;
-    for (int r = 0; r < row.blocks; ++r) {
-        z += *row.cluster.map_shared_rank(&sh.x_z, r);
-        whole += *row.cluster.map_shared_rank(&sh.x_sum, r);
-        at = min(at, *row.cluster.map_shared_rank(&sh.x_index, r));
-    }
+    z = row.of_rank(&sh.x_z);
+    const u64 of_blocks = row.of_rank(&sh.x_sum), whole = row.sum_ranks(of_blocks);
+    if (greedy) at = __reduce_min_sync(0xffffffffu, row.lane < row.blocks ? *row.cluster.map_shared_rank(&sh.x_index, row.lane) : 0xffffffffu);
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    z = __shfl_sync(0xffffffffu, z, 0);
     log_z = logf(z_is_mass ? static_cast<float>(static_cast<double>(whole) * (1. / (1ull << kFrac))) : z);
-    if (greedy) {
-        if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = static_cast<int>(at); p.logprob[b] = -log_z; }
-        row.cluster.sync();
-        return;
-    }
-    if (!use_k && !use_p) {
-        row.cluster.sync();                                        // (x_sum is written again)
-        row.locate(kept_weight, mass, aim, found);
-        row.cluster.sync();
+    if (greedy || (!use_k && !use_p)) {
+        auto here = row.cluster.barrier_arrive();                  // nothing of this block is read by others after they have got here
+        if (!greedy) row.locate_in(kept_weight, of_blocks, own_mass, aim, found);
+        else if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = static_cast<int>(at); p.logprob[b] = -log_z; }
+        row.cluster.barrier_wait(std::move(here));
         return;
     }
     const double share = fmax(static_cast<double>(top_p), 0.);
@@ -686,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     if (use_k) row.template find_cut<false>(-1., static_cast<u64>(k));
     if (use_p) row.template find_cut<true>(use_k ? share : -1., row.share_of(share, whole));   // without top-k the share is one of the whole row
     u64 drawn = 0;
-    row.each([&](int i, float l) { drawn += kept_weight(i, l); });
+    row.template each<true>([&](int i, float l, u64 w) { drawn += row.eligible(l) && row.order(i, l) >= row.cut ? w : 0; });
     row.locate(kept_weight, drawn, aim, found);
     row.cluster.sync();
 }
