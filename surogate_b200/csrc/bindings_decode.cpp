@@ -36,6 +36,13 @@ const int* index_ptr(const Tensor& t, const Tensor& like, int64_t n, const char*
     return t.data_ptr<int>();
 }
 
+// `t` where its last dimension is contiguous and all before it 16-byte aligned, else a copy that is
+Tensor rows16(const Tensor& t) {
+    bool ok = aligned(t.data_ptr(), 16) && (t.size(-1) < 2 || t.stride(-1) == 1);
+    for (int64_t d = 0; ok && d + 1 < t.dim(); ++d) ok = t.size(d) < 2 || t.stride(d) * t.element_size() % 16 == 0;
+    return ok || t.numel() == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // One layer's pages [pages, 2, heads, page size, dim]
 sg::KvPages pages_of(const Tensor& kv, const OptTensor& scales) {
     TORCH_CHECK(kv.is_cuda() && kv.dim() == 5 && kv.size(1) == 2, "kv must be a CUDA tensor [pages, 2, kv heads, page size, head size]");
@@ -84,30 +91,28 @@ void table_of(const Tensor& table, const Tensor& kv, int64_t B, const int*& ptr,
 void kv_append(const Tensor& kv, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& start, const OptTensor& count, const OptTensor& scales) {
     sg::KvAppend p{};
     p.kv = pages_of(kv, scales);
-    const Tensor* src[2] = {&k, &v};
+    TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == kv.device() && v.device() == kv.device() && k.size(2) == p.kv.heads &&
+                    k.size(3) == p.kv.dim,
+                "k and v must be [rows, tokens, ", num(p.kv.heads), ", ", num(p.kv.dim), "] of one type on the cache's device");
+    p.src_type = kv_type(k, "k and v");
+    TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.src_type != sg::kKvE4m3 : p.src_type == p.kv.type, "k and v must have the cache's type (with an e4m3 cache: bf16, fp16 or fp32)");
+    const c10::cuda::CUDAGuard guard(kv.device());
+    const Tensor src[2] = {rows16(k), rows16(v)};
     for (int i = 0; i < 2; ++i) {
-        const Tensor& t = *src[i];
-        TORCH_CHECK(t.device() == kv.device() && t.dim() == 4 && t.size(2) == p.kv.heads && t.size(3) == p.kv.dim && t.sizes() == k.sizes() && t.scalar_type() == k.scalar_type(),
-                    "k and v must be [rows, tokens, ", num(p.kv.heads), ", ", num(p.kv.dim), "] of one type on the cache's device");
-        const int64_t es = t.element_size();
-        TORCH_CHECK((t.size(3) < 2 || t.stride(3) == 1) && aligned(t.data_ptr(), 16) && t.stride(0) * es % 16 == 0 && t.stride(1) * es % 16 == 0 && t.stride(2) * es % 16 == 0,
-                    "k and v: the elements of a head must be contiguous, heads 16-byte aligned");
+        const Tensor& t = src[i];
         p.src[i] = t.data_ptr();
         p.b_stride[i] = t.stride(0);
         p.t_stride[i] = t.stride(1);
         p.h_stride[i] = t.stride(2);
     }
-    p.src_type = kv_type(k, "k and v");
-    TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.src_type != sg::kKvE4m3 : p.src_type == p.kv.type, "k and v must have the cache's type (with an e4m3 cache: bf16, fp16 or fp32)");
     const int64_t B = k.size(0), T = k.size(1);
-    TORCH_CHECK(B < (int64_t{1} << 31) && T < (int64_t{1} << 30) && B * T * 2 * p.kv.heads * 32 < (int64_t{1} << 40), "k and v: too many tokens for one call");
+    TORCH_CHECK(B <= 65535 && T < (int64_t{1} << 30) && B * T * 2 * p.kv.heads < (int64_t{1} << 34), "k and v: at most 65535 rows, and 2^34 heads, in one call");
     if (B == 0 || T == 0) return;
     table_of(table, kv, B, p.table, p.table_stride, p.table_width);
     p.start = index_ptr(start, kv, B, "start");
     if (given(count)) p.count = index_ptr(*count, kv, B, "count");
     p.B = static_cast<int>(B);
     p.T = static_cast<int>(T);
-    const c10::cuda::CUDAGuard guard(kv.device());
     p.error_flag = sg_error_flag();
     sg_count_launch(1);
     sg::kv_append(p, cur_stream());
@@ -147,21 +152,21 @@ void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const
 }
 
 // -> (output [B, Hq, dim], log-sum-exp fp32 [B, Hq] or undefined)
-std::vector<Tensor> paged_attention(const Tensor& q, const Tensor& kv, const Tensor& table, const Tensor& lengths, double scale, int64_t window, double softcap,
+std::tuple<Tensor, Tensor> paged_attention(const Tensor& q_given, const Tensor& kv, const Tensor& table, const Tensor& lengths, double scale, int64_t window, double softcap,
                                     const OptTensor& sinks, const OptTensor& scales, bool want_lse) {
     sg::PagedAttention p{};
     p.kv = pages_of(kv, scales);
     TORCH_CHECK(p.kv.type != sg::kKvFp32, "paged_attention reads bf16, fp16 and float8_e4m3fn caches");
     TORCH_CHECK(p.kv.dim == 64 || p.kv.dim == 128 || p.kv.dim == 256, "paged_attention takes head sizes 64, 128 and 256, not ", num(p.kv.dim));
-    TORCH_CHECK(q.device() == kv.device() && q.dim() == 3 && q.size(2) == p.kv.dim, "q must be [rows, query heads, ", num(p.kv.dim), "] on the cache's device");
+    TORCH_CHECK(q_given.device() == kv.device() && q_given.dim() == 3 && q_given.size(2) == p.kv.dim, "q must be [rows, query heads, ", num(p.kv.dim), "] on the cache's device");
+    const c10::cuda::CUDAGuard guard(kv.device());
+    const Tensor q = rows16(q_given);
     p.q_type = kv_type(q, "q");
     TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.q_type == sg::kKvBf16 || p.q_type == sg::kKvFp16 : p.q_type == p.kv.type, "q must have the cache's type (with an e4m3 cache: bf16 or fp16)");
     TORCH_CHECK(q.size(1) > 0 && q.size(1) <= 65535 && q.size(1) % p.kv.heads == 0, "the query heads must be a multiple of the ", num(p.kv.heads), " key heads");
     const int64_t B = q.size(0);
     TORCH_CHECK(B <= 65535, "paged_attention: at most 65535 rows in one call");
-    TORCH_CHECK(q.stride(2) == 1 && aligned(q.data_ptr(), 16) && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0, "q: the elements of a head must be contiguous, heads 16-byte aligned");
     TORCH_CHECK(window >= 0 && softcap >= 0 && std::isfinite(scale) && std::isfinite(softcap), "window and softcap must not be negative, scale and softcap finite");
-    const c10::cuda::CUDAGuard guard(kv.device());
     Tensor out = torch::empty({B, q.size(1), q.size(2)}, q.options()), lse;
     if (want_lse) lse = torch::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
     if (B == 0) return {out, lse};
@@ -192,9 +197,11 @@ std::vector<Tensor> paged_attention(const Tensor& q, const Tensor& kv, const Ten
     return {out, lse};
 }
 
-std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& u, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p,
+std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits_given, const Tensor& u, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p,
                                          double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all) {
-    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1), "logits must be a CUDA tensor [rows, vocabulary], rows contiguous");
+    TORCH_CHECK(logits_given.is_cuda() && logits_given.dim() == 2, "logits must be a CUDA tensor [rows, vocabulary]");
+    const c10::cuda::CUDAGuard guard(logits_given.device());
+    const Tensor logits = logits_given.size(1) < 2 || logits_given.stride(1) == 1 ? logits_given : logits_given.contiguous();
     sg::SampleTokens p{};
     p.type = kv_type(logits, "logits");
     TORCH_CHECK(p.type != sg::kKvE4m3, "logits must be bf16, fp16 or fp32");
@@ -219,7 +226,6 @@ std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& u, 
     p.top_k_all = static_cast<int>(std::min<int64_t>(std::max<int64_t>(top_k_all, 0), V));
     p.top_p_all = static_cast<float>(top_p_all);
     p.min_p_all = static_cast<float>(min_p_all);
-    const c10::cuda::CUDAGuard guard(logits.device());
     Tensor token = torch::empty({B}, logits.options().dtype(at::kInt)), logprob = torch::empty({B}, logits.options().dtype(at::kFloat));
     if (B == 0) return {token, logprob};
     p.logits = logits.data_ptr();

@@ -34,34 +34,54 @@ __device__ __forceinline__ bool locate_token(const KvAppend& p, int b, int t, in
 }
 
 // ------------------------------------------------------------------------------------------ same type: 16-byte copies
-// Items are the 16-byte vectors of the new tokens, in the order (token, key / value, head, vector).  A block takes kThreads * kPerThread of
-// them; a thread requests all of its vectors before it stores the first.
+// A block takes kTokens tokens of one row (blockIdx.y): it looks up where they go once, in shared memory, while the first vectors are on their
+// way, then its threads copy the tokens' 16-byte vectors (key heads, then value heads of each), kPerThread in flight each.
 constexpr int kAppendThreads = 256, kAppendPerThread = 4;
 
-__global__ void __launch_bounds__(kAppendThreads) kv_append_copy_kernel(KvAppend p, int vec_per_head, int elem_bytes, int64_t items) {
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAppendThreads * kAppendPerThread) + threadIdx.x;
-    uint4 v[kAppendPerThread];
-    char* to[kAppendPerThread];
-    const int per_token = 2 * p.kv.heads * vec_per_head;
+template <int kTokens>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_copy_kernel(KvAppend p, int vec_per_head, int elem_bytes) {
+    __shared__ int64_t sh_to[kTokens];                             // byte offset of the token's first key head, or -1: not written
+    const int b = blockIdx.y, t0 = blockIdx.x * kTokens;
+    const int count = p.count ? min(p.count[b], p.T) : p.T;
+    if (t0 >= count) return;
+    const int per_token = 2 * p.kv.heads * vec_per_head, tokens = min(kTokens, count - t0), total = tokens * per_token;
+    const char* from[2];
+    int64_t h_bytes[2], t_bytes[2];
 #pragma unroll
-    for (int i = 0; i < kAppendPerThread; ++i) {
-        const int64_t item = first + i * kAppendThreads;
-        to[i] = nullptr;
-        if (item >= items) continue;
-        const int64_t token = item / per_token;
-        const int r = static_cast<int>(item - token * per_token);
-        const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
-        int page, place;
-        if (!locate_token(p, b, t, page, place)) continue;
-        const int row = r / vec_per_head, vec = r - row * vec_per_head;
-        const int which = row >= p.kv.heads, h = row - which * p.kv.heads;
-        const char* from = static_cast<const char*>(p.src[which]) + (b * p.b_stride[which] + t * p.t_stride[which] + h * p.h_stride[which]) * elem_bytes + vec * 16;
-        v[i] = *reinterpret_cast<const uint4*>(from);
-        to[i] = static_cast<char*>(p.kv.data) + (page * p.kv.page_stride + which * p.kv.kv_stride + h * p.kv.head_stride + place * p.kv.tok_stride) * elem_bytes + vec * 16;
+    for (int w = 0; w < 2; ++w) {
+        from[w] = static_cast<const char*>(p.src[w]) + (b * p.b_stride[w] + t0 * p.t_stride[w]) * elem_bytes;
+        h_bytes[w] = p.h_stride[w] * elem_bytes;
+        t_bytes[w] = p.t_stride[w] * elem_bytes;
     }
+    if (static_cast<int>(threadIdx.x) < tokens) {
+        int page, place;
+        sh_to[threadIdx.x] = locate_token(p, b, t0 + threadIdx.x, page, place) ? (page * p.kv.page_stride + place * p.kv.tok_stride) * elem_bytes : -1;
+    }
+    char* base = static_cast<char*>(p.kv.data);
+    bool located = false;
+    for (int first = threadIdx.x; first - static_cast<int>(threadIdx.x) < total; first += kAppendThreads * kAppendPerThread) {
+        uint4 v[kAppendPerThread];
+        int token[kAppendPerThread];
+        int64_t off[kAppendPerThread];
 #pragma unroll
-    for (int i = 0; i < kAppendPerThread; ++i)
-        if (to[i]) *reinterpret_cast<uint4*>(to[i]) = v[i];
+        for (int i = 0; i < kAppendPerThread; ++i) {
+            const int item = first + i * kAppendThreads;
+            token[i] = -1;
+            if (item >= total) continue;
+            token[i] = static_cast<unsigned>(item) / static_cast<unsigned>(per_token);
+            const int r = item - token[i] * per_token, row = static_cast<unsigned>(r) / static_cast<unsigned>(vec_per_head), vec = r - row * vec_per_head;
+            const int w = row >= p.kv.heads, h = row - w * p.kv.heads;
+            v[i] = *reinterpret_cast<const uint4*>(from[w] + token[i] * t_bytes[w] + h * h_bytes[w] + vec * 16);
+            off[i] = (w * p.kv.kv_stride + h * p.kv.head_stride) * elem_bytes + vec * 16;
+        }
+        if (!located) {                                            // (all threads come here the same number of times)
+            __syncthreads();
+            located = true;
+        }
+#pragma unroll
+        for (int i = 0; i < kAppendPerThread; ++i)
+            if (token[i] >= 0 && sh_to[token[i]] >= 0) *reinterpret_cast<uint4*>(base + sh_to[token[i]] + off[i]) = v[i];
+    }
 }
 
 // ------------------------------------------------------------------------------------------ to e4m3, one scale a token and head
@@ -137,9 +157,9 @@ void kv_append(const KvAppend& p, cudaStream_t s) {
     if (p.kv.type != kKvE4m3) {
         const int es = p.kv.type == kKvFp32 ? 4 : 2;
         const int vec = p.kv.dim * es / 16;
-        const int64_t items = static_cast<int64_t>(p.B) * p.T * 2 * p.kv.heads * vec;
-        const int64_t per_block = kAppendThreads * kAppendPerThread;
-        kv_append_copy_kernel<<<static_cast<unsigned>((items + per_block - 1) / per_block), kAppendThreads, 0, s>>>(p, vec, es, items);
+        // one token a block for single tokens, whose rows are what there is to spread; eight for prompts, whose look-ups they share
+        if (p.T < 8) kv_append_copy_kernel<1><<<dim3(p.T, p.B), kAppendThreads, 0, s>>>(p, vec, es);
+        else kv_append_copy_kernel<8><<<dim3((p.T + 7) / 8, p.B), kAppendThreads, 0, s>>>(p, vec, es);
     } else if (p.src_type == kKvBf16) launch_e4m3<__nv_bfloat16>(p, s);
     else if (p.src_type == kKvFp16) launch_e4m3<__half>(p, s);
     else launch_e4m3<float>(p, s);

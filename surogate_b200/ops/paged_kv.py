@@ -91,11 +91,17 @@ def paged_attention_reference(q, kv, page_table, lengths, softmax_scale=None, wi
 
 
 # ---------------------------------------------------------------------------------------------- entry points
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where its last dimension is contiguous and everything before it 16-byte aligned, else a copy that is."""
-    es = t.element_size()
-    ok = t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(st * es % 16 == 0 for st in t.stride()[:-1])
-    return t if ok or t.numel() == 0 else t.clone(memory_format=torch.contiguous_format)
+_ext = None
+
+
+def _kernels():
+    """The extension module; kept here because looking it up costs as much as a small launch."""
+    global _ext
+    if _ext is None:
+        from . import ext
+
+        _ext = ext()
+    return _ext
 
 
 def kv_append(kv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor, count: Optional[torch.Tensor] = None,
@@ -107,9 +113,7 @@ def kv_append(kv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: to
     ``t < count[b]`` (all ``T`` without ``count``).  ``page_table`` int32 ``[rows, pages of a row]``, ``start`` and ``count`` int32 ``[rows]``.
     Two tokens of one call must not have the same place."""
     if kv.is_cuda:
-        from . import ext
-
-        return ext().kv_append(kv, _rows16(k), _rows16(v), page_table, start, count, scales)
+        return _kernels().kv_append(kv, k, v, page_table, start, count, scales)
     if kv.dim() != 5 or kv.shape[1] != 2 or k.dim() != 4 or k.shape != v.shape or k.shape[2:] != (kv.shape[2], kv.shape[4]):
         raise RuntimeError("kv_append: kv must be [pages, 2, kv heads, page size, head size], k and v [rows, tokens, kv heads, head size]")
     if (scales is not None) != (kv.dtype == torch.float8_e4m3fn):
@@ -134,9 +138,7 @@ def kv_copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, scales
     ``scales [layers, pages, 2, kv heads, page size]`` with them.  ``src``, ``dst`` int32 on the cache's device.  The pairs have no order: no
     page may be a target twice, or a target and another pair's source; pairs that break this are left out and reported."""
     if kv.is_cuda:
-        from . import ext
-
-        return ext().kv_copy_pages(kv, src, dst, scales)
+        return _kernels().kv_copy_pages(kv, src, dst, scales)
     if kv.dim() != 6 or kv.shape[2] != 2:
         raise RuntimeError("kv_copy_pages: kv must be [layers, pages, 2, kv heads, page size, head size]")
     kv_copy_pages_reference(kv, src, dst, scales)
@@ -153,9 +155,7 @@ def paged_attention(q: torch.Tensor, kv: torch.Tensor, page_table: torch.Tensor,
     fp32 log-sum-exp of the scores ``[rows, query heads]`` (without the sinks).  A row of length 0 gives zeros and -inf."""
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     if kv.is_cuda:
-        from . import ext
-
-        out, lse = ext().paged_attention(_rows16(q), kv, page_table, lengths, scale, int(window), float(softcap), sinks, scales, bool(return_lse))
+        out, lse = _kernels().paged_attention(q, kv, page_table, lengths, scale, window, softcap, sinks, scales, return_lse)
     else:
         if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or q.shape[2] != kv.shape[4] or q.shape[1] % kv.shape[2] or window < 0 or softcap < 0:
             raise RuntimeError("paged_attention: kv must be [pages, 2, kv heads, page size, head size], q [rows, query heads, head size]; window and softcap not negative")

@@ -9,6 +9,8 @@ from typing import Tuple, Union
 
 import torch
 
+from .paged_kv import _kernels
+
 Number = Union[float, torch.Tensor]
 
 
@@ -74,13 +76,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Number 
     if not torch.is_tensor(temperature) and not temperature >= 0:
         raise RuntimeError("sample_tokens: the temperature must not be negative")
     if logits.is_cuda:
-        from . import ext
-
-        if logits.stride(1) != 1 and logits.shape[1] > 1:
-            logits = logits.contiguous()
-        t = [x if torch.is_tensor(x) else None for x in (temperature, top_k, top_p, min_p)]
-        n = [d if torch.is_tensor(x) else x for x, d in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0))]
-        return ext().sample_tokens(logits, u, t[0], t[1], t[2], t[3], float(n[0]), int(n[1]), float(n[2]), float(n[3]))
+        t, k, p, m = torch.is_tensor(temperature), torch.is_tensor(top_k), torch.is_tensor(top_p), torch.is_tensor(min_p)
+        return _kernels().sample_tokens(logits, u, temperature if t else None, top_k if k else None, top_p if p else None, min_p if m else None,
+                                        1.0 if t else temperature, 0 if k else top_k, 1.0 if p else top_p, 0.0 if m else min_p)
     B = logits.shape[0]
     f = lambda x: _each(x, B, torch.float32, logits.device)  # noqa: E731
     return sample_tokens_reference(logits, u, f(temperature), _each(top_k, B, torch.int32, logits.device), f(top_p), f(min_p))
