@@ -128,7 +128,10 @@ void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const
         const Tensor& t = *part[i];
         if (i) TORCH_CHECK(t.device() == kv.device() && t.dim() == 5 && t.size(0) == kv.size(0) && t.size(1) == kv.size(1), "scales must be [layers, pages, 2, kv heads, page size] on the cache's device");
         const int64_t es = t.element_size(), bytes = t.numel() ? t.numel() / (t.size(0) * t.size(1)) * es : 0;
-        TORCH_CHECK(t.numel() == 0 || t[0][0].is_contiguous(), i ? "scales" : "kv", ": each page must be contiguous");
+        int64_t inner = 1;
+        bool whole = true;
+        for (int64_t d = t.dim() - 1; d >= 2; inner *= t.size(d--)) whole = whole && (t.size(d) < 2 || t.stride(d) == inner);
+        TORCH_CHECK(t.numel() == 0 || whole, i ? "scales" : "kv", ": each page must be contiguous");
         TORCH_CHECK(bytes % 16 == 0 && aligned(t.data_ptr(), 16) && t.stride(0) * es % 16 == 0 && t.stride(1) * es % 16 == 0 && t.stride(0) >= 0 && t.stride(1) >= 0,
                     i ? "scales" : "kv", ": pages must be 16-byte aligned");
         p.base[i] = static_cast<uint8_t*>(t.data_ptr());

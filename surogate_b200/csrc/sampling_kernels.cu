@@ -69,18 +69,20 @@ struct Shared {
     double table[kTable * kCopies];
     union {
         struct { uint32_t mass_lo[kBins], mass_hi[kBins], count[kBins]; };
+        uint32_t maxima[kThreads];    // keys of the threads' largest logits
         struct { u64 list[kList], all[kList], all_q[kList]; };   // a block's candidates for a cut, and all blocks'
     };
     float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
     int own_i[kWarps * kOwn];
     u64 warp_q[kWarps];
     float warp_z[kWarps];
+    uint32_t warp_top[kWarps], warp_at[kWarps];
     int warp_n[kWarps];               // candidates of each warp
     // what other blocks of the cluster read
     u64 x_sum, x_cut, x_bins;
     float x_z;
     int x_first;                      // index of place 0
-    uint32_t x_best, x_index, x_min, x_max, x_listed, x_noted;
+    uint32_t x_best, x_index, x_kth, x_min, x_max, x_listed, x_noted;
     // the bin found, told to all blocks
     u64 b_before;
     uint32_t b_bin;
@@ -155,12 +157,17 @@ struct Row {
     __device__ __forceinline__ double log2_weight(float l) const { return l == lmax ? 0. : (static_cast<double>(l) - static_cast<double>(lmax)) * to_log2; }
     // Coarse log2 of a weight in fp32: never increases as l falls
     __device__ __forceinline__ float coarse(float l) const { return l == lmax ? 0.f : (l - lmax) * bin_scale; }
-    __device__ __forceinline__ int bin_of(float l) const { return max(0, min(kBins - 1, static_cast<int>(-coarse(l) * (kBins / kRange)))); }
+    __device__ __forceinline__ int bin_of(float l) const { return static_cast<int>(fminf(fmaxf(-coarse(l) * (kBins / kRange), 0.f), kBins - 1.f)); }
     __device__ __forceinline__ bool eligible(float l) const { return !by_min_p || log2_weight(l) >= least; }
     // A logit that surely is not above one with this log2 of its weight
     __device__ __forceinline__ float logit_below(double log2_w) const {
         const double l = static_cast<double>(lmax) + log2_w * 1.000001 / to_log2;
         return fmaxf(__double2float_rd(l - fabs(l) * 1e-6), -3.402823466e38f);        // (-inf never counts; NaN, from infinities: the lowest number)
+    }
+    // and one that surely is not below
+    __device__ __forceinline__ float logit_above(double log2_w) const {
+        const double l = static_cast<double>(lmax) + log2_w * 0.999999 / to_log2;
+        return __double2float_ru(l + fabs(l) * 1e-6);
     }
     // 2^log2_weight as multiples of 2^-44, for logits that are not below the lowest floor: t = i / 64 + r, 2^r by its series to the fourth power
     // (|r| <= 2^-7: 4e-14).  Adding 256 to it as an fp64 leaves the multiple in the lowest bits.
@@ -175,7 +182,7 @@ struct Row {
         y = fma(r, y, kLn2D * kLn2D / 2);
         y = fma(r, y, kLn2D);
         const double v = fma(e * r, y, e);
-        const double w = __hiloint2double(__double2hiint(v) + ((i >> 6) << 20), __double2loint(v));
+        const double w = __hiloint2double(__double2hiint(v) + static_cast<int>(static_cast<unsigned>(i >> 6) << 20), __double2loint(v));
         return static_cast<u64>(__double_as_longlong(w + 256.)) - 0x4070000000000000ull;
     }
     __device__ __forceinline__ u64 weight(float l) const {
@@ -230,6 +237,10 @@ struct Row {
         }
     }
     __device__ __forceinline__ u64 order(int place, float l) const { return pack(l, first + place); }
+
+    // Not below the cut, whose logit is floor_l once there is one
+    __device__ __forceinline__ bool stays(int place, float l) const { return l > floor_l || cut == 0 || order(place, l) >= cut; }
+    __device__ __forceinline__ bool kept(int place, float l) const { return eligible(l) && stays(place, l); }
 
     // Sum over the block of one number a lane (a thread's share), the warps' own sums in sh.warp_q; every thread gets the block's
     __device__ u64 block_sums(u64 v) {
@@ -454,18 +465,19 @@ struct Row {
 
     // Keeps the tokens, in the order of falling logit, before which less than `target` has come: tokens, or mass (a share of the whole).
     template <bool MASS> __device__ void find_cut(double fraction, u64 target) {
-        const u64 old = cut;
-        auto stays = [&](int i, float l) { return order(i, l) >= old; };
         clear_bins();
         each<MASS>([&](int i, float l, u64 w) {
-            if (!eligible(l) || !stays(i, l)) return;
+            if (!kept(i, l)) return;
             if (MASS) add_mass(bin_of(l), w);
             else atomicAdd(&sh.count[bin_of(l)], 1u);
         });
         if (!find_bin<MASS>(fraction, 0, target)) return;          // fewer tokens than that: all stay
         u64 base = sh.b_before;
         uint32_t bin = sh.b_bin;
-        auto in_bin = [&](int i, float l) { return bin_of(l) == static_cast<int>(bin) && eligible(l) && stays(i, l); };
+        // (What lies below the bin is out, and is not looked at any more.)
+        const float upper = bin ? logit_above(-(bin - 0.001) * (kRange / kBins)) : INFINITY;
+        auto in_bin = [&](int i, float l) { return l <= upper && bin_of(l) == static_cast<int>(bin) && kept(i, l); };
+        floor_l = fmaxf(floor_l, logit_below(-(bin + 1.001) * (kRange / kBins)));
         if (cut_in_list<MASS>(in_bin, base, target)) return;
         // a crowded bin: divide the interval of its logits' keys
         if (threadIdx.x == 0) { sh.x_min = 0xffffffffu; sh.x_max = 0; }
@@ -483,7 +495,7 @@ struct Row {
         hi = __reduce_max_sync(0xffffffffu, of_rank(&sh.x_max));
         auto within = [&](int i, float l) {
             const uint32_t k = order_key(l);
-            return k >= lo && k <= hi && eligible(l) && stays(i, l);
+            return k >= lo && k <= hi && kept(i, l);
         };
         while (lo < hi) {
             const int shift = max(0, 32 - __clz(hi - lo) - 10);
@@ -536,8 +548,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     const uint4* gx = reinterpret_cast<const uint4*>(src - row.off);
     row.x = RESIDENT ? reinterpret_cast<const uint4*>(dyn) : gx;
 
-    // the row's part, and the largest logit that the thread meets (NaN never is)
-    float best = -INFINITY;
+    const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
+    const int k = p.top_k ? p.top_k[b] : p.top_k_all;
+    const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
+    // (& and not &&: with branches here, the device compiler of CUDA 12.9 gave up the test of k on the path without top_p)
+    const bool drawing = temp > 0.f, greedy = !drawing, use_k = drawing & (k > 0) & (k < p.V), use_p = drawing & (top_p < 1.f), use_m = drawing & (min_p > 0.f);
+    const float k2e = static_cast<float>(kLog2eD);
+
+    // The row's part into shared memory, and on the way, for each thread, the largest logit that it meets (NaN never is), the vector that held it first,
+    // and the sum of e^(l - that) over its logits.
+    float best = -INFINITY, z = 0.f;
+    int best_v = 0;
     constexpr int DEPTH = 5;
     for (int base = threadIdx.x; base < row.nvec; base += kThreads * DEPTH) {
         uint4 v[DEPTH];
@@ -548,80 +569,114 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         for (int d = 0; d < DEPTH; ++d) {
             if (base + d * kThreads >= row.nvec) break;
             if (RESIDENT) reinterpret_cast<uint4*>(dyn)[base + d * kThreads] = v[d];
-            float l[N];
+            float l[N], most;
             Vec<T>::get(v[d], l);
+            most = l[0];
 #pragma unroll
-            for (int j = 0; j < N; ++j) best = fmaxf(best, l[j]);
+            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+            if (most > best) {
+                z *= ex2((best - most) * k2e);
+                best = most;
+                best_v = base + d * kThreads;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) z += l[j] == best ? 1.f : l[j] < best ? ex2((l[j] - best) * k2e) : 0.f;   // (infinities, NaN)
         }
     }
-    const float temp = p.temperature ? p.temperature[b] : p.temperature_all;
-    const int k = p.top_k ? p.top_k[b] : p.top_k_all;
-    const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
-    const bool greedy = !(temp > 0.f), use_k = !greedy && k > 0 && k < p.V, use_p = !greedy && top_p < 1.f, use_m = !greedy && min_p > 0.f;
+    if (best == -INFINITY) z = 0.f;
     if (!greedy && threadIdx.x < kTable) {
         const double e = exp2(threadIdx.x * (1. / kTable));
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) sh.table[threadIdx.x * kCopies + (i + threadIdx.x) % kCopies] = e;
     }
-    uint32_t top = __reduce_max_sync(0xffffffffu, best == -INFINITY ? 0u : order_key(best));
-    if (threadIdx.x == 0) { sh.x_best = 0; sh.x_index = 0xffffffffu; sh.x_first = row.first; }
-    row.clear_bins();
-    if (row.lane == 0) atomicMax(&sh.x_best, top);
+
+    // the block's, from its warps'
+    const uint32_t key = best == -INFINITY ? 0u : order_key(best);
+    uint32_t top = __reduce_max_sync(0xffffffffu, key), at = 0xffffffffu;
+    if (top && key == top) {                                       // the first place that holds it
+        float l[N];
+        Vec<T>::get(row.vec(best_v), l);
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j)
+            if (l[j] == best) at = static_cast<uint32_t>(row.first + best_v * N + j);
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    auto rebased = [&](float sum, uint32_t from, uint32_t to) {    // a sum of e^(l - from) as one of e^(l - to)
+        return from == to ? sum : from ? sum * ex2((key_value(from) - key_value(to)) * k2e) : 0.f;
+    };
+    z = rebased(z, key, top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    sh.maxima[threadIdx.x] = key;
+    if (row.lane == 0) { sh.warp_top[row.warp] = top; sh.warp_z[row.warp] = z; sh.warp_at[row.warp] = at; }
+    __syncthreads();
+    // The k largest logits of a row are not below the smallest of the blocks' (k / blocks)-th largest of their threads' maxima.  (Its 18 leading bits,
+    // bit by bit: what counts is how many keys are not below.)
+    const int k_each = (k + row.blocks - 1) / row.blocks;
+    const bool by_maxima = use_k && k_each <= kThreads / 4;
+    if (row.warp == 0) {
+        uint32_t kth = 0;
+        if (by_maxima) {
+            uint32_t mine[kThreads / 32];
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; ++i) mine[i] = sh.maxima[i * 32 + row.lane];
+            for (uint32_t bit = 0x80000000u; bit >= 0x4000u; bit >>= 1) {
+                uint32_t n = 0;
+#pragma unroll
+                for (int i = 0; i < kThreads / 32; ++i) n += mine[i] >= (kth | bit);
+                if (__reduce_add_sync(0xffffffffu, n) >= static_cast<uint32_t>(k_each)) kth |= bit;
+            }
+        }
+        const uint32_t of_warp = row.lane < kWarps ? sh.warp_top[row.lane] : 0;
+        top = __reduce_max_sync(0xffffffffu, of_warp);
+        z = row.lane < kWarps ? rebased(sh.warp_z[row.lane], of_warp, top) : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        at = __reduce_min_sync(0xffffffffu, row.lane < kWarps && of_warp == top ? sh.warp_at[row.lane] : 0xffffffffu);
+        if (row.lane == 0) { sh.x_best = top; sh.x_z = z; sh.x_index = at; sh.x_kth = kth; sh.x_first = row.first; }
+    }
     __syncthreads();
     row.cluster.sync();
-    top = __reduce_max_sync(0xffffffffu, row.of_rank(&sh.x_best));
-    if (top == 0) {                                                // nothing above -inf: nothing to draw
-        if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = -1; p.logprob[b] = -INFINITY; }
+    const uint32_t of_block = row.of_rank(&sh.x_best);
+    top = __reduce_max_sync(0xffffffffu, of_block);
+    z = rebased(row.of_rank(&sh.x_z), of_block, top);
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    const float log_z = logf(__shfl_sync(0xffffffffu, z, 0));
+    if (greedy || top == 0) {                                      // top == 0: nothing above -inf, nothing to draw
+        if (row.rank == 0 && row.warp == 0) {
+            at = __reduce_min_sync(0xffffffffu, of_block == top && top ? row.of_rank(&sh.x_index) : 0xffffffffu);
+            if (row.lane == 0) { p.token[b] = static_cast<int>(at); p.logprob[b] = top ? -log_z : -INFINITY; }
+        }
         row.cluster.sync();
         return;
     }
     row.lmax = key_value(top);
-    row.to_log2 = greedy ? 1. : kLog2eD / static_cast<double>(temp);
+    row.to_log2 = kLog2eD / static_cast<double>(temp);
     row.steep = !(fabs(static_cast<double>(row.lmax)) * row.to_log2 < 1e8);
     row.bin_scale = static_cast<float>(row.to_log2);
     row.by_min_p = use_m;
     row.least = use_m ? log2(static_cast<double>(fminf(min_p, 1.f))) : -kRange;
-    const float lowest = row.logit_below(-kRange);
-    row.floor_l = use_m ? row.logit_below(fmax(row.least, -static_cast<double>(kRange))) : lowest;
+    row.floor_l = row.logit_below(fmax(row.least, -static_cast<double>(kRange)));
 
-    // the sum for the log-probability, and with it what the draw, or the bound for top-p's candidates, needs
-    const bool need_mass = !greedy && !use_k, z_is_mass = need_mass && temp == 1.f && !(min_p > 0.f);
-    const float k2e = static_cast<float>(kLog2eD);
-    float z = 0.f;
+    // the mass for the draw, or for the bound of top-p's candidates
     u64 mass = 0;
-    uint32_t at = 0xffffffffu;
-    {
+    if (!use_k) {
         const int e = min(row.nvec, (row.warp + 1) * row.seg);
         for (int v = row.warp * row.seg + row.lane; v < e; v += 32) {
-            float l[N];
+            float l[N], most;
             Vec<T>::get(row.vec(v), l);
-            if (!z_is_mass) {
+            most = l[0];
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float d = l[j] == row.lmax ? 0.f : l[j] - row.lmax;      // (equal infinities)
-                    z += l[j] == l[j] ? ex2(d * k2e) : 0.f;
-                }
-            }
-            if (greedy) {
+            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+            if (!(most >= row.floor_l)) continue;
+            u64 w[N];
+            row.weights(l, row.floor_l, w);
 #pragma unroll
-                for (int j = N - 1; j >= 0; --j)
-                    if (l[j] == row.lmax) at = min(at, static_cast<uint32_t>(row.first + v * N + j));
-            }
-            if (need_mass) {
-                float most = l[0];
-#pragma unroll
-                for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
-                if (most >= row.floor_l) {
-                    u64 w[N];
-                    row.weights(l, row.floor_l, w);
-#pragma unroll
-                    for (int j = 0; j < N; ++j) mass += use_m && !row.eligible(l[j]) ? 0 : w[j];
-                }
-            }
+            for (int j = 0; j < N; ++j) mass += use_m && !row.eligible(l[j]) ? 0 : w[j];
         }
     }
-    auto kept_weight = [&](int i, float l) -> u64 { return row.eligible(l) && row.order(i, l) >= row.cut ? row.weight(l) : 0; };
-    float log_z = 0.f;
+    auto kept_weight = [&](int i, float l) -> u64 { return row.kept(i, l) ? row.weight(l) : 0; };
     auto aim = [&](u64 total) {
         const double t = static_cast<double>(u > 0.f ? u : 0.f) * static_cast<double>(total);
         return min(total - 1, static_cast<u64>(t));
@@ -630,43 +685,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         p.token[b] = row.first + i;
         p.logprob[b] = (l == row.lmax ? 0.f : l - row.lmax) - log_z;
     };
-    // the k largest logits are not below the k-th of these maxima
-    const bool by_maxima = use_k && k <= row.blocks * (kThreads / 4);
-    if (by_maxima && best >= row.floor_l) atomicAdd(&sh.count[row.bin_of(best)], 1u);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (row.lane == 0) {
-        sh.warp_z[row.warp] = z;
-        if (greedy) atomicMin(&sh.x_index, at);
-    }
-    const u64 own_mass = row.block_sums(mass);                     // (barriers of the block)
-    if (row.warp == 0) {
-        float s = row.lane < kWarps ? sh.warp_z[row.lane] : 0.f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (row.lane == 0) { sh.x_z = s; sh.x_sum = own_mass; }
-    }
-    if (by_maxima) {
-        u64 target = k;
-        if (row.template find_bin<false>(-1., 0, target)) row.floor_l = fmaxf(row.floor_l, row.logit_below(-(sh.b_bin + 1.001) * (kRange / kBins)));
+    u64 whole = 0;
+    if (use_k) {
+        if (by_maxima) {
+            const uint32_t kth = __reduce_min_sync(0xffffffffu, row.lane < row.blocks ? *row.cluster.map_shared_rank(&sh.x_kth, row.lane) : 0xffffffffu);
+            if (kth) row.floor_l = fmaxf(row.floor_l, key_value(kth));
+        }
     } else {
-        __syncthreads();
+        const u64 own_mass = row.block_sums(mass);
+        if (threadIdx.x == 0) sh.x_sum = own_mass;
         row.cluster.sync();
-    }
-    z = row.of_rank(&sh.x_z);
-    const u64 of_blocks = row.of_rank(&sh.x_sum), whole = row.sum_ranks(of_blocks);
-    if (greedy) at = __reduce_min_sync(0xffffffffu, row.lane < row.blocks ? *row.cluster.map_shared_rank(&sh.x_index, row.lane) : 0xffffffffu);
-#pragma unroll
-    for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    z = __shfl_sync(0xffffffffu, z, 0);
-    log_z = logf(z_is_mass ? static_cast<float>(static_cast<double>(whole) * (1. / (1ull << kFrac))) : z);
-    if (greedy || (!use_k && !use_p)) {
-        auto here = row.cluster.barrier_arrive();                  // nothing of this block is read by others after they have got here
-        if (!greedy) row.locate_in(kept_weight, of_blocks, own_mass, aim, found);
-        else if (row.rank == 0 && threadIdx.x == 0) { p.token[b] = static_cast<int>(at); p.logprob[b] = -log_z; }
-        row.cluster.barrier_wait(std::move(here));
-        return;
+        const u64 of_blocks = row.of_rank(&sh.x_sum);
+        whole = row.sum_ranks(of_blocks);
+        if (!use_p) {
+            auto here = row.cluster.barrier_arrive();              // nothing of this block is read by others after they have got here
+            row.locate_in(kept_weight, of_blocks, own_mass, aim, found);
+            row.cluster.barrier_wait(std::move(here));
+            return;
+        }
     }
     const double share = fmax(static_cast<double>(top_p), 0.);
     if (use_p && !use_k) {
@@ -733,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     if (use_k) row.template find_cut<false>(-1., static_cast<u64>(k));
     if (use_p) row.template find_cut<true>(use_k ? share : -1., row.share_of(share, whole));   // without top-k the share is one of the whole row
     u64 drawn = 0;
-    row.template each<true>([&](int i, float l, u64 w) { drawn += row.eligible(l) && row.order(i, l) >= row.cut ? w : 0; });
+    row.template each<true>([&](int i, float l, u64 w) { drawn += row.kept(i, l) ? w : 0; });
     row.locate(kept_weight, drawn, aim, found);
     row.cluster.sync();
 }
