@@ -40,6 +40,7 @@ constexpr int kFrac = 44;                     // weights are multiples of 2^-44
 constexpr float kRange = 46.f;                // minus log2 of the smallest weight that is looked at: what lies below is 0 as a multiple
 constexpr int kTable = 64, kCopies = 16;      // 2^(j / 64), a copy for each of 16 lanes so that none meet in a bank
 constexpr int kMost = 190 * 1024;             // bytes of a row that a block holds at most, beside 29 KB of its own
+constexpr float kLowest = -3.402823466e38f;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 
 // fp32 as an unsigned number of the same order (-0 as +0); 0 is below all that occur
@@ -69,7 +70,6 @@ struct Shared {
     double table[kTable * kCopies];
     union {
         struct { uint32_t mass_lo[kBins], mass_hi[kBins], count[kBins]; };
-        uint32_t maxima[kThreads];    // keys of the threads' largest logits
         struct { u64 list[kList], all[kList], all_q[kList]; };   // a block's candidates for a cut, and all blocks'
     };
     float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
@@ -162,7 +162,7 @@ struct Row {
     // A logit that surely is not above one with this log2 of its weight
     __device__ __forceinline__ float logit_below(double log2_w) const {
         const double l = static_cast<double>(lmax) + log2_w * 1.000001 / to_log2;
-        return fmaxf(__double2float_rd(l - fabs(l) * 1e-6), -3.402823466e38f);        // (-inf never counts; NaN, from infinities: the lowest number)
+        return fmaxf(__double2float_rd(l - fabs(l) * 1e-6), kLowest);        // (-inf never counts; NaN, from infinities: the lowest number)
     }
     // and one that surely is not below
     __device__ __forceinline__ float logit_above(double log2_w) const {
@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 
     // The row's part into shared memory, and on the way, for each thread, the largest logit that it meets (NaN never is), the vector that held it first,
     // and the sum of e^(l - that) over its logits.
-    float best = -INFINITY, z = 0.f;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = 0;
+    float best = kLowest, z = 0.f;
     int best_v = 0;
     constexpr int DEPTH = 5;
     for (int base = threadIdx.x; base < row.nvec; base += kThreads * DEPTH) {
@@ -580,10 +581,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
                 best_v = base + d * kThreads;
             }
 #pragma unroll
-            for (int j = 0; j < N; ++j) z += l[j] == best ? 1.f : l[j] < best ? ex2((l[j] - best) * k2e) : 0.f;   // (infinities, NaN)
+            for (int j = 0; j < N; ++j) z += ex2((l[j] - best) * k2e);
         }
     }
-    if (best == -INFINITY) z = 0.f;
+    if (!(z >= 0.f) || best == kLowest) {                          // NaN, or infinities among the logits, or nothing above the lowest number: once more, with care
+        z = 0.f;
+        best_v = 0x7fffffff;
+        for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
+            float l[N];
+            Vec<T>::get(row.vec(v), l);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (l[j] == best && best_v > v) best_v = v;
+                z += l[j] == best ? 1.f : l[j] < best ? ex2((l[j] - best) * k2e) : 0.f;
+            }
+        }
+    }
     if (!greedy && threadIdx.x < kTable) {
         const double e = exp2(threadIdx.x * (1. / kTable));
 #pragma unroll
@@ -591,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     }
 
     // the block's, from its warps'
-    const uint32_t key = best == -INFINITY ? 0u : order_key(best);
+    const uint32_t key = z > 0.f ? order_key(best) : 0u;           // (the largest counts 1: without one there is nothing above -inf)
     uint32_t top = __reduce_max_sync(0xffffffffu, key), at = 0xffffffffu;
     if (top && key == top) {                                       // the first place that holds it
         float l[N];
@@ -607,33 +620,39 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     z = rebased(z, key, top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    sh.maxima[threadIdx.x] = key;
     if (row.lane == 0) { sh.warp_top[row.warp] = top; sh.warp_z[row.warp] = z; sh.warp_at[row.warp] = at; }
     __syncthreads();
-    // The k largest logits of a row are not below the smallest of the blocks' (k / blocks)-th largest of their threads' maxima.  (Its 18 leading bits,
-    // bit by bit: what counts is how many keys are not below.)
+    const uint32_t of_warp = row.lane < kWarps ? sh.warp_top[row.lane] : 0;
+    top = __reduce_max_sync(0xffffffffu, of_warp);
+    row.lmax = top ? key_value(top) : 0.f;                         // the block's, for now
+    row.to_log2 = kLog2eD / static_cast<double>(temp);
+    row.bin_scale = static_cast<float>(row.to_log2);
+    // The k largest logits of a row are not below the smallest of the blocks' (k / blocks)-th largest of their threads' maxima, nor below the lower
+    // edge of a bin that holds it.
     const int k_each = (k + row.blocks - 1) / row.blocks;
-    const bool by_maxima = use_k && k_each <= kThreads / 4;
-    if (row.warp == 0) {
-        uint32_t kth = 0;
-        if (by_maxima) {
-            uint32_t mine[kThreads / 32];
-#pragma unroll
-            for (int i = 0; i < kThreads / 32; ++i) mine[i] = sh.maxima[i * 32 + row.lane];
-            for (uint32_t bit = 0x80000000u; bit >= 0x4000u; bit >>= 1) {
-                uint32_t n = 0;
-#pragma unroll
-                for (int i = 0; i < kThreads / 32; ++i) n += mine[i] >= (kth | bit);
-                if (__reduce_add_sync(0xffffffffu, n) >= static_cast<uint32_t>(k_each)) kth |= bit;
-            }
+    const bool by_maxima = use_k & (k_each <= kThreads / 4);
+    if (by_maxima) {
+        const float t = row.coarse(best);
+        if (key && t > -kRange) atomicAdd(&sh.count[row.bin_of(best)], 1u);
+        __syncthreads();
+        const uint32_t c0 = sh.count[2 * threadIdx.x], c1 = sh.count[2 * threadIdx.x + 1];
+        const uint32_t upto = static_cast<uint32_t>(warp_scan(c0 + c1, row.lane));
+        if (row.lane == 31) sh.warp_q[row.warp] = upto;
+        if (threadIdx.x == 0) sh.x_kth = 0;
+        __syncthreads();
+        uint32_t before = upto - c0 - c1;
+        for (int w = 0; w < row.warp; ++w) before += static_cast<uint32_t>(sh.warp_q[w]);
+        if (before < static_cast<uint32_t>(k_each) && static_cast<uint32_t>(k_each) <= before + c0 + c1) {
+            const int bin = 2 * threadIdx.x + (before + c0 < static_cast<uint32_t>(k_each));
+            sh.x_kth = order_key(row.logit_below(-(bin + 1.001) * (kRange / kBins)));
         }
-        const uint32_t of_warp = row.lane < kWarps ? sh.warp_top[row.lane] : 0;
-        top = __reduce_max_sync(0xffffffffu, of_warp);
+    }
+    if (row.warp == 0) {
         z = row.lane < kWarps ? rebased(sh.warp_z[row.lane], of_warp, top) : 0.f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
         at = __reduce_min_sync(0xffffffffu, row.lane < kWarps && of_warp == top ? sh.warp_at[row.lane] : 0xffffffffu);
-        if (row.lane == 0) { sh.x_best = top; sh.x_z = z; sh.x_index = at; sh.x_kth = kth; sh.x_first = row.first; }
+        if (row.lane == 0) { sh.x_best = top; sh.x_z = z; sh.x_index = at; sh.x_first = row.first; }
     }
     __syncthreads();
     row.cluster.sync();
@@ -652,9 +671,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         return;
     }
     row.lmax = key_value(top);
-    row.to_log2 = kLog2eD / static_cast<double>(temp);
     row.steep = !(fabs(static_cast<double>(row.lmax)) * row.to_log2 < 1e8);
-    row.bin_scale = static_cast<float>(row.to_log2);
     row.by_min_p = use_m;
     row.least = use_m ? log2(static_cast<double>(fminf(min_p, 1.f))) : -kRange;
     row.floor_l = row.logit_below(fmax(row.least, -static_cast<double>(kRange)));
