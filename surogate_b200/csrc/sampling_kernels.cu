@@ -136,10 +136,21 @@ struct Row {
     bool by_min_p;
     float bin_scale;
     float floor_l;                    // what is not below this is looked at
-    bool listed = false;              // the candidates have been noted down: passes run over them
+    // The candidates have been noted down: passes run over them.  Each warp's own, list_step apart.
+    bool listed = false;
+    const float* list_l;
+    const int* list_i;
+    int list_step, list_all;          // (list_all: how many, if they lie one behind the other)
+    bool alone = false;               // one block goes on with all of them, the others have left
     u64 cut = 0;                      // kept: pack() >= cut
 
     __device__ Row(Shared& s) : sh(s) {}
+
+    __device__ __forceinline__ int list_n(int w) const { return alone ? max(0, min(list_step, list_all - w * list_step)) : sh.warp_n[w]; }
+    __device__ __forceinline__ void sync() const {
+        if (alone) __syncthreads();
+        else cluster.sync();
+    }
 
     // the vector `v` in global memory: whole where all of it belongs to the row's part
     __device__ __forceinline__ uint4 from_global(const uint4* base, int v) const {
@@ -215,9 +226,10 @@ struct Row {
     // f(place, logit, weight if WEIGH) for the tokens that are not below floor_l, each warp its own in the order of their indices, lanes apart
     template <bool WEIGH, typename F> __device__ __forceinline__ void each(F f) const {
         if (listed) {
-            for (int i = lane; i < sh.warp_n[warp]; i += 32) {
-                const float l = sh.own_l[warp * kOwn + i];
-                if (l >= floor_l) f(sh.own_i[warp * kOwn + i], l, WEIGH ? weight(l) : 0);
+            const int n = list_n(warp), at = warp * list_step;
+            for (int i = lane; i < n; i += 32) {
+                const float l = list_l[at + i];
+                if (l >= floor_l) f(list_i[at + i], l, WEIGH ? weight(l) : 0);
             }
             return;
         }
@@ -269,7 +281,7 @@ struct Row {
     template <typename Q, typename A, typename F> __device__ void locate(Q q, u64 mine, A aim, F found) {
         const u64 own = block_sums(mine);
         if (threadIdx.x == 0) sh.x_sum = own;
-        cluster.sync();
+        sync();
         locate_in(q, of_rank(&sh.x_sum), own, aim, found);
     }
     // the same, with the blocks' sums known: lane r has that of block r; the warps' are in sh.warp_q
@@ -280,15 +292,15 @@ struct Row {
         target -= before;
         int w = 0;
         while (target >= sh.warp_q[w]) target -= sh.warp_q[w++];            // the warp's tokens, over the whole block
-        if (listed) {
-            const int i = threadIdx.x, place = i < kOwn ? sh.own_i[w * kOwn + i] : 0;
-            const float l = i < kOwn ? sh.own_l[w * kOwn + i] : 0.f;
-            block_find(i < sh.warp_n[w] && l >= floor_l ? q(place, l) : 0, target, [&](u64) { found(place, l); });
-            return;
-        }
-        const int a = w * seg, b = min(nvec, a + seg), per = (b - a + kThreads - 1) / kThreads, va = min(b, a + static_cast<int>(threadIdx.x) * per), vb = min(b, va + per);
+        const int a = w * seg, m = listed ? list_n(w) : min(nvec, a + seg) - a, per = (m + kThreads - 1) / kThreads;   // entries, or vectors
+        const int va = min(m, static_cast<int>(threadIdx.x) * per), vb = min(m, va + per);
         auto share = [&](auto f) {
-            for (int v = va; v < vb; ++v) {
+            if (listed) {
+                for (int v = va; v < vb; ++v)
+                    if (list_l[w * list_step + v] >= floor_l) f(list_i[w * list_step + v], list_l[w * list_step + v]);
+                return;
+            }
+            for (int v = a + va; v < a + vb; ++v) {
                 float l[N];
                 Vec<T>::get(vec(v), l);
 #pragma unroll
@@ -344,7 +356,7 @@ struct Row {
             if (lane == 0) sh.x_noted = sum;
             if (__any_sync(0xffffffffu, c > kOwn) && lane == 0) sh.x_noted = 0x10000000u;
         }
-        cluster.sync();
+        sync();
         const u64 sum = sum_ranks(of_rank(&sh.x_noted));
         total = static_cast<int>(min(sum, u64{0x10000000u}));
         return sum < 0x10000000u;
@@ -364,7 +376,7 @@ struct Row {
     // share of the whole.  False: the whole is less than the target.  Leaves the bin and what comes before it in b_*.
     template <bool MASS> __device__ bool find_bin(double fraction, u64 base, u64& target) {
         __syncthreads();
-        cluster.sync();
+        sync();
         // A block adds up its share of the bins (words of other blocks are slow to get, so each is fetched once); their sums are exchanged, and the
         // block in whose share the target falls tells the others the bin.
         constexpr int PER = kBins / kThreads;                      // (at one block a row; with more of them some threads have none)
@@ -393,7 +405,7 @@ struct Row {
             own += sh.warp_q[w];
         }
         if (threadIdx.x == 0) sh.x_bins = own;
-        cluster.sync();
+        sync();
         const u64 of_blocks = of_rank(&sh.x_bins), total = base + sum_ranks(of_blocks);
         if (fraction >= 0.) target = share_of(fraction, total);
         if (total < target) return false;                          // (the same in all blocks)
@@ -409,7 +421,7 @@ struct Row {
             }
             before += q[k];
         }
-        cluster.sync();                                            // b_* is there, and nobody reads these bins any more
+        sync();                                            // b_* is there, and nobody reads these bins any more
         return true;
     }
     // The least mass that a prefix must reach to be `fraction` of the whole
@@ -427,7 +439,7 @@ struct Row {
             if (at < kList) sh.list[at] = order(i, l);
         });
         __syncthreads();
-        cluster.sync();
+        sync();
         const uint32_t of_block = of_rank(&sh.x_listed), total = static_cast<uint32_t>(sum_ranks(of_block));
         const bool fits = total <= kList;
         if (fits) {                                                // all lists come to each block, whose warps take every blocks-th token
@@ -454,7 +466,7 @@ struct Row {
                 if (s < target && target <= s + sh.all_q[i] && lane < blocks) *cluster.map_shared_rank(&sh.x_cut, lane) = me;
             }
         }
-        cluster.sync();
+        sync();
         if (fits) set_cut(sh.x_cut);
         return fits;
     }
@@ -490,7 +502,7 @@ struct Row {
         hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) { atomicMin(&sh.x_min, lo); atomicMax(&sh.x_max, hi); }
         __syncthreads();
-        cluster.sync();
+        sync();
         lo = __reduce_min_sync(0xffffffffu, lane < blocks ? *cluster.map_shared_rank(&sh.x_min, lane) : 0xffffffffu);
         hi = __reduce_max_sync(0xffffffffu, of_rank(&sh.x_max));
         auto within = [&](int i, float l) {
@@ -523,7 +535,7 @@ struct Row {
         locate(same, mine, [&](u64) { return need - 1; }, [&](int i, float l) {
             for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&sh.x_cut, r) = order(i, l);
         });
-        cluster.sync();
+        sync();
         set_cut(sh.x_cut);
     }
 };
@@ -630,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     // The k largest logits of a row are not below the smallest of the blocks' (k / blocks)-th largest of their threads' maxima, nor below the lower
     // edge of a bin that holds it.
     const int k_each = (k + row.blocks - 1) / row.blocks;
-    const bool by_maxima = use_k & (k_each <= kThreads / 4);
+    const bool by_maxima = use_k & (k_each <= kThreads * 3 / 4);     // (then about 1.4 times as many logits are not below)
     if (by_maxima) {
         const float t = row.coarse(best);
         if (key && t > -kRange) atomicAdd(&sh.count[row.bin_of(best)], 1u);
@@ -729,36 +741,47 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     }
     int total = 0;
     const bool noted = row.note_down(total);
-    if (noted && total <= kList) {                                 // one block has them all, in the order of their indices, one a thread
-        const int i = threadIdx.x;
-        u64 me = 0;
-        if (row.rank == 0) {
-            uint32_t* upto = sh.count;                             // candidates through each warp of the cluster
-            if (row.warp == 0) {
-                constexpr int PER = kMaxCluster * kWarps / 32;
-                uint32_t c[PER], sum = 0;
+    // One block takes them all, if they fit: up to kList are ranked at once, one a thread; more go where its part of the row was, and the other
+    // blocks leave.
+    const bool at_once = noted && total <= kList, collected = noted && RESIDENT && !at_once && row.blocks > 1 && total * 8 <= slice * static_cast<int>(sizeof(T));
+    float* all_l = reinterpret_cast<float*>(dyn);
+    int* all_i = reinterpret_cast<int*>(dyn) + total;
+    u64 me = 0;
+    if ((at_once || collected) && row.rank == 0) {
+        uint32_t* upto = sh.count;                                 // candidates through each warp of the cluster
+        if (row.warp == 0) {
+            constexpr int PER = kMaxCluster * kWarps / 32;
+            uint32_t c[PER], sum = 0;
 #pragma unroll
-                for (int x = 0; x < PER; ++x) {
-                    const int w = row.lane * PER + x, r = w / kWarps;
-                    c[x] = r < row.blocks ? *row.cluster.map_shared_rank(&sh.warp_n[w % kWarps], r) : 0;
-                    sum += c[x];
-                }
-                uint32_t through = static_cast<uint32_t>(warp_scan(sum, row.lane)) - sum;
-#pragma unroll
-                for (int x = 0; x < PER; ++x) upto[row.lane * PER + x] = through += c[x];
+            for (int x = 0; x < PER; ++x) {
+                const int w = row.lane * PER + x, r = w / kWarps;
+                c[x] = r < row.blocks ? *row.cluster.map_shared_rank(&sh.warp_n[w % kWarps], r) : 0;
+                sum += c[x];
             }
-            __syncthreads();
-            if (i < total) {
-                int w = 0;                                         // the first warp through which there are more than i
+            uint32_t through = static_cast<uint32_t>(warp_scan(sum, row.lane)) - sum;
 #pragma unroll
-                for (int half = kMaxCluster * kWarps / 2; half > 0; half >>= 1)
-                    if (upto[w + half - 1] <= static_cast<uint32_t>(i)) w += half;
-                const Shared* from = row.cluster.map_shared_rank(&sh, w / kWarps);
-                const int at_i = w % kWarps * kOwn + i - static_cast<int>(w ? upto[w - 1] : 0);
-                const float l = from->own_l[at_i];
-                if (row.eligible(l)) me = pack(l, from->own_i[at_i] + from->x_first);
+            for (int x = 0; x < PER; ++x) upto[row.lane * PER + x] = through += c[x];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < total; i += kThreads) {
+            int w = 0;                                             // the first warp through which there are more than i
+#pragma unroll
+            for (int half = kMaxCluster * kWarps / 2; half > 0; half >>= 1)
+                if (upto[w + half - 1] <= static_cast<uint32_t>(i)) w += half;
+            const Shared* from = row.cluster.map_shared_rank(&sh, w / kWarps);
+            const int at_i = w % kWarps * kOwn + i - static_cast<int>(w ? upto[w - 1] : 0);
+            const float l = from->own_l[at_i];
+            const int index = from->own_i[at_i] + from->x_first;
+            if (at_once) {
+                if (row.eligible(l)) me = pack(l, index);
+            } else {
+                all_l[i] = l;
+                all_i[i] = index;
             }
         }
+    }
+    if (at_once) {
+        const int i = threadIdx.x;
         row.cluster.sync();                                        // the other blocks are done
         if (row.rank != 0) return;
         const float l = key_value(static_cast<uint32_t>(me >> 32));
@@ -783,12 +806,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         return;
     }
     row.listed = noted;
+    row.list_l = sh.own_l;
+    row.list_i = sh.own_i;
+    row.list_step = kOwn;
+    if (collected) {
+        row.cluster.sync();                                        // the other blocks are done
+        if (row.rank != 0) return;
+        row.alone = true;
+        row.blocks = 1;
+        row.first = 0;
+        row.list_l = all_l;
+        row.list_i = all_i;
+        row.list_all = total;
+        row.list_step = (total + kWarps - 1) / kWarps;
+    }
     if (use_k) row.template find_cut<false>(-1., static_cast<u64>(k));
     if (use_p) row.template find_cut<true>(use_k ? share : -1., row.share_of(share, whole));   // without top-k the share is one of the whole row
     u64 drawn = 0;
     row.template each<true>([&](int i, float l, u64 w) { drawn += row.kept(i, l) ? w : 0; });
     row.locate(kept_weight, drawn, aim, found);
-    row.cluster.sync();
+    row.sync();
 }
 
 template <typename T, bool RESIDENT>
