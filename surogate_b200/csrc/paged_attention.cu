@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
 }
 
 // Compile-time layout of one variant.
-template <int KT, int D, int ROWS> struct Shape {
+template <int KT, int D, int ROWS, bool WHOLE> struct Shape {
     static constexpr int ES = KT == kKvE4m3 ? 1 : 2;               // bytes of a cached element
     static constexpr bool BF16 = KT == kKvBf16;                    // operand type of the products: bf16, else fp16
     static constexpr int HT = ROWS / 8;                            // groups of eight query heads
@@ -106,7 +106,10 @@ template <int KT, int D, int ROWS> struct Shape {
     static constexpr int BOXES = ROWB / PITCH, BOXEL = PITCH / ES, BOXBYTES = kStep * PITCH;
     static constexpr int KBYTES = kStep * ROWB;                    // a warp's keys of one step; its values take as much
     static constexpr int STAGE = 2 * KBYTES + (KT == kKvE4m3 ? 1024 : 0);   // swizzled tiles begin on 1024 bytes
-    static constexpr int STAGES = RING_BYTES / STAGE > 8 ? 8 : RING_BYTES / STAGE < 2 ? 2 : RING_BYTES / STAGE;
+    // Blocks that share long rows keep 16 KB a warp under way, three blocks an SM; a block that has a short row for itself asks for up to four steps
+    // at once, since nothing else hides its waits.
+    static constexpr int FITS = (WHOLE ? 2 * RING_BYTES : RING_BYTES) / STAGE, MOST_STAGES = WHOLE ? 4 : 8;
+    static constexpr int STAGES = FITS > MOST_STAGES ? MOST_STAGES : FITS < 2 ? 2 : FITS;
     static constexpr int RING = STAGE * STAGES;                    // of one warp
     static constexpr int MT = D / 16;                              // tiles of 16 outputs
     static constexpr int SMEM = 1024 + kWarps * RING;
@@ -155,15 +158,18 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
         : "memory");
 }
 
-template <int KT, typename QT, int D, int ROWS>
+template <int KT, typename QT, int D, int ROWS, bool WHOLE>
 struct Piece {
-    using S = Shape<KT, D, ROWS>;
+    using S = Shape<KT, D, ROWS, WHOLE>;
     // weights are carried as 2^7 times themselves where they become fp16, whose smallest step is 2^-24; they are below 2^(kSlack) before
     static constexpr float kShift = S::BF16 ? 0.f : 7.f, kSlack = 8.f;
 
     static __device__ Ring begin(const CUtensorMap* map, uint8_t* smem, unsigned long long* bars, int* abort_flag) {
         uint8_t* at = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~uintptr_t{1023});
-        if (threadIdx.x == 0) *abort_flag = 0;
+        if (threadIdx.x == 0) {
+            *abort_flag = 0;
+            tma_prefetch_desc(map);
+        }
         if (threadIdx.x < kWarps * S::STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
         fence_barrier_init();
         __syncthreads();
@@ -545,18 +551,18 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(cons
     __shared__ float2 sh_ml[kWarps][16];
     __shared__ unsigned long long sh_bars[kWarps * 8];
     __shared__ int sh_abort;
-    Ring rg = Piece<KT, QT, D, ROWS>::begin(&map, smem, sh_bars, &sh_abort);
+    Ring rg = Piece<KT, QT, D, ROWS, true>::begin(&map, smem, sh_bars, &sh_abort);
     const int vhs = p.kv.heads * groups, b = blockIdx.x / vhs, vh = blockIdx.x - b * vhs;
     const int n = row_keys(p, b);
     const int tb = first_key(p, n) / kTile;
-    Piece<KT, QT, D, ROWS>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, rg, sh_ml);
-    Piece<KT, QT, D, ROWS>::end(p, &sh_abort);
+    Piece<KT, QT, D, ROWS, true>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, rg, sh_ml);
+    Piece<KT, QT, D, ROWS, true>::end(p, &sh_abort);
 }
 
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  A block's first and
 // last piece may be part of a row; each goes to a slot of its own.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) paged_attention_shared_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, Cut cut, int groups) {
+__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_SM)) paged_attention_shared_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, Cut cut, int groups) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float2 sh_ml[kWarps][16];
     __shared__ unsigned long long sh_bars[kWarps * 8];
@@ -604,7 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) pag
             u += k;
         }
     }
-    Ring rg = Piece<KT, QT, D, ROWS>::begin(&map, smem, sh_bars, &sh_abort);   // (a barrier of the block)
+    Ring rg = Piece<KT, QT, D, ROWS, false>::begin(&map, smem, sh_bars, &sh_abort);   // (a barrier of the block)
     int b = sh_b;
     long long rest = sh_rest, left = end - begin;                   // units into the row, units still to do
     bool first = true;
@@ -614,12 +620,13 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) pag
         const int vh = static_cast<int>(rest / tiles), t = static_cast<int>(rest - static_cast<long long>(vh) * tiles);
         const int k = static_cast<int>(min(static_cast<long long>(tiles - t), left));
         const int tb = first_key(p, n) / kTile + t;
-        Piece<KT, QT, D, ROWS>::run(p, cut, b, vh, n, tb, tb + k, groups, k == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), rg, sh_ml);
+        Piece<KT, QT, D, ROWS, false>::run(p, cut, b, vh, n, tb, tb + k, groups, k == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), rg, sh_ml);
         first = false;
         rest += k;
         left -= k;
     }
-    Piece<KT, QT, D, ROWS>::end(p, &sh_abort);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel may take its place (it waits for this one's end)
+    Piece<KT, QT, D, ROWS, false>::end(p, &sh_abort);
 }
 
 // Joins the pieces of one row and query head, and writes the outputs of empty rows.  The pieces of a row come in the order of their blocks, so
@@ -627,10 +634,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS>::PER_SM)) pag
 template <int KT, typename QT, int D, int ROWS>
 __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttention p, Cut cut, int groups) {
     __shared__ float sh_f[128];
+    asm volatile("griddepcontrol.wait;" ::: "memory");             // until all blocks of the kernel before are done and what they wrote is there
     const int G = p.Hq / p.kv.heads, b = blockIdx.y, h = blockIdx.x, kvh = h / G, vhs = p.kv.heads * groups, vh = kvh * groups + (h - kvh * G) / ROWS, row = (h - kvh * G) % ROWS;
     const long long u = cut.prefix[b], tiles = (cut.prefix[b + 1] - u) / vhs, per = cut.prefix[p.B + 1], u0 = u + vh * tiles;
     if (tiles == 0) {
-        for (int d = threadIdx.x; d < D; d += 128) Piece<KT, QT, D, ROWS>::finish(p, b, h, d, -INFINITY, 0.f, 0.f);
+        for (int d = threadIdx.x; d < D; d += 128) Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, -INFINITY, 0.f, 0.f);
         return;
     }
     const int c0 = static_cast<int>(u0 / per), c1 = static_cast<int>((u0 + tiles - 1) / per);
@@ -663,7 +671,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttentio
 #pragma unroll
     for (int k = 0; k < (D + 127) / 128; ++k) {
         const int d = k * 128 + threadIdx.x;
-        if (d < D) Piece<KT, QT, D, ROWS>::finish(p, b, h, d, mm, ll, acc[k]);
+        if (d < D) Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, mm, ll, acc[k]);
     }
 }
 
@@ -692,14 +700,15 @@ const char* page_map(CUtensorMap* map, const KvPages& kv, int box_elements, int 
 
 template <int KT, typename QT, int D, int ROWS>
 const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
-    using S = Shape<KT, D, ROWS>;
+    using S = Shape<KT, D, ROWS, false>;
+    using W = Shape<KT, D, ROWS, true>;
     static std::atomic<uint64_t> raised_whole{0}, raised_shared{0};
     CUtensorMap map;
     if (const char* e = page_map(&map, p.kv, S::BOXEL, S::PITCH)) return e;
     if (plan.whole) {
         auto k = paged_attention_whole_kernel<KT, QT, D, ROWS>;
-        if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
-        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, S::SMEM, s>>>(map, p, plan.head_groups);
+        if (!raise_smem_limit(reinterpret_cast<const void*>(k), W::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
+        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, W::SMEM, s>>>(map, p, plan.head_groups);
     } else {
         auto k = paged_attention_shared_kernel<KT, QT, D, ROWS>;
         if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_shared)) return "paged_attention: the shared-memory limit could not be raised";
@@ -711,7 +720,19 @@ const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, floa
         cut.part_o = reinterpret_cast<float*>(cut.part_ml + 2 * static_cast<int64_t>(plan.blocks) * ROWS);
         k<<<plan.blocks, kWarps * 32, S::SMEM, s>>>(map, p, cut, plan.head_groups);
         if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
-        paged_attention_join_kernel<KT, QT, D, ROWS><<<dim3(p.Hq, p.B), 128, 0, s>>>(p, cut, plan.head_groups);
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute early[1];
+        early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // launched while the kernel before runs: saves the launch's own time
+        early[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3(p.Hq, p.B);
+        cfg.blockDim = dim3(128);
+        cfg.stream = s;
+        cfg.attrs = early;
+        cfg.numAttrs = 1;
+        if (cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<KT, QT, D, ROWS>, p, cut, plan.head_groups); e != cudaSuccess) {
+            cudaGetLastError();
+            return cudaGetErrorString(e);
+        }
     }
     if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
     return nullptr;
@@ -728,9 +749,9 @@ const char* launch_dim(const PagedAttention& p, const PagedAttentionPlan& plan, 
 
 namespace {
 template <int KT> int blocks_per_sm(int dim, int rows) {
-    if (dim == 64) return rows == 16 ? Shape<KT, 64, 16>::PER_SM : Shape<KT, 64, 8>::PER_SM;
-    if (dim == 128) return rows == 16 ? Shape<KT, 128, 16>::PER_SM : Shape<KT, 128, 8>::PER_SM;
-    return Shape<KT, 256, 8>::PER_SM;
+    if (dim == 64) return rows == 16 ? Shape<KT, 64, 16, false>::PER_SM : Shape<KT, 64, 8, false>::PER_SM;
+    if (dim == 128) return rows == 16 ? Shape<KT, 128, 16, false>::PER_SM : Shape<KT, 128, 8, false>::PER_SM;
+    return Shape<KT, 256, 8, false>::PER_SM;
 }
 }  // namespace
 
