@@ -8,7 +8,7 @@
 // memory; the passes over it (maximum; sums; the candidates) stay on the chip, and the blocks exchange a few words after each.
 //
 // * The result is a token, not a number that may be a little off, so masses are integers: weights as multiples of 2^-44 of the largest one
-//   (exponentials in fp64 by a table of 2^(j/64) and four terms of the series: relative error 2^-44), whose sums do not depend on the order.
+//   (exponentials in fp64 by a table of 2^(j/64) and three terms of the series: relative error below 2^-34), whose sums do not depend on the order.
 //   A wrong token takes a u within that of a boundary.
 // * Cuts need no sort.  Bounds leave a few candidates: the k largest logits are not below the k-th of the threads' own maxima; tokens lighter
 //   than (1 - top_p) / vocabulary of the whole mass make up less than 1 - top_p together, so the cut of top-p lies above them.  Up to 512
@@ -131,7 +131,7 @@ struct Row {
     int blocks, rank, warp, lane;
     float lmax;
     double to_log2;                   // log2(e) / T
-    bool steep;                       // what is not below floor_l may still be lighter than 2^-1000: a very low temperature, or infinite logits
+    bool steep;                       // weights need care: very low or high temperatures, infinite logits
     double least;                     // log2 of the smallest weight that min-p lets stay
     bool by_min_p;
     float bin_scale;
@@ -180,22 +180,22 @@ struct Row {
         const double l = static_cast<double>(lmax) + log2_w * 0.999999 / to_log2;
         return __double2float_ru(l + fabs(l) * 1e-6);
     }
-    // 2^log2_weight as multiples of 2^-44, for logits that are not below the lowest floor: t = i / 64 + r, 2^r by its series to the fourth power
-    // (|r| <= 2^-7: 4e-14).  Adding 256 to it as an fp64 leaves the multiple in the lowest bits.
-    __device__ __forceinline__ u64 fast_weight(float l) const {
+    // 2^log2_weight as a multiple of 2^-44 plus kBias, for logits that are not below the lowest floor (whose own is 0): t = i / 64 + r, 2^r by its series
+    // to the third power (|r| <= 2^-7: 3e-11).  Adding 256 to it as an fp64 leaves the multiple in the lowest bits.
+    static constexpr u64 kBias = 0x4070000000000000ull;
+    __device__ __forceinline__ u64 biased_weight(float l) const {
         const double d = static_cast<double>(l) - static_cast<double>(lmax);
         const double big = 6755399441055744. / kTable;            // 1.5 * 2^52 / 64: adding it rounds to multiples of 1 / 64
         const double m = fma(d, to_log2, big);
         const int i = __double2loint(m);
         const double r = fma(d, to_log2, big - m);
         const double e = sh.table[(i & (kTable - 1)) * kCopies + (lane & (kCopies - 1))];
-        double y = fma(r, kLn2D * kLn2D * kLn2D * kLn2D / 24, kLn2D * kLn2D * kLn2D / 6);
-        y = fma(r, y, kLn2D * kLn2D / 2);
-        y = fma(r, y, kLn2D);
+        const double y = fma(r, fma(r, kLn2D * kLn2D * kLn2D / 6, kLn2D * kLn2D / 2), kLn2D);
         const double v = fma(e * r, y, e);
-        const double w = __hiloint2double(__double2hiint(v) + static_cast<int>(static_cast<unsigned>(i >> 6) << 20), __double2loint(v));
-        return static_cast<u64>(__double_as_longlong(w + 256.)) - 0x4070000000000000ull;
+        const double w = __hiloint2double(__double2hiint(v) + (i & -kTable) * ((1 << 20) / kTable), __double2loint(v));
+        return static_cast<u64>(__double_as_longlong(w + 256.));
     }
+    __device__ __forceinline__ u64 fast_weight(float l) const { return biased_weight(l) - kBias; }
     __device__ __forceinline__ u64 weight(float l) const {
         if (steep) {
             if (l == lmax) return 1ull << kFrac;
@@ -565,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
     // (& and not &&: with branches here, the device compiler of CUDA 12.9 gave up the test of k on the path without top_p)
     const bool drawing = temp > 0.f, greedy = !drawing, use_k = drawing & (k > 0) & (k < p.V), use_p = drawing & (top_p < 1.f), use_m = drawing & (min_p > 0.f);
+    const bool z_is_mass = drawing & (temp == 1.f) & !use_k & !use_m;   // the sum for the log-probability is the mass of all tokens
     const float k2e = static_cast<float>(kLog2eD);
 
     // The row's part into shared memory, and on the way, for each thread, the largest logit that it meets (NaN never is), the vector that held it first,
@@ -573,11 +574,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     float best = kLowest, z = 0.f;
     int best_v = 0;
     constexpr int DEPTH = 5;
-    for (int base = threadIdx.x; base < row.nvec; base += kThreads * DEPTH) {
+    for (int base = threadIdx.x; base < max(row.nvec, kTable); base += kThreads * DEPTH) {
         uint4 v[DEPTH];
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
             if (base + d * kThreads < row.nvec) v[d] = row.from_global(gx, base + d * kThreads);
+        if (base < kTable && drawing) {                            // while the first ones are on their way
+            const double e = exp2(base * (1. / kTable));
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) sh.table[base * kCopies + (i + base) % kCopies] = e;
+        }
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             if (base + d * kThreads >= row.nvec) break;
@@ -592,8 +598,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
                 best = most;
                 best_v = base + d * kThreads;
             }
+            if (!z_is_mass) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) z += ex2((l[j] - best) * k2e);
+                for (int j = 0; j < N; ++j) z += ex2((l[j] - best) * k2e);
+            }
         }
     }
     if (!(z >= 0.f) || best == kLowest) {                          // NaN, or infinities among the logits, or nothing above the lowest number: once more, with care
@@ -609,14 +617,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
             }
         }
     }
-    if (!greedy && threadIdx.x < kTable) {
-        const double e = exp2(threadIdx.x * (1. / kTable));
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) sh.table[threadIdx.x * kCopies + (i + threadIdx.x) % kCopies] = e;
-    }
-
     // the block's, from its warps'
-    const uint32_t key = z > 0.f ? order_key(best) : 0u;           // (the largest counts 1: without one there is nothing above -inf)
+    const uint32_t key = best > kLowest || z > 0.f ? order_key(best) : 0u;   // (the largest counts 1: without one there is nothing above -inf)
     uint32_t top = __reduce_max_sync(0xffffffffu, key), at = 0xffffffffu;
     if (top && key == top) {                                       // the first place that holds it
         float l[N];
@@ -673,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     z = rebased(row.of_rank(&sh.x_z), of_block, top);
 #pragma unroll
     for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    const float log_z = logf(__shfl_sync(0xffffffffu, z, 0));
+    float log_z = logf(__shfl_sync(0xffffffffu, z, 0));
     if (greedy || top == 0) {                                      // top == 0: nothing above -inf, nothing to draw
         if (row.rank == 0 && row.warp == 0) {
             at = __reduce_min_sync(0xffffffffu, of_block == top && top ? row.of_rank(&sh.x_index) : 0xffffffffu);
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         return;
     }
     row.lmax = key_value(top);
-    row.steep = !(fabs(static_cast<double>(row.lmax)) * row.to_log2 < 1e8);
+    row.steep = !(fabs(static_cast<double>(row.lmax)) * row.to_log2 < 1e8) || row.to_log2 < 1e-30;   // (what is not below the floor may be lighter than 2^-1000, or -inf heavy)
     row.by_min_p = use_m;
     row.least = use_m ? log2(static_cast<double>(fminf(min_p, 1.f))) : -kRange;
     row.floor_l = row.logit_below(fmax(row.least, -static_cast<double>(kRange)));
@@ -699,6 +701,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 #pragma unroll
             for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
             if (!(most >= row.floor_l)) continue;
+            if (!use_m && !row.steep) {                            // what lies below the floor weighs nothing, like the floor itself
+#pragma unroll
+                for (int j = 0; j < N; ++j) mass += row.biased_weight(fmaxf(l[j], row.floor_l));
+                mass -= N * row.kBias;
+                continue;
+            }
             u64 w[N];
             row.weights(l, row.floor_l, w);
 #pragma unroll
@@ -726,6 +734,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         row.cluster.sync();
         const u64 of_blocks = row.of_rank(&sh.x_sum);
         whole = row.sum_ranks(of_blocks);
+        if (z_is_mass) log_z = logf(static_cast<float>(static_cast<double>(whole) * (1. / (1ull << kFrac))));
         if (!use_p) {
             auto here = row.cluster.barrier_arrive();              // nothing of this block is read by others after they have got here
             row.locate_in(kept_weight, of_blocks, own_mass, aim, found);
