@@ -22,6 +22,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "launch_limits.h"
@@ -69,7 +70,7 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {   // inclusive
 struct Shared {
     double table[kTable * kCopies];
     union {
-        struct { uint32_t mass_lo[kBins], mass_hi[kBins], count[kBins]; };
+        struct { alignas(16) uint32_t mass[2 * kBins]; uint32_t count[kBins]; };   // (a mass: lower word, upper word)
         struct { u64 list[kList], all[kList], all_q[kList]; };   // a block's candidates for a cut, and all blocks'
     };
     float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
@@ -79,7 +80,7 @@ struct Shared {
     uint32_t warp_top[kWarps], warp_at[kWarps];
     int warp_n[kWarps];               // candidates of each warp
     // what other blocks of the cluster read
-    u64 x_sum, x_cut, x_bins;
+    u64 x_sum, x_cut, x_bins, x_heavy[2];
     float x_z;
     int x_first;                      // index of place 0
     uint32_t x_best, x_index, x_kth, x_min, x_max, x_listed, x_noted;
@@ -363,14 +364,14 @@ struct Row {
     }
 
     __device__ void clear_bins() {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = sh.mass[2 * i] = sh.mass[2 * i + 1] = 0;
         __syncthreads();
     }
     // 64-bit sums of two words each, so that a native 32-bit atomic does it
     __device__ __forceinline__ void add_mass(int bin, u64 w) {
-        const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass_lo[bin], lo);
+        const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass[2 * bin], lo);
         const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old);
-        if (hi) atomicAdd(&sh.mass_hi[bin], hi);
+        if (hi) atomicAdd(&sh.mass[2 * bin + 1], hi);
     }
     // Adds up all blocks' bins; finds the one in which the target falls (before < target <= before + bin).  With `fraction` the target is that
     // share of the whole.  False: the whole is less than the target.  Leaves the bin and what comes before it in b_*.
@@ -389,8 +390,16 @@ struct Row {
             for (int r = 0; r < kMaxCluster; ++r) {
                 if (r >= blocks) break;
                 const Shared* from = cluster.map_shared_rank(&sh, r);
-#pragma unroll
-                for (int k = 0; k < PER; ++k) q[k] += MASS ? (static_cast<u64>(from->mass_hi[bin + k]) << 32) + from->mass_lo[bin + k] : from->count[bin + k];
+                static_assert(PER == 2, "two bins are fetched at once");
+                if (MASS) {
+                    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(from->mass + 2 * bin);
+                    q[0] += two.x;
+                    q[1] += two.y;
+                } else {
+                    const uint2 two = *reinterpret_cast<const uint2*>(from->count + bin);
+                    q[0] += two.x;
+                    q[1] += two.y;
+                }
             }
 #pragma unroll
             for (int k = 0; k < PER; ++k) mine += q[k];
@@ -691,8 +700,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     row.floor_l = row.logit_below(fmax(row.least, -static_cast<double>(kRange)));
 
     // the mass for the draw, or for the bound of top-p's candidates
-    u64 mass = 0;
-    if (!use_k) {
+    // (For top-p also the mass of the tokens of at least 2^-5 and 2^-10 of the largest weight: if one of them is enough, the cut lies above.)
+    u64 mass = 0, heavy[2] = {0, 0};
+    const float heavy_l[2] = {fmaxf(row.floor_l, row.logit_below(-5.)), fmaxf(row.floor_l, row.logit_below(-10.))};
+    auto add_up = [&](auto with_heavy) {
+        constexpr bool HEAVY = decltype(with_heavy)::value;
         const int e = min(row.nvec, (row.warp + 1) * row.seg);
         for (int v = row.warp * row.seg + row.lane; v < e; v += 32) {
             float l[N], most;
@@ -701,17 +713,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 #pragma unroll
             for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
             if (!(most >= row.floor_l)) continue;
-            if (!use_m && !row.steep) {                            // what lies below the floor weighs nothing, like the floor itself
+            if (use_m || row.steep) {
+                u64 w[N];
+                row.weights(l, row.floor_l, w);
 #pragma unroll
-                for (int j = 0; j < N; ++j) mass += row.biased_weight(fmaxf(l[j], row.floor_l));
-                mass -= N * row.kBias;
+                for (int j = 0; j < N; ++j) mass += use_m && !row.eligible(l[j]) ? 0 : w[j];
                 continue;
             }
-            u64 w[N];
-            row.weights(l, row.floor_l, w);
+#pragma unroll                                                     // what lies below the floor weighs nothing, like the floor itself
+            for (int j = 0; j < N; ++j) mass += row.biased_weight(fmaxf(l[j], row.floor_l));
+            mass -= N * row.kBias;
+            if (HEAVY && most >= heavy_l[1]) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) mass += use_m && !row.eligible(l[j]) ? 0 : w[j];
+                for (int j = 0; j < N; ++j) {
+                    if (!(l[j] >= heavy_l[1])) continue;
+                    const u64 w = row.fast_weight(l[j]);
+                    heavy[1] += w;
+                    if (l[j] >= heavy_l[0]) heavy[0] += w;
+                }
+            }
         }
+    };
+    if (!use_k) {
+        if (use_p) add_up(std::true_type{});
+        else add_up(std::false_type{});
     }
     auto kept_weight = [&](int i, float l) -> u64 { return row.kept(i, l) ? row.weight(l) : 0; };
     auto aim = [&](u64 total) {
@@ -730,7 +755,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         }
     } else {
         const u64 own_mass = row.block_sums(mass);
+        if (use_p) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u64 own = row.block_sums(heavy[i]);
+                if (threadIdx.x == 0) sh.x_heavy[i] = own;
+            }
+        }
         if (threadIdx.x == 0) sh.x_sum = own_mass;
+        __syncthreads();
         row.cluster.sync();
         const u64 of_blocks = row.of_rank(&sh.x_sum);
         whole = row.sum_ranks(of_blocks);
@@ -747,6 +780,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         // (.999: their multiples of 2^-44 are rounded, each by half a multiple at most)
         const double light = (1. - share) * 0.999 * static_cast<double>(whole) / p.V;
         if (light > 1000.) row.floor_l = fmaxf(row.floor_l, row.logit_below(fmin(log2(light) - kFrac, 0.)));
+        const u64 target = row.share_of(share, whole);
+#pragma unroll
+        for (int i = 1; i >= 0; --i)
+            if (row.sum_ranks(row.of_rank(&sh.x_heavy[i])) >= target) row.floor_l = fmaxf(row.floor_l, heavy_l[i]);
     }
     int total = 0;
     const bool noted = row.note_down(total);
