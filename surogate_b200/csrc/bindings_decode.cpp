@@ -106,7 +106,7 @@ void kv_append(const Tensor& kv, const Tensor& k, const Tensor& v, const Tensor&
         p.h_stride[i] = t.stride(2);
     }
     const int64_t B = k.size(0), T = k.size(1);
-    TORCH_CHECK(B <= 65535 && T < (int64_t{1} << 30) && B * T * 2 * p.kv.heads < (int64_t{1} << 34), "k and v: at most 65535 rows, and 2^34 heads, in one call");
+    TORCH_CHECK(B <= 65535 && T < (int64_t{1} << 30) && B * T * 2 * p.kv.heads < (int64_t{1} << 33), "k and v: at most 65535 rows, and 2^33 heads of tokens, in one call");
     if (B == 0 || T == 0) return;
     table_of(table, kv, B, p.table, p.table_stride, p.table_width);
     p.start = index_ptr(start, kv, B, "start");
@@ -121,8 +121,8 @@ void kv_append(const Tensor& kv, const Tensor& k, const Tensor& v, const Tensor&
 
 void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const OptTensor& scales) {
     TORCH_CHECK(kv.is_cuda() && kv.dim() == 6 && kv.size(2) == 2, "kv must be a CUDA tensor [layers, pages, 2, kv heads, page size, head size]");
+    TORCH_CHECK(kv.scalar_type() != at::kFloat8_e4m3fn || given(scales), "the scales of a float8_e4m3fn cache are copied with its pages");
     sg::KvCopy p{};
-    const Tensor none;
     const Tensor* part[2] = {&kv, given(scales) ? &*scales : nullptr};
     for (int i = 0; i < 2 && part[i]; ++i) {
         const Tensor& t = *part[i];
@@ -155,7 +155,7 @@ void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const
 }
 
 // -> (output [B, Hq, dim], log-sum-exp fp32 [B, Hq] or undefined)
-std::tuple<Tensor, Tensor> paged_attention(const Tensor& q_given, const Tensor& kv, const Tensor& table, const Tensor& lengths, double scale, int64_t window, double softcap,
+std::tuple<Tensor, Tensor> paged_attention(const Tensor& q_given, const Tensor& kv, const Tensor& table, const Tensor& lengths, const c10::optional<double>& given_scale, int64_t window, double softcap,
                                     const OptTensor& sinks, const OptTensor& scales, bool want_lse) {
     sg::PagedAttention p{};
     p.kv = pages_of(kv, scales);
@@ -168,7 +168,8 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q_given, const Tensor& 
     TORCH_CHECK(p.kv.type == sg::kKvE4m3 ? p.q_type == sg::kKvBf16 || p.q_type == sg::kKvFp16 : p.q_type == p.kv.type, "q must have the cache's type (with an e4m3 cache: bf16 or fp16)");
     TORCH_CHECK(q.size(1) > 0 && q.size(1) <= 65535 && q.size(1) % p.kv.heads == 0, "the query heads must be a multiple of the ", num(p.kv.heads), " key heads");
     const int64_t B = q.size(0);
-    TORCH_CHECK(B <= 65535, "paged_attention: at most 65535 rows in one call");
+    TORCH_CHECK(B <= 65535 && B * q.size(1) < (int64_t{1} << 31), "paged_attention: at most 65535 rows, and 2^31 heads of them, in one call");
+    const double scale = given_scale.has_value() ? *given_scale : 1. / std::sqrt(static_cast<double>(p.kv.dim));
     TORCH_CHECK(window >= 0 && softcap >= 0 && std::isfinite(scale) && std::isfinite(softcap), "window and softcap must not be negative, scale and softcap finite");
     Tensor out = torch::empty({B, q.size(1), q.size(2)}, q.options()), lse;
     if (want_lse) lse = torch::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
@@ -209,7 +210,8 @@ std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits_given, const Tenso
     p.type = kv_type(logits, "logits");
     TORCH_CHECK(p.type != sg::kKvE4m3, "logits must be bf16, fp16 or fp32");
     const int64_t B = logits.size(0), V = logits.size(1);
-    TORCH_CHECK(V > 0 && V <= (int64_t{1} << 28) && B < (int64_t{1} << 27), "logits: an empty or too large vocabulary, or too many rows");
+    // (a million weights of at most 2^44 each: their sum fits 64 bits)
+    TORCH_CHECK(V > 0 && V < (int64_t{1} << 20) && B < (int64_t{1} << 27), "logits: the vocabulary must have 1 to 2^20 - 1 tokens, and there may be 2^27 rows");
     auto floats = [&](const OptTensor& t, const char* what) -> const float* {
         if (!given(t)) return nullptr;
         TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == B && (B < 2 || t->stride(0) == 1), what, " must be fp32 [", num(B),
@@ -249,7 +251,7 @@ void sg_register_decode(pybind11::module_& m) {
     namespace py = pybind11;
     m.def("kv_append", &kv_append, py::arg("kv"), py::arg("k"), py::arg("v"), py::arg("page_table"), py::arg("start"), py::arg("count") = OptTensor(), py::arg("scales") = OptTensor());
     m.def("kv_copy_pages", &kv_copy_pages, py::arg("kv"), py::arg("src"), py::arg("dst"), py::arg("scales") = OptTensor());
-    m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("kv"), py::arg("page_table"), py::arg("lengths"), py::arg("scale"), py::arg("window") = 0,
+    m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("kv"), py::arg("page_table"), py::arg("lengths"), py::arg("scale") = c10::optional<double>(), py::arg("window") = 0,
           py::arg("softcap") = 0.0, py::arg("sinks") = OptTensor(), py::arg("scales") = OptTensor(), py::arg("want_lse") = false);
     m.def("sample_tokens", &sample_tokens, py::arg("logits"), py::arg("u"), py::arg("temperature") = OptTensor(), py::arg("top_k") = OptTensor(), py::arg("top_p") = OptTensor(),
           py::arg("min_p") = OptTensor(), py::arg("temperature_all") = 1.0, py::arg("top_k_all") = 0, py::arg("top_p_all") = 1.0, py::arg("min_p_all") = 0.0);

@@ -54,7 +54,7 @@ def kv_append_reference(kv, k, v, page_table, start, count=None, scales=None) ->
 def kv_copy_pages_reference(kv, src, dst, scales=None) -> None:
     s, d, n = src.tolist(), dst.tolist(), kv.shape[1]
     _check_pairs(s, d, n)
-    for part in (kv, scales):
+    for part in (kv.view(torch.uint8) if kv.dtype == torch.float8_e4m3fn else kv, scales):   # (8-bit floats cannot be indexed everywhere)
         if part is not None:
             part[:, d] = part[:, s]
 
@@ -141,6 +141,8 @@ def kv_copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, scales
         return _kernels().kv_copy_pages(kv, src, dst, scales)
     if kv.dim() != 6 or kv.shape[2] != 2:
         raise RuntimeError("kv_copy_pages: kv must be [layers, pages, 2, kv heads, page size, head size]")
+    if kv.dtype == torch.float8_e4m3fn and scales is None:
+        raise RuntimeError("kv_copy_pages: the scales of a float8_e4m3fn cache are copied with its pages")
     kv_copy_pages_reference(kv, src, dst, scales)
 
 
@@ -153,15 +155,14 @@ def paged_attention(q: torch.Tensor, kv: torch.Tensor, page_table: torch.Tensor,
     ``softcap * tanh(score / softcap)``; ``sinks`` fp32 ``[query heads]``: logits that take part in the softmax's sum without a value;
     ``softmax_scale`` defaults to ``head size ** -0.5``.  Returns ``[rows, query heads, head size]`` of q's type, with ``return_lse`` also the
     fp32 log-sum-exp of the scores ``[rows, query heads]`` (without the sinks).  A row of length 0 gives zeros and -inf."""
-    scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     if kv.is_cuda:
-        out, lse = _kernels().paged_attention(q, kv, page_table, lengths, scale, window, softcap, sinks, scales, return_lse)
+        out, lse = _kernels().paged_attention(q, kv, page_table, lengths, softmax_scale, window, softcap, sinks, scales, return_lse)
     else:
         if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or q.shape[2] != kv.shape[4] or q.shape[1] % kv.shape[2] or window < 0 or softcap < 0:
             raise RuntimeError("paged_attention: kv must be [pages, 2, kv heads, page size, head size], q [rows, query heads, head size]; window and softcap not negative")
         if (scales is not None) != (kv.dtype == torch.float8_e4m3fn):
             raise RuntimeError("paged_attention: scales go with a float8_e4m3fn cache, and only with one")
-        out, lse = paged_attention_reference(q, kv, page_table, lengths, scale, int(window), float(softcap), sinks, scales)
+        out, lse = paged_attention_reference(q, kv, page_table, lengths, softmax_scale, int(window), float(softcap), sinks, scales)
     return (out, lse) if return_lse else out
 
 

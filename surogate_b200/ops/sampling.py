@@ -61,7 +61,7 @@ def _each(value: Number, B: int, dtype: torch.dtype, device) -> torch.Tensor:
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Number = 1.0, top_k: Union[int, torch.Tensor] = 0, top_p: Number = 1.0, min_p: Number = 0.0
                   ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Draw one token of each row of ``logits [rows, vocabulary]`` (fp32, bf16 or fp16) by ``u`` fp32 ``[rows]``, uniform in [0, 1).
+    """Draw one token of each row of ``logits [rows, vocabulary]`` (fp32, bf16 or fp16; at most 2^20 - 1 tokens) by ``u`` fp32 ``[rows]``, uniform in [0, 1).
 
     Weights are ``exp((logit - largest) / temperature)``.  In the order of falling logit (equal ones: rising index) tokens are kept while fewer
     than ``top_k`` come before (0: no limit), the weight is at least ``min_p``, and the mass before is below ``top_p`` of the mass that the other
@@ -71,6 +71,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Number 
 
     Returns (tokens int32, log-probabilities fp32): the latter under the softmax of the logits as they are, without temperature and filters (what
     ``Trainer.token_logprobs`` recomputes).  NaN counts as -inf; a row without a logit above -inf gives token -1 and -inf."""
+    if logits.dim() == 2 and not 0 < logits.shape[1] < 1 << 20:
+        raise RuntimeError("sample_tokens: the vocabulary must have 1 to 2^20 - 1 tokens")
     if logits.dim() != 2 or u.shape != (logits.shape[0],) or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16) or u.dtype != torch.float32:
         raise RuntimeError("sample_tokens: logits must be fp32, bf16 or fp16 [rows, vocabulary], u fp32 [rows]")
     if not torch.is_tensor(temperature) and not temperature >= 0:

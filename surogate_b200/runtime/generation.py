@@ -97,10 +97,12 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
     trainer.drain_optimizer()
     layout = cache_layout(trainer.cm, device)
     cache = None
-    if layout is not None:
-        dtype = cache_dtype or ex.options.act_dtype
-        if device.type == "cuda" and dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+    dtype = cache_dtype or ex.options.act_dtype
+    if device.type == "cuda" and dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+        if cache_dtype is not None:
             raise ValueError(f"generate: a cache of {dtype} has no attention kernel")
+        layout = None                                                  # fp32 activations on a GPU: whole passes
+    if layout is not None:
         # a prompt's pages once, and for each completion those behind the prompt's last full page
         pages = sum((len(p) + page_size - 1) // page_size + n * ((len(p) + max_new_tokens + page_size - 1) // page_size - len(p) // page_size) for p in prompts)
         cache = PagedKVCache(trainer.cm.n_layers, pages, page_size, layout[0], layout[1], len(prompts) * n, dtype=dtype, device=device)

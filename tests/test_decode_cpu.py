@@ -83,7 +83,8 @@ def test_refusals():
                  lambda: ops.kv_append(kv, k, k, table, i32(0, 63, 0)), lambda: ops.kv_append(kv, k, k, bad, i32(32, 0, 0)), lambda: ops.kv_append(kv, k, k, table, i32(0, -1, 0)),
                  lambda: ops.kv_append(kv.to(E4M3), k, k, table, i32(0, 0, 0)), lambda: ops.kv_copy_pages(kv, i32(0), i32(1)),
                  lambda: ops.kv_copy_pages(kv[None], i32(0, 1), i32(2, 2)), lambda: ops.kv_copy_pages(kv[None], i32(0, 1), i32(1, 2)), lambda: ops.kv_copy_pages(kv[None], i32(0), i32(99)),
-                 lambda: ops.kv_copy_pages(kv[None], i32(0), i32(1, 2)), lambda: ops.sample_tokens(q[0].double(), torch.zeros(4)), lambda: ops.sample_tokens(q[0], torch.zeros(3)),
+                 lambda: ops.kv_copy_pages(kv[None], i32(0), i32(1, 2)), lambda: ops.kv_copy_pages(kv[None].to(E4M3), i32(0), i32(1)),
+                 lambda: ops.sample_tokens(torch.zeros(1, 0), torch.zeros(1)), lambda: ops.sample_tokens(q[0].double(), torch.zeros(4)), lambda: ops.sample_tokens(q[0], torch.zeros(3)),
                  lambda: ops.sample_tokens(q[0], torch.zeros(4), temperature=-1.0), lambda: ops.sample_tokens(q[0], torch.zeros(4), top_k=torch.ones(4))]:
         with pytest.raises(RuntimeError):
             call()
@@ -141,6 +142,14 @@ def test_cache_books():
     assert c.free_pages == 10
     c.reserve({0: 0})
     assert c.pages(0) == [] and c.table([0]).tolist() == [[-1]]
+    q8 = PagedKVCache(1, 4, 16, 1, 8, 2, dtype=E4M3)
+    k = torch.randn(1, 3, 1, 8)
+    q8.reserve({0: 3})
+    q8.append(0, k, k, q8.table([0]), torch.zeros(1, dtype=torch.int32))
+    q8.fork(0, [1])
+    q8.reserve({1: 1})                                                     # its own copy of the page, with the scales
+    assert torch.equal(q8.kv[0, q8.pages(1)[0], :, :, :3].float(), q8.kv[0, 0, :, :, :3].float()) and torch.equal(q8.scales[0, q8.pages(1)[0]], q8.scales[0, 0])
+    assert q8.pages(1) != q8.pages(0)
     for bad in (dict(page_size=8), dict(page_size=0), dict(num_pages=0)):
         with pytest.raises(ValueError):
             PagedKVCache(**{**dict(n_layers=1, num_pages=4, page_size=16, num_kv_heads=1, head_dim=8, max_seqs=1), **bad})

@@ -384,7 +384,7 @@ def test_kv_copy_pages_reports_what_breaks_the_rules():
             want[:, b] = kv[:, a]
         _ops().kv_copy_pages(x, i32(*src), i32(*dst))
         assert _error_word() == word and torch.equal(x, want), (src, dst)
-    for args in [(kv[0], i32(0), i32(1)), (kv, i32(0), i32(1, 2)), (kv, i32(0).long(), i32(1)), (kv.transpose(2, 3), i32(0), i32(1)), (kv, i32(0).cpu(), i32(1).cpu())]:
+    for args in [(kv[0], i32(0), i32(1)), (kv, i32(0), i32(1, 2)), (kv, i32(0).long(), i32(1)), (kv.transpose(2, 3), i32(0), i32(1)), (kv, i32(0).cpu(), i32(1).cpu()), (kv.to(E4M3), i32(0), i32(1))]:
         with pytest.raises(RuntimeError):
             _ops().kv_copy_pages(*args)
     _ops().kv_copy_pages(kv, i32(), i32())
@@ -537,7 +537,7 @@ def test_sample_tokens_follows_the_distribution():
 def test_sample_tokens_refusals():
     x, u = _logits(3, 100, FP32), _uniform(3)
     for args, kw in [((x.double(), u), {}), ((x, u.double()), {}), ((x, u[:2]), {}), ((x[0], u), {}), ((x, u), dict(temperature=-1.0)), ((x, u), dict(temperature=float("nan"))),
-                     ((x, u), dict(temperature=torch.ones(2, device=DEV))), ((x, u), dict(top_k=torch.ones(3, device=DEV))), ((x, u), dict(top_p=torch.ones(3))), ((x[:, :0], u), {}),
+                     ((x, u), dict(temperature=torch.ones(2, device=DEV))), ((x, u), dict(top_k=torch.ones(3, device=DEV))), ((x, u), dict(top_p=torch.ones(3))), ((x[:, :0], u), {}), ((torch.zeros(1, 1 << 20, device=DEV), u[:1]), {}),
                      ((x, u.cpu()), {})]:
         with pytest.raises(RuntimeError):
             _ops().sample_tokens(*args, **kw)
@@ -592,6 +592,28 @@ def test_generate_agrees_with_scoring(kind):
     small = tr.generate(prompts[:2], n=2, max_new_tokens=8, temperature=0.0, cache_dtype=E4M3)
     assert all(len(c.tokens) == 8 and all(math.isfinite(x) for x in c.logprobs) for cs in small for c in cs)
     _no_errors()
+
+
+@pytest.mark.parametrize("recipe", ["fp8_hybrid", "nvfp4"])
+def test_generate_under_low_precision_recipes(recipe):
+    """Single tokens and padded prompts run through the recipes' products; the answers are tokens with finite log-probabilities."""
+    from surogate_b200.runtime.trainer import Trainer, TrainerConfig
+
+    tr = Trainer(TrainerConfig(model=_model("qwen3"), batch_size=2, seq_len=256, recipe=recipe), device=torch.device("cuda:0"))
+    tr.init_weights(seed=0)
+    outs = tr.generate([[5], list(range(140))], n=2, max_new_tokens=12, top_k=50, seed=1)
+    assert all(len(c.tokens) == 12 and all(math.isfinite(x) and x <= 0 for x in c.logprobs) for cs in outs for c in cs)
+    _no_errors()
+
+
+def test_generate_with_fp32_activations_runs_whole_passes():
+    from surogate_b200.runtime.trainer import Trainer, TrainerConfig
+
+    tr = Trainer(TrainerConfig(model=_model("qwen3"), batch_size=2, seq_len=256, param_dtype="fp32", grad_dtype="fp32", backend="ref"), device=torch.device("cuda:0"))
+    tr.init_weights(seed=0)
+    assert len(tr.generate([[5, 6]], max_new_tokens=3, temperature=0.0)[0][0].tokens) == 3
+    with pytest.raises(ValueError):
+        tr.generate([[5, 6]], cache_dtype=FP32)
 
 
 def test_decode_step_of_a_forked_group_on_one_cache():
