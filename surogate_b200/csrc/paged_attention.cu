@@ -5,7 +5,7 @@
 // Every key and value is read once for the query heads that share it: 4 * (query heads per key head) operations for each 2 or 4 bytes, so HBM
 // bounds it, and all the rest is arranged around reading without a pause.
 //
-// * A block of four warps takes tiles of 64 keys of one row and key head; a warp has 16 of them, one page at a time (a page holds a multiple of
+// * A block of four warps takes tiles of 64 keys of one row and key head (eight warps and 128 where it has the row for itself); a warp has 16 of them, one page at a time (a page holds a multiple of
 //   16 tokens).  The query heads of the key head are the rows of m16n8k16 products; warps have their own running maximum, sum and output, and
 //   meet once, at the end of the row's piece.
 // * The sums of a product may run over the head's elements in any order.  So a lane takes whole 16-byte pieces of the key rows: the piece
@@ -35,7 +35,8 @@ namespace sg {
 
 namespace {
 
-constexpr int kTile = 64, kWarps = 4, kStep = 16;   // keys a tile, warps a block, keys a warp and tile
+constexpr int kTile = 64, kStep = 16;   // keys of a tile that blocks share, keys of a warp and step
+constexpr int kSharing = 4;              // warps of a block that shares rows with others
 constexpr int RING_BYTES = 16384;   // of a warp, where two steps fit
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -54,6 +55,7 @@ __device__ __forceinline__ float lds4(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -93,7 +95,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
 }
 
 // Compile-time layout of one variant.
-template <int KT, int D, int ROWS, bool WHOLE> struct Shape {
+template <int KT, int D, int ROWS, bool DEEP> struct Shape {
     static constexpr int ES = KT == kKvE4m3 ? 1 : 2;               // bytes of a cached element
     static constexpr bool BF16 = KT == kKvBf16;                    // operand type of the products: bf16, else fp16
     static constexpr int HT = ROWS / 8;                            // groups of eight query heads
@@ -106,13 +108,14 @@ template <int KT, int D, int ROWS, bool WHOLE> struct Shape {
     static constexpr int BOXES = ROWB / PITCH, BOXEL = PITCH / ES, BOXBYTES = kStep * PITCH;
     static constexpr int KBYTES = kStep * ROWB;                    // a warp's keys of one step; its values take as much
     static constexpr int STAGE = 2 * KBYTES + (KT == kKvE4m3 ? 1024 : 0);   // swizzled tiles begin on 1024 bytes
-    // Blocks that share long rows keep 16 KB a warp under way, three blocks an SM; a block that has a short row for itself asks for up to four steps
-    // at once, since nothing else hides its waits.
-    static constexpr int FITS = (WHOLE ? 2 * RING_BYTES : RING_BYTES) / STAGE, MOST_STAGES = WHOLE ? 4 : 8;
+    // Where blocks fill the GPU, four warps have 16 KB each under way, three blocks an SM.  Where there are fewer short rows than SMs, a block has eight,
+    // each with up to three steps requested at once, since nothing else hides its waits (heads of 256: four, for their shared memory).
+    static constexpr int WARPS = DEEP && D <= 128 ? 8 : 4, TILE = WARPS * kStep;
+    static constexpr int FITS = (DEEP ? 24576 : RING_BYTES) / STAGE, MOST_STAGES = DEEP ? 3 : 8;
     static constexpr int STAGES = FITS > MOST_STAGES ? MOST_STAGES : FITS < 2 ? 2 : FITS;
     static constexpr int RING = STAGE * STAGES;                    // of one warp
     static constexpr int MT = D / 16;                              // tiles of 16 outputs
-    static constexpr int SMEM = 1024 + kWarps * RING;
+    static constexpr int SMEM = 1024 + WARPS * RING;
     static_assert(RING >= ROWS * D * 4, "a warp's ring holds its outputs when the warps meet");
     static constexpr int FIT = 230000 / (SMEM + 2048);             // blocks that an SM's shared memory holds
     static constexpr int MOST = ROWS == 8 && D <= 128 ? 3 : 2;     // of 168 registers a thread, or 255
@@ -145,7 +148,7 @@ __device__ __forceinline__ int row_keys(const PagedAttention& p, int b) {
     return n;
 }
 __device__ __forceinline__ int first_key(const PagedAttention& p, int n) { return p.window > 0 ? max(0, n - p.window) : 0; }
-__device__ __forceinline__ int row_tiles(const PagedAttention& p, int n) { return (n + kTile - 1) / kTile - first_key(p, n) / kTile; }
+template <int TILE> __device__ __forceinline__ int row_tiles(const PagedAttention& p, int n) { return (n + TILE - 1) / TILE - first_key(p, n) / TILE; }
 
 template <typename QT> __device__ __forceinline__ QT from_float(float x);
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
@@ -158,9 +161,9 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
         : "memory");
 }
 
-template <int KT, typename QT, int D, int ROWS, bool WHOLE>
+template <int KT, typename QT, int D, int ROWS, bool DEEP>
 struct Piece {
-    using S = Shape<KT, D, ROWS, WHOLE>;
+    using S = Shape<KT, D, ROWS, DEEP>;
     // weights are carried as 2^7 times themselves where they become fp16, whose smallest step is 2^-24; they are below 2^(kSlack) before
     static constexpr float kShift = S::BF16 ? 0.f : 7.f, kSlack = 8.f;
 
@@ -170,7 +173,7 @@ struct Piece {
             *abort_flag = 0;
             tma_prefetch_desc(map);
         }
-        if (threadIdx.x < kWarps * S::STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
+        if (threadIdx.x < S::WARPS * S::STAGES) mbar_init(smem_u32(bars + threadIdx.x), 1);
         fence_barrier_init();
         __syncthreads();
         return Ring{map, smem_u32(at), smem_u32(bars), reinterpret_cast<float*>(at), abort_flag, 0, 0};
@@ -204,7 +207,7 @@ struct Piece {
 
         // page of the warp's keys in step base + lane; -1: none of them counts
         auto load_pages = [&](int base) {
-            const int64_t t = static_cast<int64_t>(tb + base + lane) * kTile + warp * kStep;
+            const int64_t t = static_cast<int64_t>(tb + base + lane) * S::TILE + warp * kStep;
             if (base + lane >= steps || t >= n || t + kStep <= lo) return -1;
             int page = table[t / p.kv.page_size];
             if (page < 0 || page >= p.kv.num_pages) {
@@ -215,8 +218,8 @@ struct Piece {
         };
         int pages = load_pages(0), pages_next = load_pages(32);
         unsigned have = 0;            // bit i % 32: step i has a page
-        int next_i = 0, next_place = (tb * kTile + warp * kStep) % p.kv.page_size;   // the step that is requested next
-        const int place_step = kTile % p.kv.page_size;
+        int next_i = 0, next_place = (tb * S::TILE + warp * kStep) % p.kv.page_size;   // the step that is requested next
+        const int place_step = S::TILE % p.kv.page_size;
 
         // Request the next step into slot `to`.  A step without a page has coordinates outside the cache: zeros, and nothing is read.
         auto issue = [&](int to) {
@@ -471,8 +474,8 @@ struct Piece {
             }
         };
 
-        int t0 = tb * kTile + warp * kStep;
-        for (int i = 0; i < steps; ++i, t0 += kTile) {
+        int t0 = tb * S::TILE + warp * kStep;
+        for (int i = 0; i < steps; ++i, t0 += S::TILE) {
             if (!mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag)) break;
             const uint32_t at = ring + rg.slot * S::STAGE;
             if ((have >> (i & 31)) & 1) {
@@ -484,7 +487,7 @@ struct Piece {
             if (++rg.slot == S::STAGES) { rg.slot = 0; rg.parity ^= 1; }
         }
 
-        // the four warps meet
+        // the warps meet
 #pragma unroll
         for (int r = 0; r < S::HT; ++r)
 #pragma unroll
@@ -502,7 +505,7 @@ struct Piece {
                 const int head = 8 * r + 2 * c + h;
                 float mm = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][head].x);
+                for (int w = 0; w < S::WARPS; ++w) mm = fmaxf(mm, sh_ml[w][head].x);
                 const float f = limit[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
 #pragma unroll
                 for (int j = 0; j < S::VCH; ++j)
@@ -513,13 +516,13 @@ struct Piece {
                     }
             }
         __syncthreads();
-        for (int x = threadIdx.x; x < nrows * D; x += kWarps * 32) {
+        for (int x = threadIdx.x; x < nrows * D; x += S::WARPS * 32) {
             const int row = x / D, d = x - row * D;
             float mm = -INFINITY, ll = 0.f, acc = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_ml[w][row].x);
+            for (int w = 0; w < S::WARPS; ++w) mm = fmaxf(mm, sh_ml[w][row].x);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < S::WARPS; ++w) {
                 const float2 v = sh_ml[w][row];
                 if (v.x != -INFINITY) ll += v.y * ex2(v.x - mm);
                 acc += rg.meet[w * (ROWS * D) + x];
@@ -544,38 +547,48 @@ struct Piece {
     }
 };
 
-// One block for each row and head group.
-template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) paged_attention_whole_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, int groups) {
+// Short rows: a block takes whole ones, one row and head group after the other.
+template <int KT, typename QT, int D, int ROWS, bool DEEP>
+__global__ void __launch_bounds__((Shape<KT, D, ROWS, DEEP>::WARPS * 32), (DEEP ? 1 : Shape<KT, D, ROWS, DEEP>::PER_SM))
+paged_attention_whole_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, int groups) {
+    using S = Shape<KT, D, ROWS, DEEP>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ float2 sh_ml[kWarps][16];
-    __shared__ unsigned long long sh_bars[kWarps * 8];
+    __shared__ float2 sh_ml[S::WARPS][16];
+    __shared__ unsigned long long sh_bars[S::WARPS * 8];
     __shared__ int sh_abort;
-    Ring rg = Piece<KT, QT, D, ROWS, true>::begin(&map, smem, sh_bars, &sh_abort);
-    const int vhs = p.kv.heads * groups, b = blockIdx.x / vhs, vh = blockIdx.x - b * vhs;
-    const int n = row_keys(p, b);
-    const int tb = first_key(p, n) / kTile;
-    Piece<KT, QT, D, ROWS, true>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles(p, n), groups, -1, rg, sh_ml);
-    Piece<KT, QT, D, ROWS, true>::end(p, &sh_abort);
+    const int vhs = p.kv.heads * groups, pairs = p.B * vhs;
+    Ring rg = Piece<KT, QT, D, ROWS, DEEP>::begin(&map, smem, sh_bars, &sh_abort);
+    for (int pair = blockIdx.x; pair < pairs; pair += gridDim.x) {
+        const int b = pair / vhs, vh = pair - b * vhs;
+        // the row's page numbers and queries are on their way while its length is
+        if (static_cast<int>(threadIdx.x) * 32 < p.table_width) prefetch_l1(p.table + b * p.table_stride + threadIdx.x * 32);
+        if (threadIdx.x >= 32 && threadIdx.x < 32 + ROWS) {
+            const int G = p.Hq / p.kv.heads, kvh = vh / groups, h = min(kvh * G + (vh - kvh * groups) * ROWS + static_cast<int>(threadIdx.x) - 32, p.Hq - 1);
+            prefetch_l1(static_cast<const QT*>(p.q) + b * p.q_b_stride + h * p.q_h_stride);
+        }
+        const int n = row_keys(p, b), tb = first_key(p, n) / S::TILE;
+        Piece<KT, QT, D, ROWS, DEEP>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles<S::TILE>(p, n), groups, -1, rg, sh_ml);
+    }
+    Piece<KT, QT, D, ROWS, DEEP>::end(p, &sh_abort);
 }
 
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  A block's first and
 // last piece may be part of a row; each goes to a slot of its own.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_SM)) paged_attention_shared_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, Cut cut, int groups) {
+__global__ void __launch_bounds__(kSharing * 32, (Shape<KT, D, ROWS, false>::PER_SM)) paged_attention_shared_kernel(const __grid_constant__ CUtensorMap map, PagedAttention p, Cut cut, int groups) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ float2 sh_ml[kWarps][16];
-    __shared__ unsigned long long sh_bars[kWarps * 8];
+    __shared__ float2 sh_ml[kSharing][16];
+    __shared__ unsigned long long sh_bars[kSharing * 8];
     __shared__ int sh_abort;
-    __shared__ long long sh_sum[kWarps];
+    __shared__ long long sh_sum[kSharing];
     __shared__ int sh_b;
     __shared__ long long sh_rest;
     const int vhs = p.kv.heads * groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // units (tiles of one head group) before each row: a thread adds up its share of the rows, the block scans the sums
-    const int each = (p.B + kWarps * 32 - 1) / (kWarps * 32), r0 = min(p.B, static_cast<int>(threadIdx.x) * each), r1 = min(p.B, r0 + each);
+    const int each = (p.B + kSharing * 32 - 1) / (kSharing * 32), r0 = min(p.B, static_cast<int>(threadIdx.x) * each), r1 = min(p.B, r0 + each);
     long long mine = 0;
-    for (int b = r0; b < r1; ++b) mine += static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+    for (int b = r0; b < r1; ++b) mine += static_cast<long long>(row_tiles<kTile>(p, row_keys(p, b))) * vhs;
     long long scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -587,7 +600,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_S
     __syncthreads();
     long long before = scan - mine, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kSharing; ++w) {
         if (w < warp) before += sh_sum[w];
         total += sh_sum[w];
     }
@@ -597,7 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_S
         long long u = before;
         for (int b = r0; b < r1; ++b) {
             cut.prefix[b] = u;
-            u += static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+            u += static_cast<long long>(row_tiles<kTile>(p, row_keys(p, b))) * vhs;
         }
         if (threadIdx.x == 0) { cut.prefix[p.B] = total; cut.prefix[p.B + 1] = per; }
     }
@@ -605,7 +618,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_S
     if (begin >= before && begin < before + mine) {                 // exactly one thread
         long long u = before;
         for (int b = r0; b < r1; ++b) {
-            const long long k = static_cast<long long>(row_tiles(p, row_keys(p, b))) * vhs;
+            const long long k = static_cast<long long>(row_tiles<kTile>(p, row_keys(p, b))) * vhs;
             if (begin < u + k) { sh_b = b; sh_rest = begin - u; break; }
             u += k;
         }
@@ -615,7 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<KT, D, ROWS, false>::PER_S
     long long rest = sh_rest, left = end - begin;                   // units into the row, units still to do
     bool first = true;
     while (left > 0 && b < p.B) {
-        const int n = row_keys(p, b), tiles = row_tiles(p, n);
+        const int n = row_keys(p, b), tiles = row_tiles<kTile>(p, n);
         if (rest >= static_cast<long long>(tiles) * vhs) { ++b; rest = 0; continue; }   // an empty row, or this one is done
         const int vh = static_cast<int>(rest / tiles), t = static_cast<int>(rest - static_cast<long long>(vh) * tiles);
         const int k = static_cast<int>(min(static_cast<long long>(tiles - t), left));
@@ -702,13 +715,17 @@ template <int KT, typename QT, int D, int ROWS>
 const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
     using S = Shape<KT, D, ROWS, false>;
     using W = Shape<KT, D, ROWS, true>;
-    static std::atomic<uint64_t> raised_whole{0}, raised_shared{0};
+    static std::atomic<uint64_t> raised_deep{0}, raised_whole{0}, raised_shared{0};
     CUtensorMap map;
     if (const char* e = page_map(&map, p.kv, S::BOXEL, S::PITCH)) return e;
-    if (plan.whole) {
-        auto k = paged_attention_whole_kernel<KT, QT, D, ROWS>;
-        if (!raise_smem_limit(reinterpret_cast<const void*>(k), W::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
-        k<<<p.B * p.kv.heads * plan.head_groups, kWarps * 32, W::SMEM, s>>>(map, p, plan.head_groups);
+    if (plan.whole && plan.deep) {
+        auto k = paged_attention_whole_kernel<KT, QT, D, ROWS, true>;
+        if (!raise_smem_limit(reinterpret_cast<const void*>(k), W::SMEM, raised_deep)) return "paged_attention: the shared-memory limit could not be raised";
+        k<<<plan.blocks, W::WARPS * 32, W::SMEM, s>>>(map, p, plan.head_groups);
+    } else if (plan.whole) {
+        auto k = paged_attention_whole_kernel<KT, QT, D, ROWS, false>;
+        if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_whole)) return "paged_attention: the shared-memory limit could not be raised";
+        k<<<plan.blocks, S::WARPS * 32, S::SMEM, s>>>(map, p, plan.head_groups);
     } else {
         auto k = paged_attention_shared_kernel<KT, QT, D, ROWS>;
         if (!raise_smem_limit(reinterpret_cast<const void*>(k), S::SMEM, raised_shared)) return "paged_attention: the shared-memory limit could not be raised";
@@ -718,7 +735,7 @@ const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, floa
         cut.prefix = reinterpret_cast<long long*>(ws);
         cut.part_ml = reinterpret_cast<float2*>(ws + 2 * (static_cast<int64_t>(p.B) + 2));
         cut.part_o = reinterpret_cast<float*>(cut.part_ml + 2 * static_cast<int64_t>(plan.blocks) * ROWS);
-        k<<<plan.blocks, kWarps * 32, S::SMEM, s>>>(map, p, cut, plan.head_groups);
+        k<<<plan.blocks, kSharing * 32, S::SMEM, s>>>(map, p, cut, plan.head_groups);
         if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute early[1];
@@ -763,9 +780,12 @@ PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_
     plan.rows = G > 8 && dim <= 128 ? 16 : 8;
     plan.head_groups = (G + plan.rows - 1) / plan.rows;
     const int64_t pairs = static_cast<int64_t>(B) * Hkv * plan.head_groups, tiles = (max_keys + kTile - 1) / kTile;
-    plan.whole = tiles <= 8;
     const int most = num_sms * (kv_type == kKvE4m3 ? blocks_per_sm<kKvE4m3>(dim, plan.rows) : blocks_per_sm<kKvBf16>(dim, plan.rows));
-    plan.blocks = static_cast<int>(pairs * tiles < most ? (pairs * tiles > 0 ? pairs * tiles : 1) : most);
+    // Rows that cannot hold more than 512 keys are not split: a block takes 1.5 us for 64 of them, the kernel that joins pieces about 3.
+    plan.whole = tiles <= 8;
+    plan.deep = plan.whole && pairs <= num_sms;
+    const int64_t work = plan.whole ? pairs : pairs * tiles;
+    plan.blocks = static_cast<int>(work < most ? (work > 0 ? work : 1) : most);
     plan.workspace_floats = plan.whole ? 0 : 2 * (static_cast<int64_t>(B) + 2) + static_cast<int64_t>(plan.blocks) * 2 * plan.rows * (dim + 2);
     return plan;
 }

@@ -58,10 +58,10 @@ struct PagedAttention {
     float scale, softcap;
     int* error_flag;
 };
-// How a problem is cut: one block for each row and head (`whole`), or `blocks` blocks that share all tiles of 64 keys evenly, whose pieces a
-// second kernel joins.
+// How a problem is cut: `blocks` blocks take whole rows and heads, one after the other (`whole`; `deep`: with more warps, few rows), or share all tiles of
+// 64 keys evenly, and a second kernel joins the pieces.
 struct PagedAttentionPlan {
-    bool whole;
+    bool whole, deep;
     int rows, blocks, head_groups;
     int64_t workspace_floats;
 };
