@@ -119,9 +119,20 @@ def test_paged_attention_lengths(dtype, P):
     lengths = [0, 1, 15, 16, 17, 63, 64, 65, 0, 127, 128, 129, 255, 256, 300, 2, 0]
     q, kv, table, n, s = _problem(len(lengths), 4, 2, 64, P, lengths, dtype, seed=P)
     _check_attention(q, kv, table, n, scales=s)
-    lengths = [0, 1, 4097, 0, 513, 6000, 33, 0]
+    lengths = [0, 1, 4097, 0, 513, 6000, 33, 0]                          # (rows that may be longer than 1024 keys are split)
     q, kv, table, n, s = _problem(len(lengths), 8, 2, 128, P, lengths, dtype, seed=P + 1)
     _check_attention(q, kv, table, n, scales=s)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 32, 2), (256, 4, 1)])
+@pytest.mark.parametrize("B", [1, 3, 180])
+@pytest.mark.parametrize("capacity", [16, 1024, 1040])
+def test_paged_attention_short_rows(B, D, Hq, Hkv, capacity):
+    """Few and many short rows, on both sides of the capacity up to which rows stay whole, with and without a window."""
+    lengths = [(i * 37) % (capacity + 1) if i else capacity for i in range(B)]
+    q, kv, table, n, s = _problem(B, Hq, Hkv, D, 16, lengths, BF16, seed=B, width=capacity // 16)
+    _check_attention(q, kv, table, n)
+    _check_attention(q, kv, table, n, window=70)
 
 
 @pytest.mark.parametrize("B,Hkv", [(1, 1), (1, 8), (2, 3), (300, 2), (1000, 1)])
