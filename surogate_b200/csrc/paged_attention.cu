@@ -118,7 +118,7 @@ template <int KT, int D, int ROWS, bool DEEP> struct Shape {
     static constexpr int SMEM = 1024 + WARPS * RING;
     static_assert(RING >= ROWS * D * 4, "a warp's ring holds its outputs when the warps meet");
     static constexpr int FIT = 230000 / (SMEM + 2048);             // blocks that an SM's shared memory holds
-    static constexpr int MOST = ROWS == 8 && D <= 128 ? 3 : 2;     // of 168 registers a thread, or 255
+    static constexpr int MOST = D <= 128 ? 3 : 2;     // of 168 registers a thread, or 255
     static constexpr int PER_SM = FIT < MOST ? FIT : MOST;
 };
 
@@ -183,7 +183,8 @@ struct Piece {
     }
 
     // Tiles [tb, te) of row b (tile numbers of the row's positions) and head group vh.  slot < 0: the whole row; its result is written.  Else the piece is.
-    static __device__ void run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, Ring& rg, float2 (*sh_ml)[16]) {
+    // False (for the whole block) when a wait gave up: the block must stop.
+    static __device__ bool run(const PagedAttention& p, const Cut& cut, int b, int vh, int n, int tb, int te, int groups, int slot, Ring& rg, float2 (*sh_ml)[16]) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         const int G = p.Hq / p.kv.heads, kvh = vh / groups, h0 = kvh * G + (vh - kvh * groups) * ROWS, nrows = min(ROWS, kvh * G + G - h0);
         const int lo = first_key(p, n), steps = te - tb;
@@ -475,8 +476,9 @@ struct Piece {
         };
 
         int t0 = tb * S::TILE + warp * kStep;
-        for (int i = 0; i < steps; ++i, t0 += S::TILE) {
-            if (!mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag)) break;
+        int i = 0;
+        for (; i < steps; ++i, t0 += S::TILE) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag))) break;   // a wait that gave up
             const uint32_t at = ring + rg.slot * S::STAGE;
             if ((have >> (i & 31)) & 1) {
                 if (t0 >= lo && t0 + kStep <= n) compute(std::true_type{}, at, t0);
@@ -484,6 +486,13 @@ struct Piece {
             }
             __syncwarp();                                          // every lane has read the slot
             if (next_i < steps) issue(rg.slot);
+            if (++rg.slot == S::STAGES) { rg.slot = 0; rg.parity ^= 1; }
+        }
+
+        const bool gave_up = i < steps;
+        for (; i < next_i; ++i) {                                  // only then: what this warp asked for, with a limit again
+            int never = 0;
+            mbar_wait(bars + rg.slot * 8, rg.parity, &never);
             if (++rg.slot == S::STAGES) { rg.slot = 0; rg.parity ^= 1; }
         }
 
@@ -535,7 +544,7 @@ struct Piece {
             }
         }
         fence_proxy_async();                                       // the rings are written by copies again
-        __syncthreads();
+        return __syncthreads_or(gave_up) == 0;
     }
 
     static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float acc) {
@@ -567,14 +576,15 @@ paged_attention_whole_kernel(const __grid_constant__ CUtensorMap map, PagedAtten
             prefetch_l1(static_cast<const QT*>(p.q) + b * p.q_b_stride + h * p.q_h_stride);
         }
         const int n = row_keys(p, b), tb = first_key(p, n) / S::TILE;
-        Piece<KT, QT, D, ROWS, DEEP>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles<S::TILE>(p, n), groups, -1, rg, sh_ml);
+        if (!Piece<KT, QT, D, ROWS, DEEP>::run(p, Cut{}, b, vh, n, tb, tb + row_tiles<S::TILE>(p, n), groups, -1, rg, sh_ml)) break;
     }
     Piece<KT, QT, D, ROWS, DEEP>::end(p, &sh_abort);
 }
 
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  Each row and head group
 // counts kStart tiles more than it has (at its beginning), for what a block spends on starting and ending one; without, blocks with many short rows
-// end late (64 rows of 100 to 4096 keys, 32/8 heads of 128: bf16 103.1 us without, 100.5 with; e4m3 81.5 and 75.5).  A block's first and last piece may be part of a row; each goes to a slot of its own.
+// end late (64 rows of 100 to 4096 keys, 32/8 heads of 128: bf16 103.1 us without, 100.5 with; e4m3 81.5 and 75.5).
+// A block's first and last piece may be part of a row; each goes to a slot of its own.
 constexpr int kStart = 1;
 __device__ __forceinline__ long long row_units(const PagedAttention& p, int b, int vhs) {
     const int tiles = row_tiles<kTile>(p, row_keys(p, b));
@@ -640,7 +650,8 @@ __global__ void __launch_bounds__(kSharing * 32, (Shape<KT, D, ROWS, false>::PER
         const int k = static_cast<int>(min(static_cast<long long>(units - u), left)), t = max(0, u - kStart), m = u + k - kStart - t;   // tiles [t, t + m)
         if (m > 0) {
             const int tb = first_key(p, n) / kTile + t;
-            Piece<KT, QT, D, ROWS, false>::run(p, cut, b, vh, n, tb, tb + m, groups, m == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1), rg, sh_ml);
+            const int slot = m == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (first ? 0 : 1);
+            if (!Piece<KT, QT, D, ROWS, false>::run(p, cut, b, vh, n, tb, tb + m, groups, slot, rg, sh_ml)) break;
             first = false;
         }
         rest += k;
