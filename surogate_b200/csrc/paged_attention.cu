@@ -525,19 +525,21 @@ struct Piece {
                     }
             }
         __syncthreads();
-        for (int x = threadIdx.x; x < nrows * D; x += S::WARPS * 32) {
+        for (int x = threadIdx.x * 4; x < nrows * D; x += S::WARPS * 128) {
             const int row = x / D, d = x - row * D;
-            float mm = -INFINITY, ll = 0.f, acc = 0.f;
+            float mm = -INFINITY, ll = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < S::WARPS; ++w) mm = fmaxf(mm, sh_ml[w][row].x);
 #pragma unroll
             for (int w = 0; w < S::WARPS; ++w) {
                 const float2 v = sh_ml[w][row];
+                const float4 a = *reinterpret_cast<const float4*>(rg.meet + w * (ROWS * D) + x);
                 if (v.x != -INFINITY) ll += v.y * ex2(v.x - mm);
-                acc += rg.meet[w * (ROWS * D) + x];
+                acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
             }
             if (slot >= 0) {
-                cut.part_o[(static_cast<int64_t>(slot) * ROWS + row) * D + d] = acc;
+                *reinterpret_cast<float4*>(cut.part_o + (static_cast<int64_t>(slot) * ROWS + row) * D + d) = acc;
                 if (d == 0) cut.part_ml[slot * ROWS + row] = make_float2(mm, ll);
             } else {
                 finish(p, b, h0 + row, d, mm, ll, acc);
@@ -547,12 +549,19 @@ struct Piece {
         return __syncthreads_or(gave_up) == 0;
     }
 
-    static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float acc) {
+    // elements d to d + 3 of one output
+    static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float4 acc) {
+        const int64_t at = static_cast<int64_t>(b) * p.Hq + h;
         float total = ll;
         if (p.sinks) total += ex2(p.sinks[h] * kLog2e - mm);       // infinite where the sink outweighs all keys by 2^128: the output is 0
-        const float y = mm == -INFINITY ? 0.f : acc * (S::BF16 ? 1.f : 0x1p-7f) / total;
-        static_cast<QT*>(p.out)[(static_cast<int64_t>(b) * p.Hq + h) * D + d] = from_float<QT>(y);
-        if (d == 0 && p.lse) p.lse[static_cast<int64_t>(b) * p.Hq + h] = mm == -INFINITY ? -INFINITY : mm * kLn2 + logf(ll);
+        const float f = S::BF16 ? 1.f : 0x1p-7f;
+        QT y[4];
+        y[0] = from_float<QT>(mm == -INFINITY ? 0.f : acc.x * f / total);
+        y[1] = from_float<QT>(mm == -INFINITY ? 0.f : acc.y * f / total);
+        y[2] = from_float<QT>(mm == -INFINITY ? 0.f : acc.z * f / total);
+        y[3] = from_float<QT>(mm == -INFINITY ? 0.f : acc.w * f / total);
+        *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + at * D + d) = *reinterpret_cast<const uint2*>(y);
+        if (d == 0 && p.lse) p.lse[at] = mm == -INFINITY ? -INFINITY : mm * kLn2 + logf(ll);
     }
 };
 
@@ -582,10 +591,11 @@ paged_attention_whole_kernel(const __grid_constant__ CUtensorMap map, PagedAtten
 }
 
 // All tiles of all rows and head groups, in that order, shared evenly by the blocks: nothing on the host knows the lengths.  Each row and head group
-// counts kStart tiles more than it has (at its beginning), for what a block spends on starting and ending one; without, blocks with many short rows
-// end late (64 rows of 100 to 4096 keys, 32/8 heads of 128: bf16 103.1 us without, 100.5 with; e4m3 81.5 and 75.5).
+// counts kStart tiles more than it has (at its beginning), for the instructions that a block spends on starting and ending a piece; without, blocks
+// with many short rows end late.  64 rows of 100 to 4096 keys, 32 over 8 heads of 128, with 0 / 1 / 2 / 4 / 6 (before the ends were made shorter):
+// bf16 103 / 101 / 100 / 98 / 99 us, e4m3 82 / 76 / 66 / 61 / 60; 128 over 8 heads, bf16 - / 147 / 136 / 123 / 120.  Rows of one length gain 1 to 2 %.
 // A block's first and last piece may be part of a row; each goes to a slot of its own.
-constexpr int kStart = 1;
+constexpr int kStart = 4;
 __device__ __forceinline__ long long row_units(const PagedAttention& p, int b, int vhs) {
     const int tiles = row_tiles<kTile>(p, row_keys(p, b));
     return tiles ? static_cast<long long>(tiles + kStart) * vhs : 0;
@@ -664,13 +674,14 @@ __global__ void __launch_bounds__(kSharing * 32, (Shape<KT, D, ROWS, false>::PER
 // Joins the pieces of one row and query head, and writes the outputs of empty rows.  The pieces of a row come in the order of their blocks, so
 // the sums do not depend on which block ended first.
 template <int KT, typename QT, int D, int ROWS>
-__global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttention p, Cut cut, int groups) {
-    __shared__ float sh_f[128];
+__global__ void __launch_bounds__(D / 4) paged_attention_join_kernel(PagedAttention p, Cut cut, int groups) {
+    __shared__ float sh_f[D / 4];
+    const int d = 4 * threadIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");             // until all blocks of the kernel before are done and what they wrote is there
     const int G = p.Hq / p.kv.heads, b = blockIdx.y, h = blockIdx.x, kvh = h / G, vhs = p.kv.heads * groups, vh = kvh * groups + (h - kvh * G) / ROWS, row = (h - kvh * G) % ROWS;
     const long long u = cut.prefix[b], units = (cut.prefix[b + 1] - u) / vhs, per = cut.prefix[p.B + 1], u0 = u + vh * units;
     if (units == 0) {
-        for (int d = threadIdx.x; d < D; d += 128) Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, -INFINITY, 0.f, 0.f);
+        Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, -INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f));
         return;
     }
     const int c0 = static_cast<int>((u0 + kStart) / per), c1 = static_cast<int>((u0 + units - 1) / per);   // blocks of its first and last tile
@@ -678,10 +689,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttentio
     auto slot = [&](int c) { return static_cast<int64_t>(2 * c + (c == c0 && c0 * per < u0 ? 1 : 0)); };
     float mm = -INFINITY, ll = 0.f;
     for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, cut.part_ml[slot(c) * ROWS + row].x);
-    float acc[(D + 127) / 128];
-#pragma unroll
-    for (int k = 0; k < (D + 127) / 128; ++k) acc[k] = 0.f;
-    for (int base = c0; base <= c1; base += 128) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = c0; base <= c1; base += D / 4) {
         __syncthreads();
         const int c = base + threadIdx.x;
         if (c <= c1) {
@@ -689,22 +698,15 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(PagedAttentio
             sh_f[threadIdx.x] = v.x == -INFINITY ? 0.f : ex2(v.x - mm);
         }
         __syncthreads();
-        const int cnt = min(128, c1 + 1 - base);
+        const int cnt = min(D / 4, c1 + 1 - base);
         for (int i = 0; i < cnt; ++i) {
             const float f = sh_f[i];
+            const float4 o = *reinterpret_cast<const float4*>(cut.part_o + (slot(base + i) * ROWS + row) * D + d);
             ll += f * cut.part_ml[slot(base + i) * ROWS + row].y;
-#pragma unroll
-            for (int k = 0; k < (D + 127) / 128; ++k) {
-                const int d = k * 128 + threadIdx.x;
-                if (d < D) acc[k] += f * cut.part_o[(slot(base + i) * ROWS + row) * D + d];
-            }
+            acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
         }
     }
-#pragma unroll
-    for (int k = 0; k < (D + 127) / 128; ++k) {
-        const int d = k * 128 + threadIdx.x;
-        if (d < D) Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, mm, ll, acc[k]);
-    }
+    Piece<KT, QT, D, ROWS, false>::finish(p, b, h, d, mm, ll, acc);
 }
 
 // The pages as a tensor of five dimensions (element, place, head, key / value, page), copied in boxes of 16 places.  Strides may come in any order.
@@ -730,6 +732,8 @@ const char* page_map(CUtensorMap* map, const KvPages& kv, int box_elements, int 
     return r == CUDA_SUCCESS ? nullptr : "paged_attention: the cache's strides do not make a tensor map";
 }
 
+int64_t prefix_floats(int B) { return 4 * ((static_cast<int64_t>(B) + 3) / 2); }   // of Cut::prefix; what follows starts on 16 bytes
+
 template <int KT, typename QT, int D, int ROWS>
 const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, float* ws, cudaStream_t s) {
     using S = Shape<KT, D, ROWS, false>;
@@ -752,7 +756,7 @@ const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, floa
         cut.blocks = plan.blocks;
         cut.min_units = 4;
         cut.prefix = reinterpret_cast<long long*>(ws);
-        cut.part_ml = reinterpret_cast<float2*>(ws + 2 * (static_cast<int64_t>(p.B) + 2));
+        cut.part_ml = reinterpret_cast<float2*>(ws + prefix_floats(p.B));
         cut.part_o = reinterpret_cast<float*>(cut.part_ml + 2 * static_cast<int64_t>(plan.blocks) * ROWS);
         k<<<plan.blocks, kSharing * 32, S::SMEM, s>>>(map, p, cut, plan.head_groups);
         if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cudaGetErrorString(e);
@@ -761,7 +765,7 @@ const char* launch(const PagedAttention& p, const PagedAttentionPlan& plan, floa
         early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // launched while the kernel before runs: saves the launch's own time
         early[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.gridDim = dim3(p.Hq, p.B);
-        cfg.blockDim = dim3(128);
+        cfg.blockDim = dim3(D / 4);
         cfg.stream = s;
         cfg.attrs = early;
         cfg.numAttrs = 1;
@@ -807,7 +811,7 @@ PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_
     plan.deep = plan.whole && pairs <= num_sms;
     const int64_t work = plan.whole ? pairs : pairs * tiles;
     plan.blocks = static_cast<int>(work < most ? (work > 0 ? work : 1) : most);
-    plan.workspace_floats = plan.whole ? 0 : 2 * (static_cast<int64_t>(B) + 2) + static_cast<int64_t>(plan.blocks) * 2 * plan.rows * (dim + 2);
+    plan.workspace_floats = plan.whole ? 0 : prefix_floats(B) + static_cast<int64_t>(plan.blocks) * 2 * plan.rows * (dim + 2);
     return plan;
 }
 
