@@ -40,7 +40,7 @@ constexpr int kOwn = 64;                      // candidates a warp can note down
 constexpr int kFrac = 44;                     // weights are multiples of 2^-44
 constexpr float kRange = 46.f;                // minus log2 of the smallest weight that is looked at: what lies below is 0 as a multiple
 constexpr int kTable = 64, kCopies = 16;      // 2^(j / 64), a copy for each of 16 lanes so that none meet in a bank
-constexpr int kMost = 190 * 1024;             // bytes of a row that a block holds at most, beside 29 KB of its own
+constexpr int kMost = 190 * 1024;             // bytes of a row that a block holds at most, beside 34 KB of its own
 constexpr float kLowest = -3.402823466e38f;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 
@@ -72,6 +72,7 @@ struct Shared {
     union {
         struct { alignas(16) uint32_t mass[2 * kBins]; uint32_t count[kBins]; };   // (a mass: lower word, upper word)
         struct { u64 list[kList], all[kList], all_q[kList]; };   // a block's candidates for a cut, and all blocks'
+        alignas(16) uint32_t estimate[4 * kBins];
     };
     float own_l[kWarps * kOwn];       // the warps' candidates: logit, place
     int own_i[kWarps * kOwn];
@@ -80,13 +81,13 @@ struct Shared {
     uint32_t warp_top[kWarps], warp_at[kWarps];
     int warp_n[kWarps];               // candidates of each warp
     // what other blocks of the cluster read
-    u64 x_sum, x_cut, x_bins, x_heavy[2];
+    u64 x_sum, x_cut, x_bins, x_above;
     float x_z;
     int x_first;                      // index of place 0
     uint32_t x_best, x_index, x_kth, x_min, x_max, x_listed, x_noted;
     // the bin found, told to all blocks
     u64 b_before;
-    uint32_t b_bin;
+    uint32_t b_bin, b_last;
 };
 
 // 16 bytes of logits as fp32
@@ -449,6 +450,10 @@ struct Row {
         });
         __syncthreads();
         sync();
+        return rank_lists<MASS>(base, target);
+    }
+    // the same with the tokens in the blocks' lists (and known to be there)
+    template <bool MASS> __device__ bool rank_lists(u64 base, u64 target) {
         const uint32_t of_block = of_rank(&sh.x_listed), total = static_cast<uint32_t>(sum_ranks(of_block));
         const bool fits = total <= kList;
         if (fits) {                                                // all lists come to each block, whose warps take every blocks-th token
@@ -478,6 +483,142 @@ struct Row {
         sync();
         if (fits) set_cut(sh.x_cut);
         return fits;
+    }
+
+    // The cut of top-p where it is thought to be: lists the tokens in [lower, upper], and adds up exactly what lies above and the whole.  Which proves the
+    // cut, or refuses it (not there, or too many tokens: false; the whole is known then, and nothing else).  `above`: this lane's part of its
+    // warp's kept mass.
+    __device__ bool proved_cut(double share, float lower, float upper, u64& above, u64& whole) {
+        u64 mass = 0;
+        above = 0;
+        __syncthreads();
+        if (threadIdx.x == 0) { sh.x_listed = 0; sh.x_cut = 0; }
+        __syncthreads();
+        const int e = min(nvec, (warp + 1) * seg);
+        for (int v = warp * seg + lane; v < e; v += 32) {
+            float l[N], most;
+            Vec<T>::get(vec(v), l);
+            most = l[0];
+#pragma unroll
+            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+            if (!(most >= floor_l)) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const u64 w = fast_weight(fmaxf(l[j], floor_l));
+                mass += w;
+                if (l[j] > upper) above += w;
+            }
+            if (!(most >= lower)) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (l[j] >= lower && l[j] <= upper) {
+                    const uint32_t at = atomicAdd(&sh.x_listed, 1u);
+                    if (at < kList) sh.list[at] = order(v * N + j, l[j]);
+                }
+        }
+        const u64 own_mass = block_sums(mass), own_above = block_sums(above);
+        if (threadIdx.x == 0) { sh.x_sum = own_mass; sh.x_above = own_above; }
+        __syncthreads();
+        cluster.sync();
+        whole = sum_ranks(of_rank(&sh.x_sum));
+        const u64 base = sum_ranks(of_rank(&sh.x_above)), target = share_of(share, whole);
+        if (base >= target || !rank_lists<true>(base, target) || cut == 0) return false;   // (the same in all blocks)
+        const int listed_here = static_cast<int>(sh.x_listed);
+        for (int i = lane; i < listed_here; i += 32) {
+            const u64 token = sh.list[i];
+            const int place = static_cast<int>(0xffffffffu - static_cast<uint32_t>(token)) - first;
+            if (token >= cut && place / N / seg == warp) above += weight(key_value(static_cast<uint32_t>(token >> 32)));
+        }
+        return true;
+    }
+
+    // The cut of top-p, from an estimate of the masses: weights in fp32 and in units of 2^-14 of their bin's heaviest, added up in bins over the logits, with
+    // native 32-bit atomics.  Tokens lighter than (1 - share) / vocabulary of the whole need no bin and only count in the whole, which `z` is at T = 1 and
+    // not below z at higher ones.  A mass estimated so
+    // is off by less than 2^-14 of itself, so the cut lies within 2^-13 of the share.
+    __device__ bool estimated_cut(double share, int vocabulary, float z, float temp, u64& above, u64& whole) {
+        constexpr int UNIT = 14;                                   // (sums stay below 2^32: a block has at most 2^17 tokens, V / 8, of 2^14)
+        const int bins = blocks == 1 ? 2 * kBins : 4 * kBins;
+        const float depth = fminf(kRange, fmaxf(static_cast<float>(log2(vocabulary / ((1. - share) * (temp >= 1.f ? z : 1.f)))), 0.f) + 0.1f), scale = bins / depth, inv_scale = depth / bins;
+        for (int i = threadIdx.x; i < bins; i += kThreads) sh.estimate[i] = 0;
+        if (threadIdx.x == 0) sh.b_bin = sh.b_last = 0xffffffffu;
+        __syncthreads();
+        const bool count_light = temp != 1.f;
+        const float deepest = count_light ? floor_l : fmaxf(floor_l, logit_below(-depth));
+        float light = 0.f;
+        const int e = min(nvec, (warp + 1) * seg);
+        for (int v = warp * seg + lane; v < e; v += 32) {
+            float l[N], most;
+            Vec<T>::get(vec(v), l);
+            most = l[0];
+#pragma unroll
+            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
+            if (!(most >= deepest)) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (!(l[j] >= deepest)) continue;
+                const float c = coarse(l[j]), at = -c * scale;
+                if (at < bins) {
+                    const int bin = static_cast<int>(at);
+                    atomicAdd(&sh.estimate[bin], __float2uint_rn(ex2(UNIT - (at - bin) * inv_scale)));
+                } else if (count_light) {
+                    light += ex2(c);
+                }
+            }
+        }
+        if (count_light) {
+            const u64 own_light = block_sums(static_cast<u64>(light * 0x1p32f));   // (estimates are multiples of 2^-32)
+            if (threadIdx.x == 0) sh.x_sum = own_light;
+        }
+        __syncthreads();
+        cluster.sync();
+        constexpr int PER = 4;
+        const int part = bins / blocks, bin = rank * part + threadIdx.x * PER;
+        u64 q[PER], mine = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) q[k] = 0;
+        if (static_cast<int>(threadIdx.x) * PER < part) {
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                if (r >= blocks) break;
+                const uint4 four = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.estimate, r) + bin);
+                q[0] += four.x; q[1] += four.y; q[2] += four.z; q[3] += four.w;
+            }
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                q[k] = static_cast<u64>(static_cast<double>(q[k]) * static_cast<double>(ex2(32 - UNIT - (bin + k) * inv_scale)));
+                mine += q[k];
+            }
+        }
+        const u64 upto = warp_scan(mine, lane);
+        __syncthreads();
+        if (lane == 31) sh.warp_q[warp] = upto;
+        __syncthreads();
+        u64 before = upto - mine, own = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += sh.warp_q[w];
+            own += sh.warp_q[w];
+        }
+        if (threadIdx.x == 0) sh.x_bins = own;
+        cluster.sync();
+        const u64 of_blocks = of_rank(&sh.x_bins);
+        const double aim = share * (count_light ? static_cast<double>(sum_ranks(of_blocks) + sum_ranks(of_rank(&sh.x_sum))) : static_cast<double>(z) * 0x1p32);
+        const u64 from = max(1ull, static_cast<u64>(aim * (1. - 0x1p-13))), to = max(1ull, static_cast<u64>(aim * (1. + 0x1p-13)));
+        before += __shfl_sync(0xffffffffu, warp_scan(of_blocks, lane) - of_blocks, rank);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const u64 after = before + q[k];
+            if (before < from && from <= after)
+                for (int r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->b_bin = bin + k;
+            if (before < to && to <= after)
+                for (int r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->b_last = bin + k;
+            before = after;
+        }
+        cluster.sync();
+        const uint32_t bin_a = sh.b_bin, bin_b = min(sh.b_last, static_cast<uint32_t>(bins) - 1);   // (none: behind all bins)
+        const float upper = bin_a == 0 ? INFINITY : bin_a < static_cast<uint32_t>(bins) ? logit_above(-(bin_a - 0.001) * inv_scale) : kLowest;
+        return proved_cut(share, fmaxf(floor_l, logit_below(-(bin_b + 1.001) * inv_scale)), upper, above, whole);
     }
     __device__ __forceinline__ void set_cut(u64 c) {
         cut = c;
@@ -574,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     const float top_p = p.top_p ? p.top_p[b] : p.top_p_all, min_p = p.min_p ? p.min_p[b] : p.min_p_all, u = p.u[b];
     // (& and not &&: with branches here, the device compiler of CUDA 12.9 gave up the test of k on the path without top_p)
     const bool drawing = temp > 0.f, greedy = !drawing, use_k = drawing & (k > 0) & (k < p.V), use_p = drawing & (top_p < 1.f), use_m = drawing & (min_p > 0.f);
-    const bool z_is_mass = drawing & (temp == 1.f) & !use_k & !use_m;   // the sum for the log-probability is the mass of all tokens
+    const bool z_is_mass = drawing & (temp == 1.f) & !use_k & !use_m & !use_p;   // the sum for the log-probability is the mass of all tokens
     const float k2e = static_cast<float>(kLog2eD);
 
     // The row's part into shared memory, and on the way, for each thread, the largest logit that it meets (NaN never is), the vector that held it first,
@@ -684,7 +825,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     z = rebased(row.of_rank(&sh.x_z), of_block, top);
 #pragma unroll
     for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    float log_z = logf(__shfl_sync(0xffffffffu, z, 0));
+    z = __shfl_sync(0xffffffffu, z, 0);
+    float log_z = logf(z);
     if (greedy || top == 0) {                                      // top == 0: nothing above -inf, nothing to draw
         if (row.rank == 0 && row.warp == 0) {
             at = __reduce_min_sync(0xffffffffu, of_block == top && top ? row.of_rank(&sh.x_index) : 0xffffffffu);
@@ -700,11 +842,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     row.floor_l = row.logit_below(fmax(row.least, -static_cast<double>(kRange)));
 
     // the mass for the draw, or for the bound of top-p's candidates
-    // (For top-p also the mass of the tokens of at least 2^-5 and 2^-10 of the largest weight: if one of them is enough, the cut lies above.)
-    u64 mass = 0, heavy[2] = {0, 0};
-    const float heavy_l[2] = {fmaxf(row.floor_l, row.logit_below(-5.)), fmaxf(row.floor_l, row.logit_below(-10.))};
-    auto add_up = [&](auto with_heavy) {
-        constexpr bool HEAVY = decltype(with_heavy)::value;
+    u64 mass = 0;
+    const bool by_estimate = use_p & !use_k & !use_m & !row.steep;
+    if (!use_k & !by_estimate) {
         const int e = min(row.nvec, (row.warp + 1) * row.seg);
         for (int v = row.warp * row.seg + row.lane; v < e; v += 32) {
             float l[N], most;
@@ -723,20 +863,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 #pragma unroll                                                     // what lies below the floor weighs nothing, like the floor itself
             for (int j = 0; j < N; ++j) mass += row.biased_weight(fmaxf(l[j], row.floor_l));
             mass -= N * row.kBias;
-            if (HEAVY && most >= heavy_l[1]) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    if (!(l[j] >= heavy_l[1])) continue;
-                    const u64 w = row.fast_weight(l[j]);
-                    heavy[1] += w;
-                    if (l[j] >= heavy_l[0]) heavy[0] += w;
-                }
-            }
         }
-    };
-    if (!use_k) {
-        if (use_p) add_up(std::true_type{});
-        else add_up(std::false_type{});
     }
     auto kept_weight = [&](int i, float l) -> u64 { return row.kept(i, l) ? row.weight(l) : 0; };
     auto aim = [&](u64 total) {
@@ -753,15 +880,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
             const uint32_t kth = __reduce_min_sync(0xffffffffu, row.lane < row.blocks ? *row.cluster.map_shared_rank(&sh.x_kth, row.lane) : 0xffffffffu);
             if (kth) row.floor_l = fmaxf(row.floor_l, key_value(kth));
         }
-    } else {
+    } else if (!by_estimate) {
         const u64 own_mass = row.block_sums(mass);
-        if (use_p) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const u64 own = row.block_sums(heavy[i]);
-                if (threadIdx.x == 0) sh.x_heavy[i] = own;
-            }
-        }
         if (threadIdx.x == 0) sh.x_sum = own_mass;
         __syncthreads();
         row.cluster.sync();
@@ -776,14 +896,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         }
     }
     const double share = fmax(static_cast<double>(top_p), 0.);
+    if (by_estimate) {
+        if (row.estimated_cut(share, p.V, z, temp, mass, whole)) {
+            row.locate(kept_weight, mass, aim, found);
+            row.sync();
+            return;
+        }
+    }
     if (use_p && !use_k) {
-        // (.999: their multiples of 2^-44 are rounded, each by half a multiple at most)
+        // Tokens lighter than this make up less than 1 - top_p together.  (.999: their multiples of 2^-44 are rounded, each by half a multiple at most)
         const double light = (1. - share) * 0.999 * static_cast<double>(whole) / p.V;
         if (light > 1000.) row.floor_l = fmaxf(row.floor_l, row.logit_below(fmin(log2(light) - kFrac, 0.)));
-        const u64 target = row.share_of(share, whole);
-#pragma unroll
-        for (int i = 1; i >= 0; --i)
-            if (row.sum_ranks(row.of_rank(&sh.x_heavy[i])) >= target) row.floor_l = fmaxf(row.floor_l, heavy_l[i]);
     }
     int total = 0;
     const bool noted = row.note_down(total);
