@@ -462,6 +462,20 @@ def test_sample_tokens_ties(V, dtype):
             _check_sample(x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("V", [300, 30011, 151936])
+@pytest.mark.parametrize("sigma", [0.05, 1.0, 4.0])
+def test_sample_tokens_top_p_alone(sigma, V, dtype):
+    """From rows that are almost flat to peaked ones; in half of them a few tokens stand out; shares from one token to all but the lightest."""
+    B = 6
+    x = _logits(B, V, FP32, seed=V, sigma=sigma)
+    x[::2, 7::V // 3] += 9.0
+    x, u = x.to(dtype), _uniform(B, V)
+    for temperature in (0.3, 1.0, 1.7, 8.0):
+        for top_p in (1e-6, 0.05, 0.5, 0.9, 0.99, 0.999999):
+            _check_sample(x, u, temperature=temperature, top_p=top_p)
+
+
 def test_sample_tokens_crowded_bins():
     """Logits crowded at two places, so that bins have to be divided again and again, down to neighbouring fp32 values."""
     B, V = 6, 30000
