@@ -691,7 +691,7 @@ struct Row {
 };
 
 template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens p, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens p, int slice, int ahead) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ Shared sh;
     Row<T, RESIDENT> row(sh);
@@ -753,6 +753,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
                 for (int j = 0; j < N; ++j) z += ex2((l[j] - best) * k2e);
             }
         }
+    }
+    // The row that comes when this one is done, as far as that can be known, into L2: HBM would be idle while this one is worked on.
+    if (RESIDENT && threadIdx.x == 0 && b + ahead < p.B) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(src + ahead * p.row_stride), to = from + static_cast<uintptr_t>(max(0, row.end - row.off)) * sizeof(T);
+        const uintptr_t lo = (from + 15) & ~uintptr_t{15}, hi = to & ~uintptr_t{15};
+        if (lo < hi) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(lo), "r"(static_cast<uint32_t>(hi - lo)) : "memory");
     }
     if (!(z >= 0.f) || best == kLowest) {                          // NaN, or infinities among the logits, or nothing above the lowest number: once more, with care
         z = 0.f;
@@ -998,7 +1004,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 }
 
 template <typename T, bool RESIDENT>
-const char* launch(const SampleTokens& p, int blocks, int slice, int smem, cudaStream_t s) {
+const char* launch(const SampleTokens& p, int blocks, int slice, int smem, int num_sms, cudaStream_t s) {
     static std::atomic<uint64_t> raised{0};
     auto k = sample_tokens_kernel<T, RESIDENT>;
     if (RESIDENT && !raise_smem_limit(reinterpret_cast<const void*>(k), kMost, raised)) return "sample_tokens: the shared-memory limit could not be raised";
@@ -1013,7 +1019,7 @@ const char* launch(const SampleTokens& p, int blocks, int slice, int smem, cudaS
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, k, p, slice); e != cudaSuccess) {
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, k, p, slice, max(1, 2 * num_sms / blocks)); e != cudaSuccess) {
         cudaGetLastError();
         return cudaGetErrorString(e);
     }
@@ -1028,8 +1034,8 @@ const char* launch_type(const SampleTokens& p, int num_sms, cudaStream_t s) {
     while (blocks < kMaxCluster && (static_cast<int64_t>(p.V) * sizeof(T) > kFit * blocks || (static_cast<int64_t>(p.B) * blocks * 2 <= num_sms && p.V > 2048 * blocks))) blocks *= 2;
     const int slice = ((p.V + blocks - 1) / blocks + 15) / 16 * 16;
     const int64_t bytes = static_cast<int64_t>(slice) * sizeof(T) + 32;    // (a part begins up to 15 bytes behind a 16-byte boundary)
-    if (bytes <= kMost) return launch<T, true>(p, blocks, slice, static_cast<int>(bytes), s);
-    return launch<T, false>(p, blocks, slice, 0, s);               // a vocabulary beyond 8 x 190 KB is read again in every pass
+    if (bytes <= kMost) return launch<T, true>(p, blocks, slice, static_cast<int>(bytes), num_sms, s);
+    return launch<T, false>(p, blocks, slice, 0, num_sms, s);               // a vocabulary beyond 8 x 190 KB is read again in every pass
 }
 
 }  // namespace
