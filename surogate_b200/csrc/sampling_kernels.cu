@@ -10,11 +10,15 @@
 // * The result is a token, not a number that may be a little off, so masses are integers: weights as multiples of 2^-44 of the largest one
 //   (exponentials in fp64 by a table of 2^(j/64) and three terms of the series: relative error below 2^-34), whose sums do not depend on the order.
 //   A wrong token takes a u within that of a boundary.
-// * Cuts need no sort.  Bounds leave a few candidates: the k largest logits are not below the k-th of the threads' own maxima; tokens lighter
-//   than (1 - top_p) / vocabulary of the whole mass make up less than 1 - top_p together, so the cut of top-p lies above them.  Up to 512
-//   candidates are ranked against one another by one block.  More (flat rows, large k) are counted, with their mass, in 1024 bins over the
-//   logits; the bin in which the cut falls is found by a scan and only its tokens are ranked; a bin with too many is divided again, equal
-//   logits are counted by index.
+// * Cuts need no sort.  Bounds leave a few candidates: the k largest logits are not below the k-th of the threads' own maxima.  Up to 512 candidates
+//   are ranked against one another by one block.  More (large k) are counted, with their mass, in 1024 bins over the logits; the bin in which
+//   the cut falls is found by a scan and only its tokens are ranked; a bin with too many is divided again, equal logits are counted by index.
+// * Top-p alone, where flat rows leave tens of thousands of candidates, estimates masses first and proves the cut after (estimated_cut).
+//
+// Measured (B200; fp32, vocabulary 151 936, 608 KB a row; one row, then 256 rows, which a copy would read in 24 us): greedy 13 and 73 us; T 1 without
+// filters 15 and 128; top-k 40 14 and 121; top-p 0.9 29 and 291; min-p 0.05 12 and 102; T 0.7, top-k 20, top-p 0.8, min-p 0.01 12 and 116.  One row is
+// latency: launch, loading, four or five exchanges in the cluster.  Many rows are bound by instructions (the fp64 weights, one to two passes) and by the
+// exchanges, with two blocks an SM to fill each other's pauses.  Bf16, 64 rows of 128 256: 22 us without filters, 49 with top-p.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
