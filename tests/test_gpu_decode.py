@@ -320,6 +320,31 @@ def test_kv_append_e4m3(src, D):
     _no_errors()
 
 
+def test_kv_append_e4m3_ends_of_the_range():
+    """fp32 rows of the largest numbers, of the smallest, of zeros of both signs, and with infinities (finite neighbours become zeros, they NaN)."""
+    from surogate_b200.ops.paged_kv import kv_append_reference
+
+    T, D, P = 12, 64, 16
+    n, table = _pages(1, 1)
+    k = torch.randn(1, T, 1, D, generator=torch.Generator().manual_seed(2)).to(DEV)
+    for t, scale in enumerate((3.0e38 / 6, 1e30, 1e-30, 1e-37, 1e-40, 1e-44)):
+        k[0, t] *= scale
+    k[0, 6] = torch.where(k[0, 6] > 0, 0.0, -0.0)
+    k[0, 7, :, ::3] = -0.0
+    k[0, 8, :, 5] = float("inf")
+    k[0, 9, :, 6] = -float("inf")
+    start = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got, gs = torch.zeros(n, 2, 1, P, D, device=DEV).to(E4M3), torch.ones(n, 2, 1, P, device=DEV)
+    want, ws = got.clone(), gs.clone()
+    kv_append_reference(want, k, -k, table, start, None, ws)
+    _ops().kv_append(got, k, -k, table, start, None, gs)
+    assert torch.equal(gs, ws)
+    a, b = got.view(torch.uint8), want.view(torch.uint8)
+    nan = (b & 0x7f) == 0x7f                                           # a NaN's sign means nothing
+    assert torch.equal((a & 0x7f) == 0x7f, nan) and torch.equal(a[~nan], b[~nan])
+    _no_errors()
+
+
 def test_kv_append_odd_sources_and_bad_places():
     B, T, P, Hkv, D = 3, 4, 16, 2, 64
     n, table = _pages(B, 2)
