@@ -171,8 +171,7 @@ class PagedKVCache:
     """The pages of all layers, and which sequence owns which.
 
     Sequences are numbers below ``max_seqs``.  Pages are counted by owner: ``fork`` lets completions of one prompt share its full pages and
-    copies only the last, partly filled one.  The books are kept on the host; ``table`` and ``lengths`` give the device copies that the kernels
-    read, refreshed only after a change."""
+    copies only the last, partly filled one.  The books are kept on the host; ``table`` makes the device copy that the kernels read."""
 
     def __init__(self, n_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, max_seqs: int, dtype: torch.dtype = torch.bfloat16, device=None):
         if page_size <= 0 or page_size % 16:
