@@ -106,7 +106,7 @@ def _problem(B, Hq, Hkv, D, P, lengths, dtype, seed=0, width=None):
 
 # ---------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("dtype", [BF16, FP16, E4M3])
-@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (32, 8, 128), (8, 8, 64), (14, 2, 64), (64, 4, 128), (12, 2, 256), (20, 1, 128), (40, 1, 64), (18, 1, 256)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (32, 8, 128), (8, 8, 64), (14, 2, 64), (64, 4, 128), (12, 2, 256), (20, 1, 128), (40, 1, 64), (18, 1, 256), (300, 2, 64), (7, 7, 128)])
 def test_paged_attention_heads(dtype, Hq, Hkv, D):
     q, kv, table, n, s = _problem(3, Hq, Hkv, D, 16, [1, 77, 1030], dtype, seed=Hq + D)
     _check_attention(q, kv, table, n, scales=s)
@@ -278,6 +278,26 @@ def test_paged_attention_refusals():
 
 
 # ---------------------------------------------------------------------------------------------- append, pages
+def test_pages_beyond_32_bit_offsets():
+    """A cache of 2^32 elements and more: new tokens, copies and attention at its far end."""
+    n, Hkv, P, D, T = 33000, 8, 64, 128, 70
+    kv = torch.empty(n, 2, Hkv, P, D, dtype=BF16, device=DEV)
+    assert kv.numel() > 2 ** 32
+    table = torch.tensor([[n - 1, 5], [n - 4, n - 2]], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(2, T, Hkv, D, generator=g).to(BF16).to(DEV) for _ in range(2))
+    start, lengths = torch.zeros(2, dtype=torch.int32, device=DEV), torch.full((2,), T, dtype=torch.int32, device=DEV)
+    _ops().kv_append(kv, k, v, table, start)
+    for b in range(2):
+        for t in (0, 63, 64, T - 1):
+            assert torch.equal(kv[table[b, t // P], 0, :, t % P], k[b, t]) and torch.equal(kv[table[b, t // P], 1, :, t % P], v[b, t])
+    q = torch.randn(2, 2 * Hkv, D, generator=g).to(BF16).to(DEV)
+    _check_attention(q, kv, table, lengths)
+    _ops().kv_copy_pages(kv[None], torch.tensor([n - 1, n - 2], dtype=torch.int32, device=DEV), torch.tensor([n - 3, 7], dtype=torch.int32, device=DEV))
+    assert torch.equal(kv[n - 3, :, :, :], kv[n - 1]) and torch.equal(kv[7, :, :, :6], kv[n - 2, :, :, :6])
+    _check_attention(q, kv, torch.tensor([[n - 3, 5], [n - 4, 7]], dtype=torch.int32, device=DEV), lengths)
+
+
 @pytest.mark.parametrize("dtype,D,Hkv", [(BF16, 128, 8), (FP16, 64, 1), (FP32, 128, 3), (BF16, 256, 2), (BF16, 80, 3), (FP16, 8, 5)])
 @pytest.mark.parametrize("T", [1, 2, 37])
 def test_kv_append(dtype, D, Hkv, T):
@@ -573,6 +593,40 @@ def test_sample_tokens_vocabulary_beyond_shared_memory(V):
         x = _logits(2, V, dtype)
         for kw in [{}, dict(top_p=0.5), dict(top_k=1000)]:
             _check_sample(x, _uniform(2), **kw)
+
+
+@pytest.mark.parametrize("B,V", [(1, 2 ** 20 - 1), (100000, 40), (3000, 1)])
+def test_sample_tokens_largest_and_most_rows(B, V):
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x, u = torch.randn(B, V, generator=g, device=DEV) * 3, torch.rand(B, generator=g, device=DEV)
+    tok, lp = _ops().sample_tokens(x, u, top_p=0.8)
+    rows = torch.arange(0, B, max(1, B // 50), device=DEV)
+    _check_sample(x[rows].contiguous(), u[rows], top_p=0.8)
+    assert torch.equal(_ops().sample_tokens(x[rows].contiguous(), u[rows], top_p=0.8)[0], tok[rows])
+    _check_sample(x[rows].contiguous(), u[rows], temperature=0.9, top_k=7)
+
+
+def test_sample_tokens_rows_far_apart():
+    """Rows whose offsets pass 2^31 elements, one row of the tensor used twice, and calls on two streams at once."""
+    V, far = 30000, 2 ** 30 + 8
+    x = torch.as_strided(torch.empty(2 * far + V, device=DEV), (3, V), (far, 1))
+    x.copy_(_logits(3, V, FP32, seed=4))
+    u = _uniform(3, 4)
+    _check_sample(x, u, top_p=0.9)
+    _check_sample(x[2:].expand(5, V), _uniform(5), temperature=0.8, top_k=30)
+    y, v = _logits(200, V, BF16, seed=5), _uniform(200, 5)
+    want = _ops().sample_tokens(x, u, top_p=0.7), _ops().sample_tokens(y, v, top_p=0.7)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        got = []
+        for s, (a, b) in zip(streams, ((x, u), (y, v))):
+            with torch.cuda.stream(s):
+                got.append(_ops().sample_tokens(a, b, top_p=0.7))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for w, g in zip(want, got) for p, q in zip(w, g))
+    _no_errors()
 
 
 def test_sample_tokens_follows_the_distribution():
