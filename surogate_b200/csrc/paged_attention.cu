@@ -813,9 +813,9 @@ PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_
     plan.head_groups = (G + plan.rows - 1) / plan.rows;
     const int64_t pairs = static_cast<int64_t>(B) * Hkv * plan.head_groups, tiles = (max_keys + kTile - 1) / kTile;
     const int most = num_sms * (kv_type == kKvE4m3 ? blocks_per_sm<kKvE4m3>(dim, plan.rows) : blocks_per_sm<kKvBf16>(dim, plan.rows));
-    // Rows that cannot hold more than 1024 keys are not split (32 query heads over 8 key heads of 128, bf16, equal rows; whole against split: 1 row of
-    // 512 / 1000 / 2000 keys 8.0 / 11.2 / 17.4 us against 10.6 / 10.9 / 11.6, 8 rows 8.3 / 11.4 / 17.9 against 11.7 / 13.6 / 18.7, 64 rows 31 / 53 / 94
-    // against 33 / 54 / 91, 256 rows 87 / 158 / 307 against 99 / 175 / 322; longer rows differ more in length, which only the split evens out).
+    // Rows that cannot hold more than 1024 keys are not split (32 query heads over 8 key heads of 128, bf16; whole against split: 1 row of 512 / 1000
+    // keys 7.6 / 10.9 us against 10.2 / 10.3, 8 rows 8.1 / 11.3 against 11.6 / 13.1, 32 rows 11 / 25 against 16 / 30, 64 rows 30 / 50 against 30 / 50, and of
+    // 50 to 1000 keys 37.5 against 33.0, 256 rows 86 / 167 against 94 / 179).  Longer rows differ more in length, which only the split evens out.
     plan.whole = tiles <= 16;
     plan.deep = plan.whole && pairs <= num_sms;
     const int64_t work = plan.whole ? pairs : pairs * tiles;
