@@ -47,7 +47,7 @@ namespace {
 constexpr int kTile = 64, kStep = 16;   // keys of a tile that blocks share, keys of a warp and step
 constexpr int kSharing = 4;              // warps of a block that shares rows with others
 constexpr int RING_BYTES = 16384;   // of a warp, where two steps fit
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
@@ -228,6 +228,7 @@ struct Piece {
         };
         int pages = load_pages(0), pages_next = load_pages(32);
         unsigned have = 0;            // bit i % 32: step i has a page
+        bool seen = false;            // a key that counts has been met
         int next_i = 0, next_place = (tb * S::TILE + warp * kStep) % p.kv.page_size;   // the step that is requested next
         const int place_step = S::TILE % p.kv.page_size;
 
@@ -490,6 +491,7 @@ struct Piece {
             if (!__all_sync(0xffffffffu, mbar_wait(bars + rg.slot * 8, rg.parity, rg.abort_flag))) break;   // a wait that gave up
             const uint32_t at = ring + rg.slot * S::STAGE;
             if ((have >> (i & 31)) & 1) {
+                seen = true;
                 if (t0 >= lo && t0 + kStep <= n) compute(std::true_type{}, at, t0);
                 else compute(std::false_type{}, at, t0);
             }
@@ -505,14 +507,16 @@ struct Piece {
             if (++rg.slot == S::STAGES) { rg.slot = 0; rg.parity ^= 1; }
         }
 
-        // the warps meet
+        // The warps meet.  A warp without keys has the maximum -inf; one whose keys had no score above -inf (all of them -inf or NaN: sums are 0 or NaN) has
+        // the lowest number, so that its NaN stay, and a row of nothing but such keys is not taken for an empty one.
 #pragma unroll
         for (int r = 0; r < S::HT; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[r][h] += __shfl_xor_sync(0xffffffffu, l[r][h], x);
-                if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(limit[r][h] == -INFINITY ? -INFINITY : top[r][h], l[r][h]);
+                if (limit[r][h] == -INFINITY) top[r][h] = seen ? kLowest : -INFINITY;
+                if (g == 0) sh_ml[warp][8 * r + 2 * c + h] = make_float2(top[r][h], l[r][h]);
             }
         __syncthreads();
         float* mine = rg.meet + warp * (ROWS * D);
@@ -524,7 +528,7 @@ struct Piece {
                 float mm = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < S::WARPS; ++w) mm = fmaxf(mm, sh_ml[w][head].x);
-                const float f = limit[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
+                const float f = top[r][h] == -INFINITY ? 0.f : ex2(top[r][h] - mm);
 #pragma unroll
                 for (int j = 0; j < S::VCH; ++j)
 #pragma unroll
@@ -558,7 +562,7 @@ struct Piece {
         return __syncthreads_or(gave_up) == 0;
     }
 
-    // elements d to d + 3 of one output
+    // elements d to d + 3 of one output.  mm == -inf: no key counts.  Keys without a score above -inf leave 0 / 0, or 0 / sink.
     static __device__ __forceinline__ void finish(const PagedAttention& p, int b, int h, int d, float mm, float ll, float4 acc) {
         const int64_t at = static_cast<int64_t>(b) * p.Hq + h;
         float total = ll;
@@ -570,7 +574,7 @@ struct Piece {
         y[2] = from_float<QT>(mm == -INFINITY ? 0.f : acc.z * f / total);
         y[3] = from_float<QT>(mm == -INFINITY ? 0.f : acc.w * f / total);
         *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + at * D + d) = *reinterpret_cast<const uint2*>(y);
-        if (d == 0 && p.lse) p.lse[at] = mm == -INFINITY ? -INFINITY : mm * kLn2 + logf(ll);
+        if (d == 0 && p.lse) p.lse[at] = fabsf(mm) == INFINITY ? mm : mm * kLn2 + logf(ll);   // (infinite scores: their weights are NaN)
     }
 };
 

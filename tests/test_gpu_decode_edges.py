@@ -1,0 +1,75 @@
+"""The kernels of the answering path where formulas meet the ends of their types: numbers that are not finite, caps of scores, values of zero,
+pages copied onto themselves, calls captured into graphs.  Tolerances as in ``test_gpu_decode``, or stated at the test."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _no_errors, _ops, _problem
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- attention: numbers that are not finite
+def _check_not_finite(q, kv, table, n, **kw):
+    """Outputs are not finite where the definition's are not (of an infinite value NaN may come out: its weight has two terms, of two signs), the
+    log-sum-exp is what the definition gives, and where the definition is finite the two agree to what their types hold."""
+    got, lse = _ops().paged_attention(q, kv, table, n, return_lse=True, **kw)
+    _no_errors()
+    want, wlse, mag, big = _attention64(q, kv, table, n, q.shape[-1] ** -0.5, **kw)
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)), (torch.isfinite(got) != torch.isfinite(want)).nonzero()[:5].tolist()
+    assert torch.isnan(got)[torch.isnan(want)].all()
+    for odd in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(odd(lse), odd(wlse)), (odd.__name__, lse, wlse)
+    fin = torch.isfinite(want)
+    # (half a step of the output, and the weights' and scores' errors: the widest of the types', e4m3's, over all)
+    bound = torch.finfo(q.dtype).eps / 2 * want.abs() + (2.0 ** -11 + 2.0 ** -17 * (1 + big.unsqueeze(-1).nan_to_num(0, 0, 0))) * mag.nan_to_num(0, 0, 0) * 1.01 + 2.0 ** -24
+    assert ((got.double() - want).abs()[fin] <= bound[fin]).all()
+    fin = torch.isfinite(wlse)
+    assert ((lse.double() - wlse)[fin].abs() <= 2.0 ** -17 * (1 + wlse[fin].abs() + big[fin].nan_to_num(0, 0, 0))).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, E4M3])
+@pytest.mark.parametrize("longest", [300, 1000, 3000])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_paged_attention_scores_that_are_not_finite(dtype, longest, sinks):
+    """NaN and infinities in a query, in one key, in all keys of a row, and over the keys of single warps: rows that stay whole, few and many, and rows
+    that are split and joined.  A row without keys stays zeros."""
+    for B in (3, 90):
+        lengths = [longest, 0, 20] + [longest // 2 + 5 * i for i in range(B - 3)]
+        lengths = [min(x, longest) for x in lengths]
+        q, kv, table, n, s = _problem(B, 4, 2, 64, 16, lengths, dtype, seed=longest + B)
+        kw = dict(scales=s, sinks=torch.linspace(-3.0, 3.0, 4, device=DEV) if sinks else None)
+        for value in (math.nan, math.inf):
+            x = q.clone()
+            x[0, 1, 7] = value
+            if value != value:
+                x[2] = value
+                x[2, 3] = q[2, 3]
+            if dtype != E4M3 or value != value:                          # (infinite elements and 8-bit zeros: NaN scores in both)
+                _check_not_finite(x, kv, table, n, **kw)
+        page = table[0].long()
+        bad = [math.nan] if dtype == E4M3 else [math.nan, math.inf, -math.inf]
+        for value in bad:
+            for keys in ([5], [longest - 1], range(longest), [j for j in range(longest) if j // 16 % 4 == 1], [j for j in range(longest) if j // 16 % 4 != 1], range(64)):
+                dirty = kv.clone()
+                j = torch.tensor(list(keys), device=DEV)
+                dirty[page[j // 16], 0, 0, j % 16, 3] = torch.full((), value, device=DEV).to(dtype)
+                _check_not_finite(q, dirty, table, n, **kw)
+        # one value, and a whole row of values
+        dirty = kv.clone()
+        dirty[page[0], 1, 1, 9, 11] = torch.full((), bad[-1], device=DEV).to(dtype)
+        dirty[page[1], 1, 0, 2] = torch.full((), math.nan, device=DEV).to(dtype)
+        _check_not_finite(q, dirty, table, n, **kw)
+
+
+def test_paged_attention_of_scores_that_are_all_minus_infinity():
+    """Without a sink 0 / 0, with one the sink takes all; the log-sum-exp is -inf."""
+    for longest in (40, 2500):
+        q, kv, table, n, _ = _problem(2, 4, 2, 64, 16, [longest, 30], BF16)
+        q[0] = q[0].abs()
+        kv[table[0].long(), 0, :, :, 5] = -math.inf
+        _check_not_finite(q, kv, table, n)
+        _check_not_finite(q, kv, table, n, sinks=torch.zeros(4, device=DEV))
+        out, lse = _ops().paged_attention(q, kv, table, n, sinks=torch.zeros(4, device=DEV), return_lse=True)
+        assert (out[0] == 0).all() and (lse[0] == -math.inf).all() and torch.isfinite(out[1]).all()
