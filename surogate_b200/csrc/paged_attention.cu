@@ -366,8 +366,9 @@ struct Piece {
                     for (int r = 0; r < S::HT; ++r)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
-                    vs[t] = fmaxf(lds4(sa + 64 + t * 32), 0x1p-100f);
-                    lv[t] = __log2f(vs[t]);
+                    vs[t] = lds4(sa + 64 + t * 32);
+                    vs[t] = vs[t] < 0x1p-100f ? 0x1p-100f : vs[t];   // (a NaN stays)
+                    lv[t] = vs[t] < INFINITY ? __log2f(vs[t]) : 0.f;   // the row's outputs become NaN, whatever the bound
                 }
             }
             if (!FULL && KT == kKvE4m3) {

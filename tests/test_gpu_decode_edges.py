@@ -73,3 +73,12 @@ def test_paged_attention_of_scores_that_are_all_minus_infinity():
         _check_not_finite(q, kv, table, n, sinks=torch.zeros(4, device=DEV))
         out, lse = _ops().paged_attention(q, kv, table, n, sinks=torch.zeros(4, device=DEV), return_lse=True)
         assert (out[0] == 0).all() and (lse[0] == -math.inf).all() and torch.isfinite(out[1]).all()
+
+
+def test_paged_attention_of_value_scales_that_are_not_finite():
+    """A value scale of NaN, or of infinity, makes the row's outputs NaN; its log-sum-exp, which no value enters, stays."""
+    for longest in (300, 3000):
+        for value in (math.nan, math.inf):
+            q, kv, table, n, s = _problem(3, 4, 2, 64, 16, [longest, 0, 20], E4M3, seed=longest)
+            s[table[0, 1].long(), 1, 0, 5] = value
+            _check_not_finite(q, kv, table, n, scales=s)
