@@ -17,8 +17,9 @@
 // * A running maximum that moves only when a score exceeds it by 2^8 (see `top`): most steps need neither a maximum over lanes nor a rescaling.
 //   The warps of a block have their own and meet at the end of the piece; pieces of a row in different blocks are joined by a second, small kernel.
 // * Weights are split into two bf16 (or fp16) terms before they meet the values, hi + lo, which keeps 16 (22) bits: tensor cores have time to
-//   spare here, and the output's own rounding stays the only one that counts.  With e4m3 values one fp16 term (2^-12) is below the
-//   values' own 2^-4.
+//   spare here, and the output's own rounding stays the only one that counts.  With e4m3 values weight times scale is one fp16 term: 2^-12 of
+//   itself down to 2^-21 of the largest one met, 2^-32 of the largest below; both are less than the values' own 2^-4 takes (of an element, or, where
+//   it is far below its row's largest, 2^-10 of the row's scale).  That holds for scales that say how large values are; rows of zeros are found by looking.
 // * e4m3: keys and values become fp16 exactly; the query as fp16 is scaled by a power of two to below 2 for each row (what it loses lies 2^-25
 //   below its largest element).  The scale of a key multiplies its score; that of a value goes into its weight, and its log2 into the comparison
 //   with the running maximum, which then bounds weight times scale.
@@ -175,6 +176,8 @@ struct Piece {
     using S = Shape<KT, D, ROWS, DEEP>;
     // weights are carried as 2^7 times themselves where they become fp16, whose smallest step is 2^-24; they are below 2^(kSlack) before
     static constexpr float kShift = S::BF16 ? 0.f : 7.f, kSlack = 8.f;
+    // log2 of the least scale that counts in a maximum: a key may then weigh 2^88 and the slack in the sum of weights, and 2^30 of them fit fp32
+    static constexpr float kLeastScale = -88.f;
 
     static __device__ Ring begin(const CUtensorMap* map, uint8_t* smem, unsigned long long* bars, int* abort_flag) {
         uint8_t* at = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~uintptr_t{1023});
@@ -368,7 +371,7 @@ struct Piece {
                         for (int h = 0; h < 2; ++h) s[r][2 * t + h] = (s[r][2 * t + h] + s2[r][2 * t + h]) * ks;
                     vs[t] = lds4(sa + 64 + t * 32);
                     vs[t] = vs[t] < 0x1p-100f ? 0x1p-100f : vs[t];   // (a NaN stays)
-                    lv[t] = vs[t] < INFINITY ? __log2f(vs[t]) : 0.f;   // the row's outputs become NaN, whatever the bound
+                    lv[t] = vs[t] < INFINITY ? fmaxf(__log2f(vs[t]), kLeastScale) : 0.f;   // (not finite: outputs become NaN, whatever the bound)
                 }
             }
             if (!FULL && KT == kKvE4m3) {
@@ -397,6 +400,32 @@ struct Piece {
                 }
             }
             if (__any_sync(0xffffffffu, above)) {
+                // A row of zeros has the scale 1, thousands of times its neighbours', and adds nothing: with that in the maximum their weights would be lost
+                // among fp16's subnormals.  So such rows get the least scale.  (One that does not exceed the limit does no harm.)
+                if (KT == kKvE4m3) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        uint32_t some = 0;                         // the four lanes of a key look at its values together
+                        const uint32_t row = at + S::KBYTES + (k0 + 8 * t) * S::PITCH + c * 16;
+#pragma unroll
+                        for (int x = 0; x < S::BOXES; ++x)
+#pragma unroll
+                            for (int y = 0; y < S::PITCH; y += 64) {
+                                const uint4 v = lds16(row + x * S::BOXBYTES + y);
+                                some |= (v.x | v.y | v.z | v.w) & 0x7f7f7f7fu;
+                            }
+                        some |= __shfl_xor_sync(0xffffffffu, some, 1);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 2);
+                        if (some == 0 && vs[t] < INFINITY) {
+                            lv[t] = kLeastScale;
+                            vs[t] = 0x1p-88f;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < S::HT; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) most[r][h] = fmaxf(s[r][h] + lv[0], s[r][2 + h] + lv[1]);
+                }
 #pragma unroll
                 for (int r = 0; r < S::HT; ++r)
 #pragma unroll

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _no_errors, _ops, _problem
+from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _no_errors, _ops, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,26 @@ def test_paged_attention_of_value_scales_that_are_not_finite():
             q, kv, table, n, s = _problem(3, 4, 2, 64, 16, [longest, 0, 20], E4M3, seed=longest)
             s[table[0, 1].long(), 1, 0, 5] = value
             _check_not_finite(q, kv, table, n, scales=s)
+
+
+def test_paged_attention_of_zero_values():
+    """Tokens whose values are all zero have the scale 1, far above the others' 1e-4; where they have the highest scores, the weights of the others keep
+    their bits: errors as in ``test_gpu_decode``.  One such token, every third, the first ones only, and all of a row."""
+    for dtype in (E4M3, BF16, FP16):
+        for longest in (200, 2100):
+            for zero in ([0], [longest // 2], range(0, longest, 3), range(70), range(longest)):
+                q, kv, table, n, s = _problem(2, 4, 2, 64, 16, [longest, longest // 3], dtype, seed=longest)
+                j = torch.tensor(list(zero), device=DEV)
+                page, place = table[0].long()[j // 16], j % 16
+                # their scores, q . k / 8: 14 (base 2) for the first half of them, 50 for the second
+                score = torch.where(torch.arange(len(j), device=DEV) < (len(j) + 1) // 2, 14.0, 50.0) * math.log(2)
+                q[:, :, 0] = 8.0
+                kv[page, :, :, place] = torch.zeros((), device=DEV).to(dtype)
+                if dtype == E4M3:
+                    kv[page, 0, :, place, 0] = torch.full((), 256.0, device=DEV).to(dtype)
+                    s[:, 1] = 0.05 / 448
+                    s[page, 0, :, place] = (score / 256)[:, None].expand(-1, 2)
+                    s[page, 1, :, place] = 1.0
+                else:
+                    kv[page, 0, :, place, 0] = score[:, None].to(dtype).expand(-1, 2)
+                _check_attention(q, kv, table, n, scales=s)
