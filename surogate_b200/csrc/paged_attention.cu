@@ -71,6 +71,16 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// tanh(y) to some 2^-21 of itself: below 0.8 Lambert's continued fraction y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))) as one quotient (its
+// next term is 2^-26 there), above it (e^2y - 1) / (e^2y + 1), which would cancel for small y, and with a cap of 50 cost small scores 2^-16
+// of themselves and more.  NaN stays.
+__device__ __forceinline__ float tanh_ratio(float y) {
+    const float a = fabsf(y), q = y * y;
+    const bool small = a < 0.8f;
+    const float e = ex2((a > 12.f ? 12.f : a) * (2.f * kLog2e));   // (tanh 12 = 1 - 2^-34)
+    const float num = small ? a * fmaf(q, q + 105.f, 945.f) : e - 1.f, den = small ? fmaf(q, fmaf(q, 15.f, 420.f), 945.f) : e + 1.f;
+    return copysignf(__fdividef(num, den), y);
+}
 // d[16 x 8] += a[16 x 16] b[16 x 8]
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -311,7 +321,7 @@ struct Piece {
             mult[r][0] = __shfl_sync(0xffffffffu, own, 8 * c);     // lane 4 * head holds that head's
             mult[r][1] = __shfl_sync(0xffffffffu, own, 8 * c + 4);
         }
-        const float cap = p.softcap, inv_cap2 = cap != 0.f ? 2.f * kLog2e / cap : 0.f, cap2 = cap * kLog2e;
+        const float cap = p.softcap, inv_cap = cap != 0.f ? 1.f / cap : 0.f, cap2 = cap * kLog2e;
 
         // o[m][r]: outputs of two elements of the head and of heads 8 r + 2c, + 1: [0], [1] the first element's, [2], [3] the second's
         float o[S::MT][S::HT][4];
@@ -386,7 +396,7 @@ struct Piece {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float x = (KT == kKvE4m3 ? s[r][k] : s[r][k] + s2[r][k]) * mult[r][k & 1];
-                    if (cap != 0.f) x = cap2 * (1.f - __fdividef(2.f, ex2(x * inv_cap2) + 1.f));   // tanh(y) = 1 - 2 / (e^2y + 1)
+                    if (cap != 0.f) x = cap2 * tanh_ratio(x * inv_cap);
                     if (!FULL) {
                         const int key = t0 + k0 + 4 * (k & 2);
                         if (key < lo || key >= n) x = -INFINITY;

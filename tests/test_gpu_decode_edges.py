@@ -105,3 +105,19 @@ def test_paged_attention_of_zero_values():
                 else:
                     kv[page, 0, :, place, 0] = score[:, None].to(dtype).expand(-1, 2)
                 _check_attention(q, kv, table, n, scales=s)
+
+
+# ---------------------------------------------------------------------------------------------- attention: caps of the scores
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 5.0, 30.0, 50.0, 1e3, 1e4, 1e6, 1e12])
+@pytest.mark.parametrize("spread", [1e-3, 0.05, 2.0, 30.0])
+def test_paged_attention_cap_keeps_small_scores(cap, spread):
+    """Capped scores keep the relative accuracy of fp32.  Scores come out of fp32 sums of 64 products (some 2^-20 of the largest one, over
+    ``test_gpu_decode``'s 2^-19 with the rest); the cap adds 2^-20 of a score, and the log-sum-exp a rounding of its own.  Errors of the
+    log-sum-exp are held without what the cap's size could excuse: 2^-19 of the largest score, 2^-20 of the result and 2^-22."""
+    for longest in (300, 2500):
+        q, kv, table, n, _ = _problem(3, 4, 2, 64, 16, [longest, 1, 77], FP16, seed=int(spread * 1000))
+        q = (q.float() * spread / 2).half()
+        _check_attention(q, kv, table, n, softcap=cap)
+        _, lse = _ops().paged_attention(q, kv, table, n, softcap=cap, return_lse=True)
+        _, want, _, big = _attention64(q, kv, table, n, 0.125, softcap=cap)
+        assert ((lse.double() - want).abs() <= 2.0 ** -19 * big + 2.0 ** -20 * want.abs() + 2.0 ** -22).all()
