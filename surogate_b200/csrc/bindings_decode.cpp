@@ -170,7 +170,9 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q_given, const Tensor& 
     const int64_t B = q.size(0);
     TORCH_CHECK(B <= 65535 && B * q.size(1) < (int64_t{1} << 31), "paged_attention: at most 65535 rows, and 2^31 heads of them, in one call");
     const double scale = given_scale.has_value() ? *given_scale : 1. / std::sqrt(static_cast<double>(p.kv.dim));
-    TORCH_CHECK(window >= 0 && softcap >= 0 && std::isfinite(scale) && std::isfinite(softcap), "window and softcap must not be negative, scale and softcap finite");
+    // (fp32 holds the cap, its multiple by log2 e and its inverse)
+    TORCH_CHECK(window >= 0 && (softcap == 0 || (softcap >= 0x1p-64 && softcap <= 0x1p64)) && std::isfinite(static_cast<float>(scale)),
+                "window must not be negative, softcap 0 or within 2^-64 and 2^64, the scale finite in fp32");
     Tensor out = torch::empty({B, q.size(1), q.size(2)}, q.options()), lse;
     if (want_lse) lse = torch::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
     if (B == 0) return {out, lse};

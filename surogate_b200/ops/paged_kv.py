@@ -152,7 +152,7 @@ def paged_attention(q: torch.Tensor, kv: torch.Tensor, page_table: torch.Tensor,
 
     ``q [rows, query heads, head size]`` (64, 128 or 256 on a GPU; query head ``h`` reads key head ``h // (query heads / kv heads)``), of the
     cache's type, or bf16 / fp16 with an e4m3 cache.  ``window`` > 0: only the last ``window`` tokens; ``softcap`` > 0: scores become
-    ``softcap * tanh(score / softcap)``; ``sinks`` fp32 ``[query heads]``: logits that take part in the softmax's sum without a value;
+    ``softcap * tanh(score / softcap)`` (2^-64 to 2^64); ``sinks`` fp32 ``[query heads]``: logits that take part in the softmax's sum without a value;
     ``softmax_scale`` defaults to ``head size ** -0.5``.  Returns ``[rows, query heads, head size]`` of q's type, with ``return_lse`` also the
     fp32 log-sum-exp of the scores ``[rows, query heads]`` (without the sinks).  A row of length 0 gives zeros and -inf."""
     if kv.is_cuda:
@@ -160,6 +160,8 @@ def paged_attention(q: torch.Tensor, kv: torch.Tensor, page_table: torch.Tensor,
     else:
         if kv.dim() != 5 or kv.shape[1] != 2 or q.dim() != 3 or q.shape[2] != kv.shape[4] or q.shape[1] % kv.shape[2] or window < 0 or softcap < 0:
             raise RuntimeError("paged_attention: kv must be [pages, 2, kv heads, page size, head size], q [rows, query heads, head size]; window and softcap not negative")
+        if not (softcap == 0 or 2.0 ** -64 <= softcap <= 2.0 ** 64) or (softmax_scale is not None and not abs(softmax_scale) < 2.0 ** 128):
+            raise RuntimeError("paged_attention: softcap must be 0 or within 2^-64 and 2^64, the scale finite in fp32")
         if (scales is not None) != (kv.dtype == torch.float8_e4m3fn):
             raise RuntimeError("paged_attention: scales go with a float8_e4m3fn cache, and only with one")
         out, lse = paged_attention_reference(q, kv, page_table, lengths, softmax_scale, int(window), float(softcap), sinks, scales)

@@ -121,3 +121,12 @@ def test_paged_attention_cap_keeps_small_scores(cap, spread):
         _, lse = _ops().paged_attention(q, kv, table, n, softcap=cap, return_lse=True)
         _, want, _, big = _attention64(q, kv, table, n, 0.125, softcap=cap)
         assert ((lse.double() - want).abs() <= 2.0 ** -19 * big + 2.0 ** -20 * want.abs() + 2.0 ** -22).all()
+
+
+def test_paged_attention_refuses_caps_and_scales_that_fp32_cannot_hold():
+    q, kv, table, n, _ = _problem(2, 4, 2, 64, 16, [20, 20], BF16)
+    for kw in (dict(softcap=1e300), dict(softcap=1e38), dict(softcap=1e-300), dict(softcap=1e-38), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(softmax_scale=1e300),
+               dict(softmax_scale=float("inf"))):
+        with pytest.raises(RuntimeError):
+            _ops().paged_attention(q, kv, table, n, **kw)
+    _no_errors()
