@@ -119,6 +119,7 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
             tokens, logprobs = sample_tokens(logits, u[torch.tensor(alive, device=device)] if len(alive) < len(u) else u, **draw)
             got, lp = tokens.tolist(), logprobs.tolist()
             if min(got) < 0:
+                _check_device(device)
                 raise FloatingPointError("generate: a row of logits has no finite value")
             going = []
             for row, s in enumerate(alive):
@@ -135,9 +136,18 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
             if len(going) < len(alive):
                 tokens = tokens[torch.tensor(going, device=device)]
                 alive = [alive[r] for r in going]
+        _check_device(device)
     finally:
         trainer.store.grads_enabled = True
     return out
+
+
+def _check_device(device: torch.device) -> None:
+    """Raise if a kernel gave up or left something out (a wait, a page, a token): the answers would look like any others."""
+    if device.type == "cuda":
+        from ..ops import check_device_errors
+
+        check_device_errors()
 
 
 class _Cached:

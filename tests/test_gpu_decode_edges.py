@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _no_errors, _ops, _problem
+from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _model, _no_errors, _ops, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,31 @@ def test_paged_attention_refuses_caps_and_scales_that_fp32_cannot_hold():
         with pytest.raises(RuntimeError):
             _ops().paged_attention(q, kv, table, n, **kw)
     _no_errors()
+
+
+# ---------------------------------------------------------------------------------------------- answers
+def _trainer(kind="qwen3", **kw):
+    from surogate_b200.runtime.trainer import Trainer, TrainerConfig
+
+    tr = Trainer(TrainerConfig(**{**dict(model=_model(kind), batch_size=2, seq_len=256), **kw}), device=torch.device("cuda:0"))
+    tr.init_weights(seed=0)
+    return tr
+
+
+def test_generate_raises_what_its_kernels_report(monkeypatch):
+    """A page number outside the cache, which the kernels leave out and report, ends ``generate`` with that error, and none is left for the next call."""
+    tr, table = _trainer(), _ops().PagedKVCache.table
+    kw = dict(max_new_tokens=3, temperature=0.0)
+    want = tr.generate([[5, 6, 7]], **kw)[0][0].tokens
+
+    def wrong(self, seqs, tokens=0):
+        t = table(self, seqs, tokens)
+        t[0, 0] = self.num_pages
+        return t
+
+    with monkeypatch.context() as m:
+        m.setattr(_ops().PagedKVCache, "table", wrong)
+        with pytest.raises(RuntimeError, match="paged key/value cache"):
+            tr.generate([[5, 6, 7]], **kw)
+    _no_errors()
+    assert tr.store.grads_enabled and tr.generate([[5, 6, 7]], **kw)[0][0].tokens == want
