@@ -84,6 +84,9 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
     prompts = [[int(t) for t in p] for p in prompts]
     if any(not p for p in prompts):
         raise ValueError("generate: a prompt needs at least one token")
+    vocab = trainer.model.vocab_size
+    if any(not 0 <= t < vocab for p in prompts for t in p):
+        raise ValueError(f"generate: a prompt has a token outside the vocabulary of {vocab}")
     if n < 1 or max_new_tokens < 0 or prompt_rows < 1:
         raise ValueError("generate: n and prompt_rows must be positive, max_new_tokens not negative")
     if trainer.world > 1 and (trainer.cfg.zero_level >= 3 or trainer.cfg.ep_size > 1):

@@ -158,3 +158,13 @@ def test_generate_raises_what_its_kernels_report(monkeypatch):
             tr.generate([[5, 6, 7]], **kw)
     _no_errors()
     assert tr.store.grads_enabled and tr.generate([[5, 6, 7]], **kw)[0][0].tokens == want
+
+
+def test_generate_refuses_prompt_tokens_outside_the_vocabulary_before_any_launch():
+    tr = _trainer()
+    for bad in (-1, 4096):
+        before = _ops().ext().launch_count()
+        with pytest.raises(ValueError):
+            tr.generate([[5, bad]], max_new_tokens=2)
+        assert _ops().ext().launch_count() == before
+    _no_errors()
