@@ -8,6 +8,8 @@ Parity: csrc/src/recipes/recipe.h:62-318, recipe_factory.cpp.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 
 class Recipe:
     name = "base"
@@ -26,6 +28,11 @@ class Recipe:
 
     def end_step(self) -> None:
         pass
+
+    @contextmanager
+    def inference(self):
+        """Around passes that belong to no training step: nothing that they measure of activations or weights reaches the training's state."""
+        yield
 
     def on_weights_updated(self, store) -> None:
         pass

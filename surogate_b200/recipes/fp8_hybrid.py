@@ -21,7 +21,7 @@ recipes/fp8_hybrid/kernels/{quant,delayed_scaling}.cu.
 from __future__ import annotations
 
 import os
-
+from contextlib import contextmanager
 from typing import Dict, Tuple
 
 import torch
@@ -61,6 +61,7 @@ class FP8HybridRecipe(GroupedFp8Mixin, Recipe):
         self.scale = torch.ones(Q, dtype=torch.float32, device=device)
         self.scale_inv = torch.ones(Q, dtype=torch.float32, device=device)
         self.have_history = False
+        self.apart = False           # inside inference()
         self.weight_cache: Dict[Tuple[int, str], Fp8Tensor] = {}
         self.expert_weight_cache: Dict[Tuple[int, str], tuple] = {}
         self.weight_version = 0
@@ -74,6 +75,8 @@ class FP8HybridRecipe(GroupedFp8Mixin, Recipe):
         x = x.contiguous()
         if not self.have_history:
             am = self.amax_cur[q:q + 1]
+            if self.apart:
+                am.zero_()           # (the micro-batches of a step share one abs-max; passes outside of one do not)
             ext.amax(x, am)
             # scale = fmax / amax (amax > 0), computed on the device: no host sync
             s = torch.where(am > 0, self.fmax[q:q + 1] / am / (2.0 ** self.margin), torch.ones_like(am))
@@ -96,6 +99,22 @@ class FP8HybridRecipe(GroupedFp8Mixin, Recipe):
         self.amax_cur.zero_()
         self.have_history = True
         self.grouped_end_step()
+
+    @contextmanager
+    def inference(self):
+        """Delayed scales are used but not recorded; without a history each tensor's own abs-max gives its scale.  Copies of weights made
+        meanwhile are dropped: the next step's own must record theirs."""
+        state = (self.amax_cur, self.scale, self.scale_inv)
+        kept, weights = [t.clone() for t in state], dict(self.weight_cache)
+        self.apart = True
+        try:
+            with self.grouped_inference():
+                yield
+        finally:
+            self.apart = False
+            for t, k in zip(state, kept):
+                t.copy_(k)
+            self.weight_cache = weights
 
     def on_weights_updated(self, store) -> None:
         self.weight_cache.clear()

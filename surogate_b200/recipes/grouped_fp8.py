@@ -17,6 +17,8 @@ grouped expert GEMMs).
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import torch
 
 E4M3_MAX = 448.0
@@ -59,6 +61,21 @@ class GroupedFp8Mixin:
         st["inv"].copy_(1.0 / st["scale"])
         st["amax"].zero_()
         st["have"] = True
+
+    @contextmanager
+    def grouped_inference(self):
+        """The experts' share of ``Recipe.inference``."""
+        st, weights = self.__dict__.get("_g_state"), dict(self.expert_weight_cache)
+        kept = {k: v.clone() if torch.is_tensor(v) else v for k, v in (st or {}).items()}
+        try:
+            yield
+        finally:
+            if st is None:
+                self.__dict__.pop("_g_state", None)
+            else:
+                for k in ("scale", "inv", "amax"):
+                    st[k].copy_(kept[k])
+            self.expert_weight_cache = weights
 
     def _gq(self, ext, x: torch.Tensor, e5m2: bool, used, q: int):
         """(fp8 data, de-scale) of ``x``.  With a scale from the previous step: one pass that quantises and records the abs-max for the

@@ -21,6 +21,7 @@ Parity: csrc/src/recipes/nvfp4/nvfp4_recipe.cpp:629-1131, recipes/nvfp4/kernels/
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -67,6 +68,16 @@ class NVFP4Recipe(GroupedFp8Mixin, Recipe):
 
     def end_step(self) -> None:
         self.grouped_end_step()
+
+    @contextmanager
+    def inference(self):
+        """The step's count of stochastic roundings goes on where it was; the quantised weights, which depend on nothing else, are kept."""
+        calls = self.calls
+        try:
+            with self.grouped_inference():
+                yield
+        finally:
+            self.calls = calls
 
     def on_weights_updated(self, store) -> None:
         self.weight_cache.clear()

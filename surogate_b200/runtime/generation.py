@@ -3,7 +3,9 @@
 ``generate`` (public as ``Trainer.generate``) runs the prompts once, keeps their keys and values in a paged cache (``ops.PagedKVCache``) and
 then one token of every unfinished completion per step: embed, attend over the pages, draw (``ops.sample_tokens``).  Completions of one prompt
 share its pages; only the last, partly filled one is copied when they part.  The uniform numbers of step ``i`` are row ``i`` of one generator's
-stream, one for each completion, so a completion does not depend on when its neighbours end.
+stream, one for each completion, so a completion's draws do not depend on when its neighbours end.  (Its logits may, within their rounding: products over
+other numbers of rows add up in another order, and a recipe with one scale for a whole tensor takes it from all rows.)  What recipes
+measure here does not reach the scales of training.
 
 Models whose layers mix positions by other means than attention (short convolutions, state-space and delta-rule mixers, attention that keeps
 values of other layers) have no such cache: for them every step runs the whole prefix again, with the same draws.
@@ -113,32 +115,33 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
         raise ValueError("generate: this model has no key/value cache")
     trainer.store.grads_enabled = False
     try:
-        run = _Cached(trainer, cache, prompts, n, prompt_rows) if cache is not None else _Uncached(trainer, prompts, n, prompt_rows)
-        alive = list(range(len(prompts) * n))                          # completion c of prompt i is number i * n + c
-        tokens = None
-        for step in range(max_new_tokens):
-            u = torch.rand(len(prompts) * n, generator=gen, device=device)
-            logits = run.first() if step == 0 else run.next(alive, tokens)
-            tokens, logprobs = sample_tokens(logits, u[torch.tensor(alive, device=device)] if len(alive) < len(u) else u, **draw)
-            got, lp = tokens.tolist(), logprobs.tolist()
-            if min(got) < 0:
-                _check_device(device)
-                raise FloatingPointError("generate: a row of logits has no finite value")
-            going = []
-            for row, s in enumerate(alive):
-                c = out[s // n][s % n]
-                c.tokens.append(got[row])
-                c.logprobs.append(lp[row])
-                if eos_id is not None and got[row] == eos_id:
-                    c.finish_reason = "stop"
-                    run.drop(s)
-                else:
-                    going.append(row)
-            if not going:
-                break
-            if len(going) < len(alive):
-                tokens = tokens[torch.tensor(going, device=device)]
-                alive = [alive[r] for r in going]
+        with trainer.recipe.inference():
+            run = _Cached(trainer, cache, prompts, n, prompt_rows) if cache is not None else _Uncached(trainer, prompts, n, prompt_rows)
+            alive = list(range(len(prompts) * n))                          # completion c of prompt i is number i * n + c
+            tokens = None
+            for step in range(max_new_tokens):
+                u = torch.rand(len(prompts) * n, generator=gen, device=device)
+                logits = run.first() if step == 0 else run.next(alive, tokens)
+                tokens, logprobs = sample_tokens(logits, u[torch.tensor(alive, device=device)] if len(alive) < len(u) else u, **draw)
+                got, lp = tokens.tolist(), logprobs.tolist()
+                if min(got) < 0:
+                    _check_device(device)
+                    raise FloatingPointError("generate: a row of logits has no finite value")
+                going = []
+                for row, s in enumerate(alive):
+                    c = out[s // n][s % n]
+                    c.tokens.append(got[row])
+                    c.logprobs.append(lp[row])
+                    if eos_id is not None and got[row] == eos_id:
+                        c.finish_reason = "stop"
+                        run.drop(s)
+                    else:
+                        going.append(row)
+                if not going:
+                    break
+                if len(going) < len(alive):
+                    tokens = tokens[torch.tensor(going, device=device)]
+                    alive = [alive[r] for r in going]
         _check_device(device)
     finally:
         trainer.store.grads_enabled = True

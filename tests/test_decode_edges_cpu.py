@@ -27,3 +27,39 @@ def test_generate_refuses_prompt_tokens_outside_the_vocabulary(tmp_path):
         with pytest.raises(ValueError, match="vocabulary"):
             tr.generate([[1, 2], [3, bad, 4]], max_new_tokens=2)
     assert len(tr.generate([[0, V - 1]], max_new_tokens=2)[0][0].tokens) == 2 and tr.store.grads_enabled
+
+
+def test_recipes_keep_their_state_over_inference():
+    """What passes between training steps measure, and the copies of weights that they make, are gone afterwards, after an error too."""
+    from types import SimpleNamespace
+
+    from surogate_b200.recipes.base import Recipe
+    from surogate_b200.recipes.fp8_hybrid import FP8HybridRecipe
+
+    with Recipe().inference():
+        pass
+    for grouped in (False, True):
+        r = FP8HybridRecipe(SimpleNamespace(n_layers=2), torch.device("cpu"))
+        r.amax_cur.uniform_(), r.scale.uniform_(), r.scale_inv.uniform_()
+        r.weight_cache[(0, "qkv")] = "kept"
+        if grouped:
+            r._gstate(torch.device("cpu"))["amax"].uniform_()
+            r.expert_weight_cache[(1, "experts_down")] = "kept too"
+        kept = [t.clone() for t in (r.amax_cur, r.scale, r.scale_inv)]
+        same = [r.amax_cur, r.scale, r.scale_inv]
+        g = {k: v.clone() for k, v in r._gstate(torch.device("cpu")).items() if torch.is_tensor(v)} if grouped else None
+        try:
+            with r.inference():
+                assert r.apart
+                for t in same:
+                    t.add_(1.0)
+                r.weight_cache[(0, "out")] = r.expert_weight_cache[(0, "experts_down")] = "new"
+                st = r._gstate(torch.device("cpu"))
+                for k in ("scale", "inv", "amax"):
+                    st[k].add_(2.0)
+                raise KeyError
+        except KeyError:
+            pass
+        assert not r.apart and all(a is b and torch.equal(a, k) for a, b, k in zip((r.amax_cur, r.scale, r.scale_inv), same, kept))
+        assert r.weight_cache == {(0, "qkv"): "kept"} and r.expert_weight_cache == ({(1, "experts_down"): "kept too"} if grouped else {})
+        assert all(torch.equal(r._g_state[k], v) for k, v in g.items()) if grouped else not hasattr(r, "_g_state")

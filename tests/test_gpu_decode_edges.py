@@ -168,3 +168,29 @@ def test_generate_refuses_prompt_tokens_outside_the_vocabulary_before_any_launch
             tr.generate([[5, bad]], max_new_tokens=2)
         assert _ops().ext().launch_count() == before
     _no_errors()
+
+
+@pytest.mark.parametrize("kind,recipe", [("qwen3", "fp8_hybrid"), ("moe", "fp8_hybrid"), ("qwen3", "nvfp4"), ("moe", "nvfp4")])
+def test_generate_leaves_the_recipes_scales_alone(kind, recipe):
+    """Answers before the first training step, between steps, and twice with one seed: the recipe's scales, abs-max values and copies of weights are what they
+    were, bit for bit, and the same call gives the same answers."""
+    import numpy as np
+
+    tr = _trainer(kind, recipe=recipe)
+    r = tr.recipe
+    tensors = lambda: {n: getattr(r, n).clone() for n in ("amax_hist", "amax_cur", "scale", "scale_inv") if hasattr(r, n)}  # noqa: E731
+    grouped = lambda: {k: v.clone() for k, v in (r.__dict__.get("_g_state") or {}).items() if torch.is_tensor(v)}  # noqa: E731
+    g = np.random.default_rng(0)
+    for step in range(3):
+        before, gb, calls, copies = tensors(), grouped(), getattr(r, "calls", 0), set(r.expert_weight_cache)
+        small = tr.generate([[5], list(range(140))], n=2, max_new_tokens=6, top_k=50, seed=1)
+        tr.generate([list(range(900, 930))], max_new_tokens=3, seed=9)
+        again = tr.generate([[5], list(range(140))], n=2, max_new_tokens=6, top_k=50, seed=1)
+        if kind == "qwen3":                                              # (experts add up their tokens in no fixed order)
+            assert [(c.tokens, c.logprobs) for cs in small for c in cs] == [(c.tokens, c.logprobs) for cs in again for c in cs]
+        after, ga = tensors(), grouped()
+        assert all(torch.equal(before[k], after[k]) for k in before) and set(gb) == set(ga) and all(torch.equal(gb[k], ga[k]) for k in gb)
+        assert getattr(r, "calls", 0) == calls and set(r.expert_weight_cache) == copies
+        tokens = g.integers(0, 4096, (2, 257)).astype(np.int32)
+        tr.step(tokens[:, :-1], tokens[:, 1:])
+    _no_errors()
