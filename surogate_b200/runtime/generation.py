@@ -93,6 +93,8 @@ def generate(trainer, prompts: Sequence[Sequence[int]], *, n: int = 1, max_new_t
         raise ValueError("generate: n and prompt_rows must be positive, max_new_tokens not negative")
     if trainer.world > 1 and (trainer.cfg.zero_level >= 3 or trainer.cfg.ep_size > 1):
         raise NotImplementedError("generate: weights spread over ranks (ZeRO-3, expert parallelism) would need every rank to take the same steps")
+    if trainer._visual is not None:
+        raise NotImplementedError("generate answers text: clear the visual inputs first (set_visual_inputs without arguments)")
     out = [[Completion() for _ in range(n)] for _ in prompts]
     if not prompts or max_new_tokens == 0:
         return out

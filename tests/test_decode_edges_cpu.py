@@ -63,3 +63,13 @@ def test_recipes_keep_their_state_over_inference():
         assert not r.apart and all(a is b and torch.equal(a, k) for a, b, k in zip((r.amax_cur, r.scale, r.scale_inv), same, kept))
         assert r.weight_cache == {(0, "qkv"): "kept"} and r.expert_weight_cache == ({(1, "experts_down"): "kept too"} if grouped else {})
         assert all(torch.equal(r._g_state[k], v) for k, v in g.items()) if grouped else not hasattr(r, "_g_state")
+
+
+def test_generate_refuses_visual_inputs(tmp_path):
+    """They were left out without a word."""
+    tr = _trainer(tmp_path, "qwen3")
+    tr.set_visual_inputs(mrope_position_ids=torch.zeros(3, 1, 2, dtype=torch.int32))
+    with pytest.raises(NotImplementedError, match="visual"):
+        tr.generate([[1, 2]], max_new_tokens=2)
+    tr.set_visual_inputs()
+    assert len(tr.generate([[1, 2]], max_new_tokens=2)[0][0].tokens) == 2
