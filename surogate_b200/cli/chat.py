@@ -14,7 +14,7 @@ from typing import List, Optional
 def generate(trainer, tokenizer, prompt_ids: List[int], max_new_tokens: int = 64, temperature: float = 0.0, seed: int = 0, eos_id: Optional[int] = None, top_k: int = 0,
              top_p: float = 1.0, min_p: float = 0.0) -> List[int]:
     eos = tokenizer.eos_token_id if eos_id is None and tokenizer is not None else eos_id
-    return trainer.generate([prompt_ids], max_new_tokens=max_new_tokens, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, seed=seed, eos_id=eos)[0][0].tokens
+    return trainer.generate([prompt_ids], max_new_tokens=max(0, max_new_tokens), temperature=temperature if temperature > 0 else 0.0, top_k=top_k, top_p=top_p, min_p=min_p, seed=seed, eos_id=eos)[0][0].tokens
 
 
 def main(argv, command: str = "chat") -> int:

@@ -73,3 +73,13 @@ def test_generate_refuses_visual_inputs(tmp_path):
         tr.generate([[1, 2]], max_new_tokens=2)
     tr.set_visual_inputs()
     assert len(tr.generate([[1, 2]], max_new_tokens=2)[0][0].tokens) == 2
+
+
+def test_chat_without_a_positive_temperature_is_greedy(tmp_path):
+    """As the helper always was: temperatures that are not above 0 are greedy, no room means no tokens."""
+    from surogate_b200.cli.chat import generate
+
+    tr = _trainer(tmp_path, "qwen3")
+    want = generate(tr, None, [1, 2, 3], max_new_tokens=4)
+    assert len(want) == 4 and all(generate(tr, None, [1, 2, 3], max_new_tokens=4, temperature=t) == want for t in (-1.0, math.nan))
+    assert generate(tr, None, [1, 2, 3], max_new_tokens=-1) == []
