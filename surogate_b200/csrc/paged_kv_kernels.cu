@@ -226,12 +226,13 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_pages_kernel(KvCopy p, i
     const int from = p.src[pair], to = p.dst[pair];
     const bool outside = from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages;
     int clash = 0;
-    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) clash |= j != pair && (p.src[j] == to || p.dst[j] == to);
+    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) clash |= j != pair && (p.dst[j] == to || (p.src[j] == to && from != to));
     clash = __syncthreads_or(clash);
     if (outside || clash) {
         if (threadIdx.x == 0) atomicExch(p.error_flag, outside ? kErrBadPage : kErrPageOverlap);
         return;
     }
+    if (from == to) return;                                        // stays as it is, and others may read it
     const int part = static_cast<int>(blockIdx.x) >= pieces0;
     const int64_t off = static_cast<int64_t>(part ? blockIdx.x - pieces0 : blockIdx.x) * kCopyPiece;
     const int64_t left = p.page_bytes[part] - off;

@@ -136,7 +136,8 @@ def _check_pairs(src: Sequence[int], dst: Sequence[int], pages: int) -> None:
 def kv_copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, scales: Optional[torch.Tensor] = None) -> None:
     """Copy page ``src[i]`` to page ``dst[i]`` in every layer of ``kv [layers, pages, 2, kv heads, page size, head size]``, in place, and of
     ``scales [layers, pages, 2, kv heads, page size]`` with them.  ``src``, ``dst`` int32 on the cache's device.  The pairs have no order: no
-    page may be a target twice, or a target and another pair's source; pairs that break this are left out and reported."""
+    page may be a target twice, or a target and another pair's source (a page copied onto itself is no target for the others); pairs that break
+    this are left out and reported."""
     if kv.is_cuda:
         return _kernels().kv_copy_pages(kv, src, dst, scales)
     if kv.dim() != 6 or kv.shape[2] != 2:

@@ -132,6 +132,23 @@ def test_paged_attention_refuses_caps_and_scales_that_fp32_cannot_hold():
     _no_errors()
 
 
+# ---------------------------------------------------------------------------------------------- pages
+def test_kv_copy_pages_onto_themselves():
+    """A pair of one page leaves it as it is, and other pairs may read it; what breaks the rules does so here as on the CPU."""
+    kv = torch.randn(2, 8, 2, 2, 16, 64, device=DEV).bfloat16()
+    for src, dst in [((1, 1), (1, 4)), ((2, 1, 2, 2), (3, 4, 2, 5)), ((1, 0), (1, 1)), ((0, 1), (1, 1)), ((6,), (6,)), ((1, 1), (1, 1))]:
+        pairs = [torch.tensor(x, dtype=torch.int32) for x in (src, dst)]
+        got, want = kv.clone(), kv.cpu()
+        _ops().kv_copy_pages(got, *(x.to(DEV) for x in pairs))
+        try:
+            _ops().kv_copy_pages(want, *pairs)
+            word = 0
+        except RuntimeError:
+            word = 9
+        torch.cuda.synchronize()
+        assert int(_ops().ext().read_error_flag(True)) == word and torch.equal(got.cpu(), want), (src, dst)
+
+
 # ---------------------------------------------------------------------------------------------- answers
 def _trainer(kind="qwen3", **kw):
     from surogate_b200.runtime.trainer import Trainer, TrainerConfig
