@@ -126,7 +126,7 @@ void kv_copy_pages(const Tensor& kv, const Tensor& src, const Tensor& dst, const
     const Tensor* part[2] = {&kv, given(scales) ? &*scales : nullptr};
     for (int i = 0; i < 2 && part[i]; ++i) {
         const Tensor& t = *part[i];
-        if (i) TORCH_CHECK(t.device() == kv.device() && t.dim() == 5 && t.size(0) == kv.size(0) && t.size(1) == kv.size(1), "scales must be [layers, pages, 2, kv heads, page size] on the cache's device");
+        if (i) TORCH_CHECK(t.device() == kv.device() && t.scalar_type() == at::kFloat && t.sizes() == kv.sizes().slice(0, 5), "scales must be fp32 [layers, pages, 2, kv heads, page size] on the cache's device");
         const int64_t es = t.element_size(), bytes = t.numel() ? t.numel() / (t.size(0) * t.size(1)) * es : 0;
         int64_t inner = 1;
         bool whole = true;

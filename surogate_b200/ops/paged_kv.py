@@ -144,6 +144,8 @@ def kv_copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, scales
         raise RuntimeError("kv_copy_pages: kv must be [layers, pages, 2, kv heads, page size, head size]")
     if kv.dtype == torch.float8_e4m3fn and scales is None:
         raise RuntimeError("kv_copy_pages: the scales of a float8_e4m3fn cache are copied with its pages")
+    if scales is not None and (scales.shape != kv.shape[:5] or scales.dtype != torch.float32):
+        raise RuntimeError("kv_copy_pages: scales must be fp32 [layers, pages, 2, kv heads, page size]")
     kv_copy_pages_reference(kv, src, dst, scales)
 
 

@@ -83,3 +83,13 @@ def test_chat_without_a_positive_temperature_is_greedy(tmp_path):
     want = generate(tr, None, [1, 2, 3], max_new_tokens=4)
     assert len(want) == 4 and all(generate(tr, None, [1, 2, 3], max_new_tokens=4, temperature=t) == want for t in (-1.0, math.nan))
     assert generate(tr, None, [1, 2, 3], max_new_tokens=-1) == []
+
+
+def test_copying_pages_refuses_scales_of_other_caches():
+    kv = torch.zeros(2, 4, 2, 1, 16, 8)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    good = torch.ones(kv.shape[:5])
+    for bad in (good.double(), good[:1], good[:, :3], good[:, :, :1], good.expand(2, 4, 2, 2, 16), good[..., :8], good[0]):
+        with pytest.raises(RuntimeError):
+            ops.kv_copy_pages(kv.to(torch.float8_e4m3fn), i32(0), i32(1), bad)
+    ops.kv_copy_pages(kv.to(torch.float8_e4m3fn), i32(0), i32(1), good)

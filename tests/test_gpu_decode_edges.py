@@ -149,6 +149,17 @@ def test_kv_copy_pages_onto_themselves():
         assert int(_ops().ext().read_error_flag(True)) == word and torch.equal(got.cpu(), want), (src, dst)
 
 
+def test_kv_copy_pages_refuses_scales_of_other_caches():
+    kv = torch.zeros(2, 4, 2, 1, 16, 64, device=DEV).to(E4M3)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    good = torch.ones(kv.shape[:5], device=DEV)
+    for bad in (good.double(), good.half(), good[:1], good[:, :3], good[:, :, :1].contiguous(), good.expand(2, 4, 2, 2, 16).contiguous(), good[..., :8].contiguous(), good[0], good.cpu()):
+        with pytest.raises(RuntimeError):
+            _ops().kv_copy_pages(kv, i32(0), i32(1), bad)
+    _ops().kv_copy_pages(kv, i32(0), i32(1), good)
+    _no_errors()
+
+
 # ---------------------------------------------------------------------------------------------- answers
 def _trainer(kind="qwen3", **kw):
     from surogate_b200.runtime.trainer import Trainer, TrainerConfig
