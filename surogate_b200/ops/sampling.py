@@ -31,7 +31,7 @@ def sample_tokens_reference(logits: torch.Tensor, u: torch.Tensor, temperature: 
         if not T > 0:
             i = int((l == top).nonzero()[0])
         else:
-            w = torch.where(d == 0, torch.ones_like(d), torch.exp(d / T))
+            w = torch.where(d == 0, torch.ones_like(d), torch.where(d == -float("inf"), torch.zeros_like(d), torch.exp(d / T)))   # (T may be infinite)
             order = torch.sort(l, descending=True, stable=True).indices          # equal logits in the order of their indices
             s = w[order]
             keep = s >= min(m, 1.0) if m > 0 else torch.ones_like(s, dtype=torch.bool)

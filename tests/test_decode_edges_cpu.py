@@ -93,3 +93,14 @@ def test_copying_pages_refuses_scales_of_other_caches():
         with pytest.raises(RuntimeError):
             ops.kv_copy_pages(kv.to(torch.float8_e4m3fn), i32(0), i32(1), bad)
     ops.kv_copy_pages(kv.to(torch.float8_e4m3fn), i32(0), i32(1), good)
+
+
+def test_sampling_at_a_temperature_without_end():
+    """All tokens weigh the same, those of -inf and NaN nothing; of infinite logits only those count."""
+    x = torch.tensor([[0.0, -math.inf, 3.0, math.nan, 1.0]]).expand(6, 5)
+    u = torch.tensor([0.0, 0.3, 0.34, 0.66, 0.67, 0.999])
+    for t in (math.inf, torch.full((6,), math.inf)):
+        tok, lp = ops.sample_tokens(x, u, temperature=t)
+        assert tok.tolist() == [0, 0, 2, 2, 4, 4]
+        assert torch.allclose(lp, torch.log_softmax(torch.tensor([0.0, -math.inf, 3.0, -math.inf, 1.0]), 0)[tok.long()])
+    assert ops.sample_tokens(torch.tensor([[1.0, math.inf, math.inf]]), torch.tensor([0.6]), temperature=math.inf)[0].tolist() == [2]

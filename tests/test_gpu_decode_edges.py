@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _model, _no_errors, _ops, _problem
+from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _check_sample, _model, _no_errors, _ops, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -158,6 +158,17 @@ def test_kv_copy_pages_refuses_scales_of_other_caches():
             _ops().kv_copy_pages(kv, i32(0), i32(1), bad)
     _ops().kv_copy_pages(kv, i32(0), i32(1), good)
     _no_errors()
+
+
+# ---------------------------------------------------------------------------------------------- drawing
+@pytest.mark.parametrize("V", [5, 700, 40000])
+def test_sample_tokens_at_a_temperature_without_end(V):
+    """All tokens weigh the same, those of -inf and NaN nothing; of infinite logits only those count."""
+    x = torch.randn(6, V, generator=torch.Generator().manual_seed(V)).to(DEV)
+    x[:, 1::3], x[2, 0], x[5, 2:] = -math.inf, math.nan, math.inf
+    u = torch.tensor([0.0, 0.3, 0.34, 0.66, 0.67, 0.999], device=DEV)
+    for kw in ({}, dict(top_k=3), dict(top_p=0.4), dict(min_p=0.5)):
+        _check_sample(x, u, temperature=math.inf, **kw)
 
 
 # ---------------------------------------------------------------------------------------------- answers
