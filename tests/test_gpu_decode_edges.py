@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import BF16, DEV, E4M3, FP16, _attention64, _check_attention, _check_sample, _model, _no_errors, _ops, _problem
+from test_gpu_decode import BF16, DEV, E4M3, FP16, FP32, _attention64, _check_attention, _check_sample, _model, _no_errors, _ops, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -107,6 +107,15 @@ def test_paged_attention_of_zero_values():
                 _check_attention(q, kv, table, n, scales=s)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, E4M3])
+@pytest.mark.parametrize("Hq,Hkv", [(18, 1), (40, 2)])
+def test_paged_attention_of_long_rows_with_heads_of_256_in_groups(dtype, Hq, Hkv):
+    """More than eight query heads a key head of 256 elements: groups of eight, each over all of a row's pieces."""
+    q, kv, table, n, s = _problem(4, Hq, Hkv, 256, 16, [5003, 0, 33, 9001], dtype, seed=Hq)
+    _check_attention(q, kv, table, n, scales=s)
+    _check_attention(q, kv, table, n, scales=s, window=3000, softcap=30.0, sinks=torch.linspace(-3.0, 3.0, Hq, device=DEV))
+
+
 # ---------------------------------------------------------------------------------------------- attention: caps of the scores
 @pytest.mark.parametrize("cap", [1e-3, 0.5, 5.0, 30.0, 50.0, 1e3, 1e4, 1e6, 1e12])
 @pytest.mark.parametrize("spread", [1e-3, 0.05, 2.0, 30.0])
@@ -171,6 +180,85 @@ def test_sample_tokens_at_a_temperature_without_end(V):
         _check_sample(x, u, temperature=math.inf, **kw)
 
 
+# ---------------------------------------------------------------------------------------------- graphs
+def _captured(f):
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = f()
+    return graph, out
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_append_and_copy_in_a_graph(dtype):
+    """A replay writes what its inputs hold at its time: other keys, starts, counts and pairs of pages than at the capture; nothing else is touched."""
+    g = torch.Generator().manual_seed(0)
+    L, n, H, P, D, B, T = 2, 20, 2, 16, 64, 3, 9
+    kv = torch.randn(L, n, 2, H, P, D, generator=g).to(DEV).to(dtype)
+    s = torch.rand(L, n, 2, H, P, generator=g).to(DEV) if dtype == E4M3 else None
+    part = lambda x, layer: None if x is None else x[layer]  # noqa: E731
+    table = torch.randperm(n, generator=g)[:6].view(3, 2).to(torch.int32).to(DEV)
+    k, v = (torch.randn(B, T, H, D, generator=g).to(DEV).bfloat16() for _ in range(2))
+    start, count = torch.zeros(B, dtype=torch.int32, device=DEV), torch.full((B,), T, dtype=torch.int32, device=DEV)
+    rest = [p for p in range(n) if p not in table.flatten().tolist()]
+    src, dst = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (rest[:3], rest[3:6]))
+
+    def step():
+        _ops().kv_append(kv[1], k, v, table, start, count, part(s, 1))
+        _ops().kv_copy_pages(kv, src, dst, s)
+
+    graph, _ = _captured(step)
+    for i in range(3):
+        k.copy_(torch.randn(k.shape, generator=g)), v.copy_(torch.randn(v.shape, generator=g))
+        start.copy_(torch.tensor([0, 5 + i, 20], dtype=torch.int32)), count.copy_(torch.tensor([T, i, 0], dtype=torch.int32))
+        dst.copy_(torch.tensor(rest[3 + i:6 + i], dtype=torch.int32))
+        kept, ks = kv.clone(), None if s is None else s.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, gs = kv.clone(), None if s is None else s.clone()
+        kv.copy_(kept)
+        if s is not None:
+            s.copy_(ks)
+        step()
+        assert torch.equal(got.view(torch.uint8), kv.view(torch.uint8)) and (s is None or torch.equal(gs, s))
+        assert not torch.equal(got.view(torch.uint8), kept.view(torch.uint8))
+    _no_errors()
+
+
+def test_a_decode_step_in_graphs_of_one_memory_pool():
+    """Append, attention and draw captured together, twice, in one pool: the two replayed in turn give what eager calls give, whose workspaces are their own."""
+    g = torch.Generator().manual_seed(3)
+    B, Hq, H, D, P, V = 4, 8, 2, 64, 16, 5000
+    kv = torch.zeros(200 * B, 2, H, P, D, device=DEV).bfloat16()
+    table = torch.randperm(200 * B, generator=g).view(B, 200).to(torch.int32).to(DEV)
+    head = torch.randn(Hq * D, V, generator=g).to(DEV).bfloat16() * 0.05
+    _ops().kv_append(kv, *(torch.randn(B, 2990, H, D, generator=g).to(DEV).bfloat16() for _ in range(2)), table, torch.zeros(B, dtype=torch.int32, device=DEV))
+    ins = [[torch.zeros(B, 1, H, D, device=DEV).bfloat16(), torch.zeros(B, 1, H, D, device=DEV).bfloat16(), torch.zeros(B, Hq, D, device=DEV).bfloat16(),
+            torch.zeros(B, dtype=torch.int32, device=DEV), torch.zeros(B, device=DEV)] for _ in range(2)]
+
+    def step(k, v, q, start, u):
+        _ops().kv_append(kv, k, v, table, start)
+        att = _ops().paged_attention(q, kv, table, start + 1)
+        return (att,) + _ops().sample_tokens(att.reshape(B, -1) @ head, u, top_p=0.9, top_k=200)
+
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for x in ins:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, pool=pool):
+            graphs.append((graph, step(*x)))
+    for t in range(6):
+        x, (graph, out) = ins[t % 2], graphs[t % 2]
+        for y in x[:3] + x[4:]:
+            y.copy_(torch.randn(y.shape, generator=g).abs() % 1 if y.dtype == FP32 else torch.randn(y.shape, generator=g))
+        x[3].copy_(torch.tensor([2990 + t, 10 + t, 1500, t], dtype=torch.int32))
+        graph.replay()
+        got = [y.clone() for y in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step(*x)))
+    torch.cuda.synchronize()
+    _no_errors()
+
+
 # ---------------------------------------------------------------------------------------------- answers
 def _trainer(kind="qwen3", **kw):
     from surogate_b200.runtime.trainer import Trainer, TrainerConfig
@@ -232,4 +320,31 @@ def test_generate_leaves_the_recipes_scales_alone(kind, recipe):
         assert getattr(r, "calls", 0) == calls and set(r.expert_weight_cache) == copies
         tokens = g.integers(0, 4096, (2, 257)).astype(np.int32)
         tr.step(tokens[:, :-1], tokens[:, 1:])
+    _no_errors()
+
+
+@pytest.mark.parametrize("recipe,cache_dtype,mean,most", [("fp8_hybrid", None, 0.1, 0.3), ("nvfp4", None, 0.2, 1.2), ("bf16", E4M3, 0.06, 0.2)])
+def test_generate_in_low_precision_agrees_with_scoring(recipe, cache_dtype, mean, most):
+    """Log-probabilities of the answers against ``token_logprobs`` of the finished rows, whose tensors are quantised by other scales.  Rounding to e4m3 is 0.026
+    (rms) of an element, so two passes differ by 0.037 in each of the eight products of two layers: 0.1 of the hidden state, 0.05 on logits of spread
+    0.5, at most twice that in the mean and six times over all.  E2m1 in blocks rounds by 0.1: four times as much.  An e4m3 cache errs by 0.026 in
+    keys (of the scores, whose spread is 1) and in values: 0.06 of the hidden state after two layers, 0.03 on the logits.  The same tokens behind
+    other prompts are further away than the mean's bound, so wrong places, pages or scales would be."""
+    import numpy as np
+
+    tr = _trainer(recipe=recipe, batch_size=4)
+    g = np.random.default_rng(0)
+    prompts = [g.integers(0, 4096, n).tolist() for n in (100, 128, 213, 129)]
+    outs = tr.generate(prompts, max_new_tokens=40, seed=3, page_size=32, cache_dtype=cache_dtype)
+
+    def errors(prompts):
+        rows = np.zeros((4, 256), np.int32)
+        for i, p in enumerate(prompts):
+            rows[i, :len(p) + 40] = p + outs[i][0].tokens
+        lp = tr.token_logprobs(rows, np.roll(rows, -1, axis=1)).cpu()
+        return torch.stack([(lp[i, len(p) - 1:len(p) + 39] - torch.tensor(outs[i][0].logprobs)).abs() for i, p in enumerate(prompts)])
+
+    err = errors(prompts)
+    assert err.mean() <= mean and err.max() <= most, (err.mean(), err.max())
+    assert errors([[(t + 1) % 4096 for t in p] for p in prompts]).mean(1).min() > mean
     _no_errors()
