@@ -1,6 +1,7 @@
 // Python bindings (pybind11 through torch's extension machinery) for the sm_100a kernels.
 // Tensors are validated here (device, dtype, contiguity, alignment) so that kernels can assume their layout.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -48,7 +49,15 @@ struct ErrorFlags {
     Tensor& current() {
         const size_t d = static_cast<size_t>(at::cuda::current_device());
         if (on.size() <= d) on.resize(d + 1);
-        if (!on[d].defined()) on[d] = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(d)));
+        if (!on[d].defined()) {
+            // Cleared on a stream of its own, and there before any kernel is launched: inside a graph that is being captured the clearing would become
+            // part of it, and a second stream's kernels could come before it.
+            const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+            const auto side = at::cuda::getStreamFromPool(false, static_cast<c10::DeviceIndex>(d));
+            const c10::cuda::CUDAStreamGuard guard(side);
+            on[d] = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(d)));
+            side.synchronize();
+        }
         return on[d];
     }
 } g_error_flags;

@@ -1,6 +1,9 @@
 """The kernels of the answering path where formulas meet the ends of their types: numbers that are not finite, caps of scores, values of zero,
 pages copied onto themselves, calls captured into graphs.  Tolerances as in ``test_gpu_decode``, or stated at the test."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -223,6 +226,30 @@ def test_append_and_copy_in_a_graph(dtype):
         assert torch.equal(got.view(torch.uint8), kv.view(torch.uint8)) and (s is None or torch.equal(gs, s))
         assert not torch.equal(got.view(torch.uint8), kept.view(torch.uint8))
     _no_errors()
+
+
+def test_errors_outlive_the_replay_of_a_graph_that_was_the_first_call():
+    """In a process whose first call of all is captured: the error word is not part of the graph, whose replay would clear it."""
+    code = """if True:
+        import torch
+        from surogate_b200 import ops
+        q, kv = torch.zeros(1, 2, 64, device="cuda").bfloat16(), torch.zeros(2, 2, 1, 16, 64, device="cuda").bfloat16()
+        table, n = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.paged_attention(q, kv, table, n)
+        torch.cuda.synchronize()
+        assert ops.ext().read_error_flag(True) == 0
+        ops.paged_attention(q, kv, table + 2, n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ops.ext().read_error_flag(True) == 8
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ops.ext().read_error_flag(True) == 0 and (out == 0).all()
+    """
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=200)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_a_decode_step_in_graphs_of_one_memory_pool():
