@@ -94,6 +94,26 @@ struct Shared {
     uint32_t b_bin, b_last;
 };
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// e^s for s <= 0, to 2^-22 (the exponential's own error: the rounding of s log2(e) is put right); 0 below -150, and for NaN
+__device__ __forceinline__ float exp_below(float s) {
+    constexpr float k2e = static_cast<float>(kLog2eD), ln2 = static_cast<float>(kLn2D);
+    s = fmaxf(s, -150.f);
+    const float t = __fmul_rn(s, k2e), left = fmaf(s, k2e, -t);
+    const float r = ex2(t);
+    return fmaf(r, left * ln2, r);
+}
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // 16 bytes of logits as fp32
 template <typename T> struct Vec;
 template <> struct Vec<float> {
@@ -118,12 +138,6 @@ template <> struct Vec<__half> {
         for (int i = 0; i < 4; ++i) { const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i])); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
     }
 };
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // One block's part of a row.  Places count its logits from the 16-byte boundary at or before its first one; places that hold none read as -inf.
 template <typename T, bool RESIDENT>
@@ -720,12 +734,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     // (& and not &&: with branches here, the device compiler of CUDA 12.9 gave up the test of k on the path without top_p)
     const bool drawing = temp > 0.f, greedy = !drawing, use_k = drawing & (k > 0) & (k < p.V), use_p = drawing & (top_p < 1.f), use_m = drawing & (min_p > 0.f);
     const bool z_is_mass = drawing & (temp == 1.f) & !use_k & !use_m & !use_p;   // the sum for the log-probability is the mass of all tokens
-    const float k2e = static_cast<float>(kLog2eD);
 
     // The row's part into shared memory, and on the way, for each thread, the largest logit that it meets (NaN never is), the vector that held it first,
-    // and the sum of e^(l - that) over its logits.
+    // and the sum of e^(l - that) over its other logits.  The largest itself stays out of the sum, there and where sums meet, so that the
+    // log-probability of a token that is almost sure, -log(1 + z), keeps the accuracy of what is left.  Weights are 2^(l log2(e) - c) with one rounding of
+    // the exponent; c's own is put right at the end.
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = 0;
-    float best = kLowest, z = 0.f;
+    constexpr float k2e = static_cast<float>(kLog2eD);
+    float best = kLowest, z = 0.f, c = 0.f;
     int best_v = 0;
     constexpr int DEPTH = 5;
     for (int base = threadIdx.x; base < max(row.nvec, kTable); base += kThreads * DEPTH) {
@@ -742,30 +758,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         for (int d = 0; d < DEPTH; ++d) {
             if (base + d * kThreads >= row.nvec) break;
             if (RESIDENT) reinterpret_cast<uint4*>(dyn)[base + d * kThreads] = v[d];
-            float l[N], most;
+            float l[N];
             Vec<T>::get(v[d], l);
-            most = l[0];
 #pragma unroll
-            for (int j = 1; j < N; ++j) most = fmaxf(most, l[j]);
-            if (most > best) {
-                z *= ex2((best - most) * k2e);
+            for (int w = N / 2; w > 0; w /= 2)                     // the largest to l[0], the others behind it (where one is NaN, NaN)
+#pragma unroll
+                for (int j = 0; j < w; ++j) {
+                    const float less = min_or_nan(l[j], l[j + w]);
+                    l[j] = fmaxf(l[j], l[j + w]);
+                    l[j + w] = less;
+                }
+            if (l[0] > best) {
+                const float most = l[0], to = most * k2e;
+                z *= ex2(c - to);
+                c = to;
+                l[0] = best;
                 best = most;
                 best_v = base + d * kThreads;
             }
             if (!z_is_mass) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) z += ex2((l[j] - best) * k2e);
+                for (int j = 0; j < N; ++j) z += ex2(fmaf(l[j], k2e, -c));
             }
         }
     }
+    z = fmaf(z, fmaf(-best, k2e, c) * static_cast<float>(kLn2D), z);
     // The row that comes when this one is done, as far as that can be known, into L2: HBM would be idle while this one is worked on.
     if (RESIDENT && threadIdx.x == 0 && b + ahead < p.B) {
         const uintptr_t from = reinterpret_cast<uintptr_t>(src + ahead * p.row_stride), to = from + static_cast<uintptr_t>(max(0, row.end - row.off)) * sizeof(T);
         const uintptr_t lo = (from + 15) & ~uintptr_t{15}, hi = to & ~uintptr_t{15};
         if (lo < hi) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(lo), "r"(static_cast<uint32_t>(hi - lo)) : "memory");
     }
-    if (!(z >= 0.f) || best == kLowest) {                          // NaN, or infinities among the logits, or nothing above the lowest number: once more, with care
+    bool some = true;                                              // a logit above -inf
+    if (!(z >= 0.f) || best == INFINITY || best == kLowest) {      // NaN, or infinities, or nothing above the lowest number: once more, with care
         z = 0.f;
+        some = false;
         best_v = 0x7fffffff;
         for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
             float l[N];
@@ -773,12 +800,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 if (l[j] == best && best_v > v) best_v = v;
-                z += l[j] == best ? 1.f : l[j] < best ? ex2((l[j] - best) * k2e) : 0.f;
+                z += l[j] == best ? static_cast<float>(some) : l[j] < best ? exp_below(l[j] - best) : 0.f;
+                some = some || l[j] == best;
             }
         }
     }
     // the block's, from its warps'
-    const uint32_t key = best > kLowest || z > 0.f ? order_key(best) : 0u;   // (the largest counts 1: without one there is nothing above -inf)
+    const uint32_t key = some ? order_key(best) : 0u;
     uint32_t top = __reduce_max_sync(0xffffffffu, key), at = 0xffffffffu;
     if (top && key == top) {                                       // the first place that holds it
         float l[N];
@@ -788,12 +816,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
             if (l[j] == best) at = static_cast<uint32_t>(row.first + best_v * N + j);
     }
     at = __reduce_min_sync(0xffffffffu, at);
-    auto rebased = [&](float sum, uint32_t from, uint32_t to) {    // a sum of e^(l - from) as one of e^(l - to)
-        return from == to ? sum : from ? sum * ex2((key_value(from) - key_value(to)) * k2e) : 0.f;
-    };
-    z = rebased(z, key, top);
+    // The lanes' sums with what stayed out of them, `from`, as one without the largest, `to`
+    auto joined = [](float sum, uint32_t from, uint32_t to) {
+        if (from != to) sum = from ? (sum + 1.f) * exp_below(key_value(from) - key_value(to)) : 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        return to ? sum + static_cast<float>(__popc(__ballot_sync(0xffffffffu, from == to)) - 1) : 0.f;
+    };
+    z = joined(z, key, top);
     if (row.lane == 0) { sh.warp_top[row.warp] = top; sh.warp_z[row.warp] = z; sh.warp_at[row.warp] = at; }
     __syncthreads();
     const uint32_t of_warp = row.lane < kWarps ? sh.warp_top[row.lane] : 0;
@@ -822,9 +852,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         }
     }
     if (row.warp == 0) {
-        z = row.lane < kWarps ? rebased(sh.warp_z[row.lane], of_warp, top) : 0.f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        z = joined(row.lane < kWarps ? sh.warp_z[row.lane] : 0.f, of_warp, top);
         at = __reduce_min_sync(0xffffffffu, row.lane < kWarps && of_warp == top ? sh.warp_at[row.lane] : 0xffffffffu);
         if (row.lane == 0) { sh.x_best = top; sh.x_z = z; sh.x_index = at; sh.x_first = row.first; }
     }
@@ -832,11 +860,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     row.cluster.sync();
     const uint32_t of_block = row.of_rank(&sh.x_best);
     top = __reduce_max_sync(0xffffffffu, of_block);
-    z = rebased(row.of_rank(&sh.x_z), of_block, top);
-#pragma unroll
-    for (int o = 1; o < kMaxCluster; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    z = __shfl_sync(0xffffffffu, z, 0);
-    float log_z = logf(z);
+    z = joined(row.of_rank(&sh.x_z), of_block, top);
+    float log_z = log1pf(z);
     if (greedy || top == 0) {                                      // top == 0: nothing above -inf, nothing to draw
         if (row.rank == 0 && row.warp == 0) {
             at = __reduce_min_sync(0xffffffffu, of_block == top && top ? row.of_rank(&sh.x_index) : 0xffffffffu);
@@ -897,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
         row.cluster.sync();
         const u64 of_blocks = row.of_rank(&sh.x_sum);
         whole = row.sum_ranks(of_blocks);
-        if (z_is_mass) log_z = logf(static_cast<float>(static_cast<double>(whole) * (1. / (1ull << kFrac))));
+        if (z_is_mass) log_z = log1pf(static_cast<float>(static_cast<double>(whole - (1ull << kFrac)) * (1. / (1ull << kFrac))));   // (the largest weighs 2^kFrac)
         if (!use_p) {
             auto here = row.cluster.barrier_arrive();              // nothing of this block is read by others after they have got here
             row.locate_in(kept_weight, of_blocks, own_mass, aim, found);
@@ -907,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleTokens
     }
     const double share = fmax(static_cast<double>(top_p), 0.);
     if (by_estimate) {
-        if (row.estimated_cut(share, p.V, z, temp, mass, whole)) {
+        if (row.estimated_cut(share, p.V, 1.f + z, temp, mass, whole)) {
             row.locate(kept_weight, mass, aim, found);
             row.sync();
             return;

@@ -183,6 +183,34 @@ def test_sample_tokens_at_a_temperature_without_end(V):
         _check_sample(x, u, temperature=math.inf, **kw)
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("V", [7, 3000, 151936])
+def test_sample_tokens_log_probabilities_near_zero(V, dtype):
+    """A token that is almost sure: its log-probability is -log(1 + z), z the sum of the others, and keeps z's accuracy however small z is.  The weight of a
+    logit 14 below: exponents of base 2 round by 2^-20 there, 2^-20.5 of the weight, the constant log2(e) by 2^-22, the exponential by 2^-22; sums and the
+    logarithm add 2^-22: 2^-19 in all, of the result.  Without filters at T = 1 z is a sum of multiples of 2^-44, each off by up to 2^-45."""
+    B = 24
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(B, V, generator=g) * 2.5
+    margin = torch.linspace(0.25, 14.0, B)
+    second, top = torch.arange(B) % (V - 1), V - 1
+    x[::2] = -math.inf                                                  # every other row: one token beside it, margin below
+    x[torch.arange(B), second] = torch.where(torch.arange(B) % 2 == 0, 1.5, x[torch.arange(B), second])
+    x[:, top] = x[:, :top].max(1).values + margin
+    x = x.to(dtype).to(DEV)
+    u = torch.linspace(0.0, 0.999, B).to(DEV)
+    lf = x.double()
+    for kw in (dict(temperature=0.0), dict(top_k=3), dict(top_p=0.95), dict(min_p=1e-6, temperature=0.8), dict(temperature=1.3), {}):
+        tok, lp = _ops().sample_tokens(x, u, **kw)
+        _check_sample(x, u, **kw)
+        t = tok.long()[:, None]
+        rest = torch.exp(lf - lf.max(1, keepdim=True).values)
+        rest[torch.arange(B), lf.argmax(1)] = 0.0
+        want = (lf.gather(1, t) - lf.max(1, keepdim=True).values)[:, 0] - torch.log1p(rest.sum(1))
+        bound = 2.0 ** -19 * want.abs() + (V * 2.0 ** -45 if kw == {} else 0.0)
+        assert ((lp.double() - want).abs() <= bound).all(), (kw, ((lp.double() - want).abs() / bound).max())
+
+
 # ---------------------------------------------------------------------------------------------- graphs
 def _captured(f):
     graph = torch.cuda.CUDAGraph()
