@@ -25,7 +25,7 @@
 //   with the running maximum, which then bounds weight times scale.
 //
 // Measured (B200, a copy runs at 6.55 TB/s): see kStart and paged_attention_plan; 2 rows of 100 001 to 131 072 keys, 64 over 8 heads of 128, bf16
-// 169 us, 6.1 TB/s; 128 rows of 2000 to 16 384 keys, 32 over 4 heads, e4m3 204 us, 6.1 TB/s; one row of 300 keys 6.5 us, which is latency:
+// 167 us, 6.1 TB/s; 128 rows of 2000 to 16 384 keys, 32 over 4 heads, e4m3 202 us, 6.2 TB/s; one row of 300 keys 6.6 us, which is latency:
 // launch, length, page number, keys, one after the other.  A next piece requested before the warps meet, with places of their own to meet at, cost more in
 // instructions than it hid (e4m3 61 -> 71 us): three blocks an SM hide one another's starts.
 #include <cuda_bf16.h>
@@ -852,14 +852,22 @@ PagedAttentionPlan paged_attention_plan(int B, int Hq, int Hkv, int dim, int kv_
     PagedAttentionPlan plan{};
     const int G = Hq / Hkv;
     // Eight rows of a product suffice up to eight query heads a key head.  Heads of 256 stay with eight: sixteen rows of 256 outputs and queries
-    // would not fit a thread's registers.
+    // would not fit a thread's registers.  With more query heads the cache is read once for each eight: 64 over 4 heads of 256, 64 rows of 100 to 4096
+    // keys, bf16, 178 us where 8 over 4 take 94.
     plan.rows = G > 8 && dim <= 128 ? 16 : 8;
     plan.head_groups = (G + plan.rows - 1) / plan.rows;
     const int64_t pairs = static_cast<int64_t>(B) * Hkv * plan.head_groups, tiles = (max_keys + kTile - 1) / kTile;
     const int most = num_sms * (kv_type == kKvE4m3 ? blocks_per_sm<kKvE4m3>(dim, plan.rows) : blocks_per_sm<kKvBf16>(dim, plan.rows));
-    // Rows that cannot hold more than 1024 keys are not split (32 query heads over 8 key heads of 128, bf16; whole against split: 1 row of 512 / 1000
-    // keys 7.6 / 10.9 us against 10.2 / 10.3, 8 rows 8.1 / 11.3 against 11.6 / 13.1, 32 rows 11 / 25 against 16 / 30, 64 rows 30 / 50 against 30 / 50, and of
-    // 50 to 1000 keys 37.5 against 33.0, 256 rows 86 / 167 against 94 / 179).  Longer rows differ more in length, which only the split evens out.
+    // Rows that cannot hold more than 1024 keys (the table's width; nothing here knows their lengths) are not split.  32 query heads over 8 key heads of
+    // 128, bf16, us whole / split:
+    //     rows      50 to 1000 keys   512 keys      1000 keys
+    //        1       10.3 / 10.2      7.3 / 10.0    10.6 / 10.2
+    //        8       10.3 / 12.3      7.5 / 11.5    10.7 / 12.8
+    //       32       16.4 / 17.5     11.1 / 15.9    24.9 / 29.9
+    //       64       37.6 / 32.0     29.0 / 30.2    50.6 / 50.3
+    //      128       55.4 / 53.5     49.1 / 52.2    85.6 / 90.3
+    //      256       95.1 / 97.3     87.1 / 94.9   157.6 / 171.3
+    // The split wins where rows of uneven length are one or two for each block.  Longer rows differ more in length, which only the split evens out.
     plan.whole = tiles <= 16;
     plan.deep = plan.whole && pairs <= num_sms;
     const int64_t work = plan.whole ? pairs : pairs * tiles;

@@ -15,10 +15,10 @@
 //   the cut falls is found by a scan and only its tokens are ranked; a bin with too many is divided again, equal logits are counted by index.
 // * Top-p alone, where flat rows leave tens of thousands of candidates, estimates masses first and proves the cut after (estimated_cut).
 //
-// Measured (B200; fp32, vocabulary 151 936, 608 KB a row; one row, then 256 rows, which a copy would read in 24 us): greedy 13 and 73 us; T 1 without
-// filters 15 and 128; top-k 40 14 and 121; top-p 0.9 29 and 291; min-p 0.05 12 and 102; T 0.7, top-k 20, top-p 0.8, min-p 0.01 12 and 116.  One row is
+// Measured in graphs (B200; fp32, vocabulary 151 936, 608 KB a row; one row, then 256 rows, which a copy would read in 24 us): greedy 7 and 69 us; T 1
+// without filters 14 and 128; top-k 40 14 and 117; top-p 0.9 28 and 290; min-p 0.05 12 and 103; T 0.7, top-k 20, top-p 0.8, min-p 0.01 12 and 111.  One row is
 // latency: launch, loading, four or five exchanges in the cluster.  Many rows are bound by instructions (the fp64 weights, one to two passes) and by the
-// exchanges, with two blocks an SM to fill each other's pauses.  Bf16, 64 rows of 128 256: 22 us without filters, 49 with top-p.
+// exchanges, with two blocks an SM to fill each other's pauses.  Bf16, 64 rows of 128 256: 23 us without filters, 49 with top-p.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

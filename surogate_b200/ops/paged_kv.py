@@ -157,7 +157,8 @@ def paged_attention(q: torch.Tensor, kv: torch.Tensor, page_table: torch.Tensor,
     cache's type, or bf16 / fp16 with an e4m3 cache.  ``window`` > 0: only the last ``window`` tokens; ``softcap`` > 0: scores become
     ``softcap * tanh(score / softcap)`` (2^-64 to 2^64); ``sinks`` fp32 ``[query heads]``: logits that take part in the softmax's sum without a value;
     ``softmax_scale`` defaults to ``head size ** -0.5``.  Returns ``[rows, query heads, head size]`` of q's type, with ``return_lse`` also the
-    fp32 log-sum-exp of the scores ``[rows, query heads]`` (without the sinks).  A row of length 0 gives zeros and -inf."""
+    fp32 log-sum-exp of the scores ``[rows, query heads]`` (without the sinks).  A row of length 0 gives zeros and -inf; NaN and infinities in places
+    that count make outputs NaN as the formula does, those in other places are not seen.  Scales of an e4m3 cache are positive."""
     if kv.is_cuda:
         out, lse = _kernels().paged_attention(q, kv, page_table, lengths, softmax_scale, window, softcap, sinks, scales, return_lse)
     else:
