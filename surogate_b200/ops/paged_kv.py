@@ -10,8 +10,9 @@ An 8-bit cache (``float8_e4m3fn``) has one fp32 scale for each token, head and k
 * ``PagedKVCache`` keeps the pages of all layers and who owns them: ``append``, ``fork``, ``free``, ``compact``.
 
 On a GPU they run the kernels of ``csrc/paged_kv_kernels.cu`` and ``csrc/paged_attention.cu`` on the current stream, without a host
-synchronisation; elsewhere the PyTorch forms below, which are also the oracle of the kernel tests.  A page number, position or length outside
-the cache found by a kernel leaves that token out and is reported by ``check_device_errors``.
+synchronisation; elsewhere the PyTorch forms below, which are also the oracle of the kernel tests.  (Attention on a GPU reads bf16, fp16 and
+e4m3 caches with heads of 64, 128 or 256; caches of fp32 and of other head sizes can be written and copied there, and read by the caller.)
+A page number, position or length outside the cache found by a kernel leaves that token out and is reported by ``check_device_errors``.
 """
 from __future__ import annotations
 
